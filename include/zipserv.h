@@ -469,6 +469,90 @@ int zs_decode_attention_dense_paged(void* stream, const uint16_t* q, const uint1
                                     float softmax_scale, uint16_t* out, float* softmax_lse,
                                     void* workspace, size_t workspace_bytes, int num_splits);
 
+/* ---------------------------------------------------------------------- */
+/* Serving from an appendable paged bf16 cache (no counterpart in the       */
+/* reference, which is given finished caches and tables).  A pool holds     */
+/* num_blocks pages [page_block_size][num_heads_k][head_dim] for K and as   */
+/* many for V; token t of sequence b is row t % page_block_size of page     */
+/* block_table[b * table_stride + t / page_block_size], its slot that page  */
+/* times page_block_size plus the row.  Pages are a multiple of 16 tokens,  */
+/* num_blocks * page_block_size at most 2^31 - 1, head_dim 64 or 128.       */
+/* ---------------------------------------------------------------------- */
+
+/* The tables of one step, from the lengths of its requests (device int32):
+ * sequence b has context_lens[b] tokens in its pages and brings new_lens[b]
+ * more (negative: 0).  The new tokens stand one behind another, in the order of
+ * the sequences; what does not fit max_tokens is left out.  New pages come off the
+ * end of free_pages[0 .. *num_free): the g-th one that the step takes is
+ * free_pages[*num_free - 1 - g], in the order of the sequences; block_table
+ * gets them, its other entries stay.  Writes
+ *   slots, sequences, positions [max_tokens]: each new token's slot (-1 where no
+ *     page was left or the table's row is full), its sequence and its place in
+ *     it; all -1 behind the last token;
+ *   seqlens [batch]: tokens with a slot, the context's and the step's;
+ *   cu_new [batch + 1]: each sequence's first token of the step, and the end;
+ *   counts [4]: tokens asked for, pages taken, pages missing, pages left (the
+ *     *num_free of the next step).
+ * batch is at most 4096.  The outputs overlap neither each other nor the inputs. */
+int zs_paged_plan(void* stream, const int32_t* context_lens, const int32_t* new_lens, int batch,
+                  int32_t* block_table, int64_t table_stride, int max_blocks_per_seq,
+                  const int32_t* free_pages, int free_capacity, const int32_t* num_free,
+                  int page_block_size, int max_tokens, int32_t* slots, int32_t* sequences,
+                  int32_t* positions, int32_t* seqlens, int32_t* cu_new, int32_t* counts);
+
+/* New keys and values into their slots: row i of k and v ([num_tokens]
+ * [num_heads_k][head_dim], strides in elements, multiples of 8) goes to slot
+ * slots[i]; a slot outside the pool is skipped.  page_bounds (optional,
+ * [num_blocks][num_heads_k][2][head_dim] bf16) holds each page's smallest and
+ * largest key per channel: the token at offset 0 of a page starts them anew,
+ * the others widen them, NaNs are passed over.  The tokens of one page must stand
+ * next to one another, and no slot may occur twice (which token it gets is then
+ * not defined).  Pointers are 16-byte aligned. */
+int zs_paged_append(void* stream, const uint16_t* k, const uint16_t* v, int64_t k_token_stride,
+                    int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                    const int32_t* slots, int num_tokens, uint16_t* k_cache, uint16_t* v_cache,
+                    uint16_t* page_bounds, int num_blocks, int page_block_size, int num_heads_k,
+                    int head_dim);
+
+/* The pages that each query should read: for (sequence b, KV head h) the
+ * logical page p scores
+ *   max over the heads of the group of  sum_d max(q_d, 0) kmax_d + min(q_d, 0) kmin_d,
+ * the largest q.k that its bounds allow, in 64 bits (not a number: +inf; a table
+ * entry outside the pool: below all others).  The first sink_pages and the last
+ * local_pages of the sequence's ceil(len / page_block_size) pages are taken, then
+ * the largest scores, ties to the lowest page.  pages [batch][num_heads_k][top_k]
+ * gets them in ascending order, -1 behind.  sink_pages + local_pages <= top_k;
+ * at most 16 query heads a KV head, batch * num_heads_k at most 65535.  q:
+ * [batch][num_heads][head_dim], strides in elements, multiples of 8; q and
+ * page_bounds 16-byte aligned.  workspace: the queried bytes, 8-byte aligned. */
+size_t zs_select_kv_pages_workspace_bytes(int batch, int num_heads_k, int max_blocks_per_seq);
+int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_batch_stride, int64_t q_head_stride,
+                       const uint16_t* page_bounds, int num_blocks, int page_block_size,
+                       const int32_t* block_table, int64_t table_stride, int max_blocks_per_seq,
+                       const int32_t* cache_seqlens, int batch, int num_heads, int num_heads_k,
+                       int head_dim, int top_k, int sink_pages, int local_pages, int32_t* pages,
+                       void* workspace, size_t workspace_bytes);
+
+/* zs_decode_attention_dense_paged over chosen pages: head group h of sequence b
+ * attends to the tokens below cache_seqlens[b] of the logical pages
+ * pages[b][h][0 .. top_k), in any order; entries that are no page of the
+ * sequence (-1, or past its length) count for nothing, a page listed twice
+ * counts twice.  A row without tokens gives zeros and softmax_lse -inf.
+ * num_splits = 0 picks the splits of the lists; the workspace (16-byte aligned)
+ * is what the query says for the same arguments. */
+size_t zs_decode_attention_sparse_workspace_bytes(int batch, int num_heads, int num_heads_k,
+                                                  int head_dim, int top_k, int page_block_size,
+                                                  int num_splits);
+int zs_decode_attention_sparse_paged(void* stream, const uint16_t* q, int64_t q_batch_stride,
+                                     int64_t q_head_stride, const uint16_t* k_cache,
+                                     const uint16_t* v_cache, int num_blocks, int page_block_size,
+                                     const int32_t* block_table, int64_t table_stride,
+                                     int max_blocks_per_seq, const int32_t* pages, int top_k,
+                                     const int32_t* cache_seqlens, int batch, int num_heads,
+                                     int num_heads_k, int head_dim, float softmax_scale,
+                                     uint16_t* out, float* softmax_lse, void* workspace,
+                                     size_t workspace_bytes, int num_splits);
+
 /* Stage profiler of the re-tiled record pipeline
  * (kernel_benchmark/zipserv_tile_stage_bench_ext.cu measure_zipserv_tile_stages):
  * one wave consumes records record0 + i*stride (mod num_records), waiting

@@ -107,6 +107,19 @@ SIGNATURES = {
     "zs_decode_attention_dense_paged": (
         C.c_int, [_p, _p, _p, _p, _p, C.c_int, C.c_int, C.c_int, _p, C.c_int, C.c_int, C.c_int,
                   C.c_int, C.c_int, C.c_float, _p, _p, _p, C.c_size_t, C.c_int]),
+    "zs_paged_plan": (
+        C.c_int, [_p, _p, _p, C.c_int, _p, _i64, C.c_int, _p, C.c_int, _p, C.c_int, C.c_int] + [_p] * 6),
+    "zs_paged_append": (
+        C.c_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, C.c_int, _p, _p, _p, C.c_int, C.c_int, C.c_int,
+                  C.c_int]),
+    "zs_select_kv_pages_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "zs_select_kv_pages": (
+        C.c_int, [_p, _p, _i64, _i64, _p, C.c_int, C.c_int, _p, _i64, C.c_int, _p, C.c_int, C.c_int, C.c_int,
+                  C.c_int, C.c_int, C.c_int, C.c_int, _p, _p, C.c_size_t]),
+    "zs_decode_attention_sparse_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
+    "zs_decode_attention_sparse_paged": (
+        C.c_int, [_p, _p, _i64, _i64, _p, _p, C.c_int, C.c_int, _p, _i64, C.c_int, _p, C.c_int, _p, C.c_int,
+                  C.c_int, C.c_int, C.c_int, C.c_float, _p, _p, _p, C.c_size_t, C.c_int]),
     "zs_measure_record_stages": (
         C.c_int, [_p, _p, _p, _p, C.c_uint8, C.c_int, C.c_int, _i64, _i64, C.c_int, C.c_int,
                   _p, _p, _p]),

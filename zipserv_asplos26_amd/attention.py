@@ -14,7 +14,7 @@ import ctypes
 import math
 from typing import Optional
 
-from . import _lib
+from . import _lib, paged
 from ._lib import check, lib
 from .codec import (ZipservRetiled, _check_cuda, _dptr, _stream, _torch, compress, compress_retiled,
                     compress_retiled_kv)
@@ -350,6 +350,50 @@ def _dense_paged(q3, shape, k_cache, v_cache, block_table, cache_seqlens, softma
         _stream(), _dptr(q3), _dptr(kc), _dptr(vc), _dptr(bt),
         maxb, nblocks, page, _dptr(sl), cap, B, H, Hkv, D, scale, _dptr(out), _dptr(lse),
         _dptr(ws), ws.numel(), int(num_splits)))
+    out = out.view(shape)
+    return (out, lse) if return_softmax_lse else out
+
+
+def flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cache_seqlens,
+                                   softmax_scale: Optional[float] = None, num_splits: int = 0,
+                                   return_softmax_lse: bool = False):
+    """Decode attention over chosen pages of a paged cache: each KV head's
+    queries attend to the tokens below cache_seqlens (int32 [B] or an int) in the
+    logical pages that `pages` (B, Hkv, top_k) int32 lists, as
+    `paged.select_kv_pages` gives them or in any other order.  Entries that are no
+    page of the sequence (-1, or past its length) count for nothing, a page listed
+    twice counts twice.  q: (B, 1, H, D) or (B, H, D) bf16, possibly a slice of a
+    fused projection's output; k_cache / v_cache: pages (num_blocks,
+    page_block_size, Hkv, D), head_dim 64 or 128, page_block_size a multiple of
+    16.  Returns out shaped like q (and softmax_lse [B, H] when asked); a row
+    without tokens gives zeros and lse -inf."""
+    torch = _torch()
+    shape = q.shape
+    q3 = q[:, 0] if q.dim() == 4 and q.shape[1] == 1 else q
+    paged._check(q3, "q", torch.bfloat16, (None,) * 3, contiguous=False)
+    B, H, D = q3.shape
+    device = q3.device
+    paged._check(k_cache, "k_cache", torch.bfloat16, (None, None, None, D), device)
+    paged._check(v_cache, "v_cache", torch.bfloat16, k_cache.shape, device)
+    nblocks, page, Hkv, _ = k_cache.shape
+    table = paged._table(block_table, B, device)
+    paged._check(pages, "pages", torch.int32, (B, Hkv, None), device)
+    top_k = pages.shape[2]
+    if Hkv == 0 or H % Hkv:
+        raise ValueError(f"{H} query heads do not share {Hkv} KV heads evenly")
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    with paged._device_of(q3):
+        lens = paged._lengths(cache_seqlens, B, device)
+        q3 = paged._rows(q3)
+        out = torch.empty((B, H, D), dtype=torch.bfloat16, device=device)
+        lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_softmax_lse else None
+        L = lib()
+        wsb = int(L.zs_decode_attention_sparse_workspace_bytes(B, H, Hkv, D, top_k, page, num_splits))
+        ws = torch.empty(wsb, dtype=torch.uint8, device=device) if wsb else None
+        check("zs_decode_attention_sparse_paged", L.zs_decode_attention_sparse_paged(
+            _stream(), q3.data_ptr(), q3.stride(0), q3.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), nblocks,
+            page, table.data_ptr(), table.stride(0), table.shape[1], pages.data_ptr(), top_k, lens.data_ptr(), B, H,
+            Hkv, D, scale, out.data_ptr(), _dptr(lse), _dptr(ws), wsb, int(num_splits)))
     out = out.view(shape)
     return (out, lse) if return_softmax_lse else out
 

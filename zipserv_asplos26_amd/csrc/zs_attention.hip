@@ -205,43 +205,6 @@ __device__ __forceinline__ void build_e1(uint4* e1, int start_exp, int tid, int 
   }
 }
 
-// Max / sum over lanes l, l^16, l^32, l^48 (the four row groups), in every
-// lane: v_permlane16_swap of x with itself leaves rows (0, 0, 2, 2) and
-// (1, 1, 3, 3) of x, v_permlane32_swap rows (0, 1, 0, 1) and (2, 3, 2, 3) --
-// vector instructions instead of the LDS permutes that a shuffle compiles to
-// (token-major kernel 61.3 -> 56.9 us on a ragged batch of 201 MB, head-major
-// 81.5 -> 80.0 us on 398 MB).
-__device__ __forceinline__ void row_swap16(float x, float& a, float& b) {
-  const uint32_t u = __float_as_uint(x);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  a = __uint_as_float(r[0]);
-  b = __uint_as_float(r[1]);
-}
-__device__ __forceinline__ void row_swap32(float x, float& a, float& b) {
-  const uint32_t u = __float_as_uint(x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  a = __uint_as_float(r[0]);
-  b = __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float wave_max16(float x) {
-  float a, b;
-  row_swap16(x, a, b);
-  row_swap32(fmaxf(a, b), a, b);
-  return fmaxf(a, b);
-}
-__device__ __forceinline__ float wave_sum16(float x) {
-  float a, b;
-  row_swap16(x, a, b);
-  row_swap32(a + b, a, b);
-  return a + b;
-}
-
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
-}
-
 // Per-wave attention state over one (batch, KV head, token range): the q^T
 // fragments (B operand, lane l -> head l%16 of the group, dims 32c +
 // 8*(l/16)..+7), the O^T accumulators (lane l: head l%16, dims 16*i +

@@ -1,0 +1,194 @@
+"""An appendable paged KV cache: the tables of a step, new keys and values, and
+the pages that a query should read.
+
+A pool of pages holds keys and values of all sequences, (num_blocks,
+page_block_size, Hkv, D) bf16 each, as `attention.flash_attn_with_kvcache_dense`
+reads them with a block table.  One decode or prefill step is
+
+    plan = plan_paged_step(seqlens, new_lens, block_table, free_pages, num_free, page, max_tokens)
+    for every layer:
+        append_paged_kv(k, v, k_cache, v_cache, plan.slots, page_bounds)
+        pages = select_kv_pages(q, page_bounds, block_table, plan.seqlens, page, top_k)
+        out = attention.flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, plan.seqlens)
+
+and the next one goes on with `plan.seqlens` and `plan.num_free`.  Nothing waits
+for the GPU, so a step can be captured into a HIP graph; every call has its own
+outputs and workspace.
+"""
+from __future__ import annotations
+
+import contextlib
+from dataclasses import dataclass
+
+from ._lib import check, lib
+from .codec import _dptr, _stream, _torch
+
+_here = contextlib.nullcontext()
+
+
+def _device_of(t):
+    """A context in which t's device is the current one, whose current stream
+    the call goes to."""
+    cuda = _torch().cuda
+    return _here if t.device.index == cuda.current_device() else cuda.device(t.device)
+
+
+def _check(t, name, dtype, shape, device=None, contiguous=True):
+    """`shape`: the sizes asked for, None where any will do."""
+    torch = _torch()
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("*" if n is None else str(n) for n in shape)
+        raise ValueError(f"{name} must be ({want}), got {tuple(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _rows(t):
+    """t (rows, heads, dim) as the kernels take it: 16-byte pieces of contiguous
+    heads at any stride between rows and heads (a slice of a fused projection is
+    one), a copy otherwise."""
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or s0 % 8 or s1 % 8 or t.data_ptr() % 16:
+        return t.clone(memory_format=_torch().contiguous_format)
+    return t
+
+
+def _table(block_table, batch, device):
+    _check(block_table, "block_table", _torch().int32, (batch, None), device, contiguous=False)
+    inner, width = block_table.stride(1), block_table.shape[1]
+    apart = block_table.stride(0) >= width and (inner == 1 or width == 1)
+    return block_table if apart else block_table.contiguous()
+
+
+@dataclass
+class PagedPlan:
+    """One step's tables (all int32 on the GPU)."""
+    slots: object       # [max_tokens] slot of each new token, -1 without one
+    sequences: object   # [max_tokens] its sequence, -1 behind the last token
+    positions: object   # [max_tokens] its place in the sequence, -1 behind the last
+    seqlens: object     # [batch] cached tokens after the step
+    cu_new: object      # [batch + 1] each sequence's first token of the step
+    counts: object      # [4] tokens asked for, pages taken, missing, left
+
+    @property
+    def num_free(self):
+        """Free pages after the step, [1]: what the next step takes."""
+        return self.counts[3:]
+
+
+def plan_paged_step(context_lens, new_lens, block_table, free_pages, num_free, page_block_size: int,
+                    max_tokens: int) -> PagedPlan:
+    """The tables of one step from its requests' lengths, on the GPU: sequence b
+    has context_lens[b] tokens in its pages and brings new_lens[b] more (int32
+    [B], B <= 4096).  New pages come off the end of free_pages[:num_free] (int32,
+    num_free [1]) in the order of the sequences and are entered into block_table
+    (B, max_blocks) in place.  max_tokens is the size of the step's buffers: new
+    tokens past it are left out, entries behind the last one are -1.
+
+    Where pages run out (or a row of the table is full) the tokens that would
+    need them get slot -1, and seqlens and counts say so: counts[0] against
+    cu_new[-1] shows tokens left out, counts[2] the pages missing."""
+    torch = _torch()
+    _check(context_lens, "context_lens", torch.int32, (None,))
+    device, batch = context_lens.device, context_lens.shape[0]
+    _check(new_lens, "new_lens", torch.int32, (batch,), device)
+    _check(block_table, "block_table", torch.int32, (batch, None), device, contiguous=False)
+    width = block_table.shape[1]
+    stride = block_table.stride(0) if batch > 1 else width
+    if (block_table.stride(1) != 1 and width > 1) or stride < width:
+        raise ValueError("block_table is written in place: its rows must be contiguous and apart")
+    _check(free_pages, "free_pages", torch.int32, (None,), device)
+    _check(num_free, "num_free", torch.int32, (1,), device)
+    page, most = int(page_block_size), int(max_tokens)
+    if most < 0:
+        raise ValueError("max_tokens must not be negative")
+    with _device_of(context_lens):
+        out = torch.empty(3 * most + 2 * batch + 5, dtype=torch.int32, device=device)
+        plan = PagedPlan(*out.split([most, most, most, batch, batch + 1, 4]))
+        at = out.data_ptr()
+        check("zs_paged_plan", lib().zs_paged_plan(
+            _stream(), context_lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), stride, width,
+            free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), page, most, at, at + 4 * most,
+            at + 8 * most, at + 12 * most, at + 12 * most + 4 * batch, at + 12 * most + 8 * batch + 4))
+    return plan
+
+
+def append_paged_kv(k, v, k_cache, v_cache, slots, page_bounds=None) -> None:
+    """New keys and values (tokens, Hkv, D) bf16 into their slots (int32
+    [tokens], `PagedPlan.slots`; slots outside the pool are skipped).  k and v may
+    be slices of a fused projection's output.  page_bounds (num_blocks, Hkv, 2,
+    D) bf16, if given, is brought up to date: the smallest and the largest key of
+    each channel in the pages written to, NaNs passed over; a page's bounds start
+    anew with the token at its offset 0, so they need no first fill.  The tokens
+    of one page stand next to one another, as a plan puts them, and no slot
+    occurs twice."""
+    torch = _torch()
+    _check(k_cache, "k_cache", torch.bfloat16, (None,) * 4)
+    device = k_cache.device
+    blocks, page, heads_k, dim = k_cache.shape
+    _check(v_cache, "v_cache", torch.bfloat16, k_cache.shape, device)
+    _check(slots, "slots", torch.int32, (None,), device)
+    n = slots.shape[0]
+    _check(k, "k", torch.bfloat16, (n, heads_k, dim), device, contiguous=False)
+    _check(v, "v", torch.bfloat16, (n, heads_k, dim), device, contiguous=False)
+    if page_bounds is not None:
+        _check(page_bounds, "page_bounds", torch.bfloat16, (blocks, heads_k, 2, dim), device)
+    with _device_of(k_cache):
+        k, v = _rows(k), _rows(v)
+        check("zs_paged_append", lib().zs_paged_append(
+            _stream(), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            slots.data_ptr(), n, k_cache.data_ptr(), v_cache.data_ptr(), _dptr(page_bounds), blocks, page, heads_k,
+            dim))
+
+
+def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size: int, top_k: int,
+                    sink_pages: int = 1, local_pages: int = 1):
+    """The pages that each query's attention should read: (B, Hkv, top_k) int32
+    logical pages in ascending order, -1 behind.  q: (B, 1, H, D) or (B, H, D)
+    bf16; page_bounds as `append_paged_kv` keeps them; cache_seqlens: int32 [B] or
+    an int.
+
+    A page scores the largest q.k that its bounds allow, the most over the heads
+    that share the KV head (in 64 bits, so the selection is the definition's;
+    scores that are no number count as +inf).  The first sink_pages and the last
+    local_pages of a sequence are always taken, the others by score, ties to the
+    lowest page; sequences of at most top_k pages keep them all."""
+    torch = _torch()
+    if isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[1] == 1:
+        q = q[:, 0]
+    _check(q, "q", torch.bfloat16, (None,) * 3, contiguous=False)
+    batch, heads, dim = q.shape
+    device = q.device
+    _check(page_bounds, "page_bounds", torch.bfloat16, (None, None, 2, dim), device)
+    blocks, heads_k = page_bounds.shape[:2]
+    table = _table(block_table, batch, device)
+    width, page, top_k = table.shape[1], int(page_block_size), int(top_k)
+    if top_k <= 0 or sink_pages < 0 or local_pages < 0 or sink_pages + local_pages > top_k:
+        raise ValueError("top_k must be positive and hold sink_pages and local_pages")
+    if heads_k == 0 or heads % heads_k:
+        raise ValueError(f"{heads} query heads do not share {heads_k} KV heads evenly")
+    with _device_of(q):
+        lens = _lengths(cache_seqlens, batch, device)
+        q = _rows(q)
+        pages = torch.empty((batch, heads_k, top_k), dtype=torch.int32, device=device)
+        need = int(lib().zs_select_kv_pages_workspace_bytes(batch, heads_k, width))
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        check("zs_select_kv_pages", lib().zs_select_kv_pages(
+            _stream(), q.data_ptr(), q.stride(0), q.stride(1), page_bounds.data_ptr(), blocks, page,
+            table.data_ptr(), table.stride(0), width, lens.data_ptr(), batch, heads, heads_k, dim, top_k,
+            int(sink_pages), int(local_pages), pages.data_ptr(), ws.data_ptr(), need))
+    return pages
+
+
+def _lengths(cache_seqlens, batch, device):
+    torch = _torch()
+    if isinstance(cache_seqlens, int):
+        return torch.full((batch,), cache_seqlens, dtype=torch.int32, device=device)
+    _check(cache_seqlens, "cache_seqlens", torch.int32, (batch,), device)
+    return cache_seqlens
