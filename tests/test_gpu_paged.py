@@ -296,21 +296,70 @@ def test_select_near_ties(torch_cuda):
     check_select(T, q, bounds, table, [3200, 3111], 16, 50, sink_pages=0, local_pages=0)
 
 
-def test_select_long_sequence(torch_cuda):
-    # more pages than a workgroup has threads many times over; the scores by torch, in 64 bits
-    T = torch_cuda
-    heads, heads_k, dim, page, width, top_k = 8, 2, 128, 16, 40000, 700
-    g = T.Generator(device="cuda").manual_seed(2)
-    q = T.randn(1, heads, dim, device="cuda", generator=g).to(T.bfloat16)
-    bounds = T.randn(width, heads_k, 2, dim, device="cuda", generator=g).sort(2).values.to(T.bfloat16)
-    table = T.randperm(width, device="cuda", generator=g).to(T.int32).view(1, width)
-    got = paged.select_kv_pages(q, bounds, table, width * page - 3, page, top_k)
-    b = bounds[table[0].long()].double()
+def check_select_many(T, q, bounds, table, length, page, top_k, sink=1, local=1):
+    """One sequence of many pages: the scores by torch, in 64 bits, sorted with ties to the lowest page."""
+    got = paged.select_kv_pages(q, bounds, table, length, page, top_k, sink, local)
+    n, heads_k = -(-length // page), bounds.shape[1]
+    b = bounds[table[0, :n].long()].double()
+    group = q.shape[1] // heads_k
     for h in range(heads_k):
-        x = q[0, 4 * h:4 * h + 4].double()
-        s = (b[:, h, 1] @ x.clamp(min=0).t().contiguous() + b[:, h, 0] @ x.clamp(max=0).t().contiguous()).amax(1)
-        s[0] = s[-1] = float("inf")
-        assert T.equal(got[0, h].long(), s.topk(top_k).indices.sort().values)
+        x = q[0, group * h:group * h + group].double()
+        s = ((b[:, None, h, 1] * x.clamp(min=0)).sum(2) + (b[:, None, h, 0] * x.clamp(max=0)).sum(2)).amax(1)
+        s = s.masked_fill(s.isnan(), float("inf"))
+        index = T.arange(n, device="cuda")
+        order = T.argsort(s, descending=True, stable=True)
+        forced = (index < sink) | (index >= n - local)
+        take = T.cat([index[forced], order[~forced[order]][: top_k - sink - local]]).sort().values
+        assert T.equal(got[0, h].long(), take)
+
+
+@pytest.mark.parametrize("width,top_k", [(2048, 100), (2049, 1000), (8192, 8191), (8200, 64), (40000, 700),
+                                         (65536, 300), (70001, 5000), (140000, 64)])
+def test_select_long_sequence(torch_cuda, width, top_k):
+    # more pages than a workgroup holds in registers, and than one bit map of them
+    T = torch_cuda
+    g = T.Generator(device="cuda").manual_seed(width)
+    q = T.randn(1, 8, 128, device="cuda", generator=g).to(T.bfloat16)
+    bounds = T.randn(width, 2, 2, 128, device="cuda", generator=g).sort(2).values.to(T.bfloat16)
+    table = T.randperm(width, device="cuda", generator=g).to(T.int32).view(1, width)
+    for sink, local in ((1, 1), (0, 0), (3, 61)):
+        check_select_many(T, q, bounds, table, width * 16 - 3, 16, top_k, sink, local)
+
+
+@pytest.mark.parametrize("kind", ["equal", "few values", "crowd and one far", "two crowds", "one page far below",
+                                  "large", "nearly equal", "stranger"])
+@pytest.mark.parametrize("width,top_k", [(1500, 400), (5000, 90), (70000, 9000)])
+def test_select_score_distributions(torch_cuda, kind, width, top_k):
+    # the scores themselves, as the first channel of bounds that are 0 elsewhere: crowds that a first look cannot
+    # part, scores that fp32 cannot tell from each other, values past what its error is known for
+    T = torch_cuda
+    g = T.Generator(device="cuda").manual_seed(5)
+    q = T.zeros(1, 2, 64, dtype=T.bfloat16, device="cuda")
+    q[..., :4] = T.tensor([1.0, 1.0, 2.0 ** -20, 1.0])
+    bounds = T.zeros(width, 1, 2, 64, dtype=T.bfloat16, device="cuda")
+    x = T.rand(width, device="cuda", generator=g)
+    if kind == "equal":
+        x.fill_(0.5)
+    elif kind == "few values":
+        x = (4 * x).floor()
+    elif kind == "crowd and one far":
+        x[width // 2] = 300.0
+    elif kind == "two crowds":
+        x[:top_k - 7] += 1e6
+    elif kind == "one page far below":
+        x[width // 3] = -1e7
+    elif kind == "large":
+        x *= 1e30
+    elif kind == "nearly equal":
+        bounds[:, 0, 1, 2] = x.to(T.bfloat16)  # 2^-20 of it counts
+        x.fill_(0.75)
+    bounds[:, 0, 1, 0] = x.to(T.bfloat16)
+    bounds[:, 0, 1, 1] = (x - bounds[:, 0, 1, 0].float()).to(T.bfloat16)  # 16 bits of x in all
+    if kind == "stranger":
+        bounds[width // 2, 0, 1, 3] = float("nan")
+    table = T.randperm(width, device="cuda", generator=g).to(T.int32).view(1, width)
+    check_select_many(T, q, bounds, table, width * 16, 16, top_k)
+    check_select_many(T, q, bounds, table, width * 16, 16, top_k, 0, 0)
 
 
 @pytest.mark.parametrize("how", ["row", "heads", "offset", "four"])

@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "../../include/zipserv.h"
 #include "zs_device.hpp"
@@ -254,12 +255,25 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendParams p) 
 // Selection
 // ---------------------------------------------------------------------------
 // score[b][h][p] = max over the group's heads of sum_d max(q_d, 0) kmax_d +
-// min(q_d, 0) kmin_d, the largest q.k that the bounds of page p allow.  In 64
-// bits: products of two bf16 are exact there and a sum is off by 2^-53, so the
-// answer is the definition's and not a rounding's.  As 2 score = sum_d q_d (kmax
-// + kmin) + |q_d| (kmax - kmin), which needs q once.  NaN (a bound or a query
-// that is not finite) counts as +inf.  Keys are the scores' bits in an order of
-// unsigned numbers; pages that are always taken have the largest key.
+// min(q_d, 0) kmin_d, the largest q.k that the bounds of page p allow, with NaN
+// as +inf.  The selection is the one of the exact scores:
+//
+// score_kernel computes them in fp32 on the matrix cores, with a bound of their
+// error.  A product of two bf16 is exact there, and the 2D additions are off by
+// 2^-22 of the sum of the products' sizes at most (a rounded one by 2^-24; the
+// allowance covers sums aligned and cut inside the instruction), so a score is
+// off by less than E = kScoreError * sum |terms|.  The sum of sizes is a second
+// product, of the same operands without their signs.
+// pick_kernel finds a narrow window that holds the top_k-th largest fp32 score,
+// 2 E wider on both sides: scores above it are taken and scores below it are not,
+// whatever their errors.  What lies in it, a few pages, is scored again in 64 bits
+// and ranked, ties to the lowest page.  Rows where that cannot be told from a
+// bound (scores or operands so large that products or sums leave fp32's range,
+// values that are no numbers, hundreds of equal scores) are scored in 64 bits as a
+// whole.
+//
+// In 64 bits: 2 score = sum_d q_d (kmax + kmin) + |q_d| (kmax - kmin), each sum
+// off by 2^-53.
 struct SelectParams {
   const uint16_t* q;
   int64_t q_batch, q_head;  // strides in elements
@@ -268,7 +282,7 @@ struct SelectParams {
   int64_t table_stride;
   const int32_t* seqlens;
   int32_t* pages;           // [B][Hkv][top_k]
-  uint64_t* keys;           // [B][Hkv][width]
+  float2* scores;           // [B][Hkv][width]: the fp32 score and the sum of its terms' sizes
   int num_blocks, width, page, batch, heads_k, group, top_k, sink, local;
 };
 
@@ -277,132 +291,438 @@ __device__ __forceinline__ int select_pages(const SelectParams& p, int b) {
   return min(len / p.page + (len % p.page != 0), p.width);
 }
 
-__device__ __forceinline__ uint64_t select_key(double x) {
-  if (x != x) x = INFINITY;
+// 2 D 2^-22 of the sizes, rounded up (D = 128), and an absolute rest for operands
+// and products below the normal range, which an instruction may take as 0.
+constexpr float kScoreError = 1.02f / (1 << 14), kScoreRest = 0x1p-50f;
+constexpr uint32_t kScoreLarge = 0x5D80;  // 2^60 in bf16: from there on the rest is no bound
+
+constexpr int kScoreWaves = 4;
+constexpr int kScoreTiles = 4;  // 16-page tiles of a wave
+
+// max over the 16 lanes of a row, in all of them
+__device__ __forceinline__ float row_max16(float x) {
+  auto step = [&](auto ctrl) {
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, 0xF, 0xF,
+                                                             false)));
+  };
+  step(std::integral_constant<int, 0x128>{});  // row_ror:8
+  step(std::integral_constant<int, 0x124>{});
+  step(std::integral_constant<int, 0x122>{});
+  step(std::integral_constant<int, 0x121>{});
+  return x;
+}
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
+template <int D>
+__global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p) {
+  constexpr int kC = D / 32;
+  const int b = blockIdx.y / p.heads_k, h = blockIdx.y % p.heads_k;
+  const int n = select_pages(p, b);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l & 15, lg = l >> 4;
+  const int p0 = (blockIdx.x * kScoreWaves + w) * 16 * kScoreTiles;
+  if (n <= p.top_k || p0 >= n) return;
+  // lane i: the place of the wave's i-th page, -1 without one
+  int block = -1;
+  if (l < 16 * kScoreTiles && p0 + l < n) block = p.table[b * p.table_stride + p0 + l];
+  if (block >= p.num_blocks) block = -1;
+  // the B operands (lane l: head l%16, dims 32c + 8*(l/16)..+7): q's positive and
+  // negative parts
+  u32x4 qp[kC], qn[kC];
+  uint32_t large = 0;
+  const uint16_t* qrow = p.q + b * p.q_batch + (h * p.group + (g < p.group ? g : 0)) * p.q_head + 8 * lg;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(qrow + 32 * c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t neg = ((x[i] >> 15) & 0x00010001u) * 0xFFFFu;
+      qp[c][i] = x[i] & ~neg;
+      qn[c][i] = x[i] & neg;
+      large = max_u16x2(large, x[i] & 0x7FFF7FFFu);
+    }
+  }
+  auto is_large = [](uint32_t x) { return (x & 0xFFFFu) >= kScoreLarge || x >> 16 >= kScoreLarge; };
+  const bool large_q = __builtin_amdgcn_ballot_w64(is_large(large));
+  const uint32_t no_sign = 0x7FFF7FFFu;
+  float2* out = p.scores + (int64_t)blockIdx.y * p.width + p0;
+#pragma unroll
+  for (int t = 0; t < kScoreTiles; ++t) {
+    if (p0 + 16 * t >= n) break;  // (uniform)
+    const int mine = __shfl(block, 16 * t + g);
+    const uint16_t* lo = p.bounds + ((int64_t)max(mine, 0) * p.heads_k + h) * 2 * D + 8 * lg;
+    u32x4 x[kC], y[kC];
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      x[c] = *reinterpret_cast<const u32x4*>(lo + 32 * c);
+      y[c] = *reinterpret_cast<const u32x4*>(lo + D + 32 * c);
+    }
+    f32x4 S = {0.f, 0.f, 0.f, 0.f}, A = {0.f, 0.f, 0.f, 0.f};
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c]), as_bf16x8(qn[c]), S, 0, 0, 0);
+      S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c]), as_bf16x8(qp[c]), S, 0, 0, 0);
+      u32x4 an;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[c][i] &= no_sign;
+        y[c][i] &= no_sign;
+        an[i] = qn[c][i] & no_sign;
+        most = max_u16x2(most, max_u16x2(x[c][i], y[c][i]));
+      }
+      A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c]), as_bf16x8(an), A, 0, 0, 0);
+      A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c]), as_bf16x8(qp[c]), A, 0, 0, 0);
+    }
+    // lane l: head l%16, pages 4*(l/16)..+3 of S and A
+    uint64_t wide = __builtin_amdgcn_ballot_w64(is_large(most));  // of page l%16, in each of its four lanes
+    wide |= wide >> 32;
+    wide |= wide >> 16;
+    float s = 0.f, a = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float sr = row_max16(S[r]), ar = row_max16(A[r]);
+      if (g == r) s = sr, a = ar;
+    }
+    const int at = 4 * lg + (g & 3);  // the page whose score lanes with g < 4 have now
+    const bool gone = __shfl(block, 16 * t + at) < 0;
+    // an infinite sum of sizes says that the score is not to be gone by
+    if (large_q || gone || (wide >> at & 1)) a = INFINITY;
+    if (g < 4 && p0 + 16 * t + at < n) out[16 * t + at] = float2{s, a};
+  }
+}
+
+// The exact score of page lp as a number in its order: NaN as +inf, a page
+// outside the pool 0.  For the 16 (8) lanes of a page together.
+__device__ __forceinline__ uint64_t score_key(double x) {
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);  // -0 is 0
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
-constexpr int kScoreThreads = 256;
-
 template <int D>
-__global__ __launch_bounds__(kScoreThreads) void score_kernel(SelectParams p) {
-  constexpr int kLanes = D / 8, kPages = kScoreThreads / kLanes;
-  const int b = blockIdx.y / p.heads_k, h = blockIdx.y % p.heads_k;
-  const int n = select_pages(p, b);
-  const int lp = blockIdx.x * kPages + threadIdx.x / kLanes, c = threadIdx.x % kLanes;
-  if (n <= p.top_k || lp >= n) return;  // (all lanes of a page alike)
-  uint64_t key = ~0ull;
-  if (lp >= p.sink && lp < n - p.local) {
-    const int block = p.table[b * p.table_stride + lp];
-    double best = -INFINITY;
-    bool odd = true;
-    if (block >= 0 && block < p.num_blocks) {
-      const uint16_t* lo = p.bounds + ((int64_t)block * p.heads_k + h) * 2 * D + 8 * c;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(lo), y = *reinterpret_cast<const u32x4*>(lo + D);
-      double mid[8], wide[8];
+__device__ __forceinline__ uint64_t exact_key(const SelectParams& p, int b, int h, int lp, int c) {
+  constexpr int kLanes = D / 8;
+  const int block = p.table[b * p.table_stride + lp];
+  if (block < 0 || block >= p.num_blocks) return 0;
+  const uint16_t* lo = p.bounds + ((int64_t)block * p.heads_k + h) * 2 * D + 8 * c;
+  const u32x4 x = *reinterpret_cast<const u32x4*>(lo), y = *reinterpret_cast<const u32x4*>(lo + D);
+  double mid[8], wide[8], best = -INFINITY;
+  bool odd = false;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double k0 = bf16_bits_to_f32(i & 1 ? x[i / 2] >> 16 : x[i / 2] & 0xFFFF);
-        const double k1 = bf16_bits_to_f32(i & 1 ? y[i / 2] >> 16 : y[i / 2] & 0xFFFF);
-        mid[i] = k1 + k0;
-        wide[i] = k1 - k0;
-      }
-      odd = false;
-      for (int g = 0; g < p.group; ++g) {
-        const u32x4 u = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head + 8 * c);
-        double s = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const double q = bf16_bits_to_f32(i & 1 ? u[i / 2] >> 16 : u[i / 2] & 0xFFFF);
-          s = fma(q, mid[i], s);
-          s = fma(fabs(q), wide[i], s);
-        }
-#pragma unroll
-        for (int off = 1; off < kLanes; off <<= 1) s += __shfl_xor(s, off);
-        odd |= s != s;
-        best = fmax(best, s);
-      }
-    }
-    key = min(select_key(odd ? INFINITY : best), ~0ull - 1);
-    if (block < 0 || block >= p.num_blocks) key = 0;  // no such page: taken last
+  for (int i = 0; i < 8; ++i) {
+    const double k0 = bf16_bits_to_f32(i & 1 ? x[i / 2] >> 16 : x[i / 2] & 0xFFFF);
+    const double k1 = bf16_bits_to_f32(i & 1 ? y[i / 2] >> 16 : y[i / 2] & 0xFFFF);
+    mid[i] = k1 + k0;
+    wide[i] = k1 - k0;
   }
-  if (c == 0) p.keys[(int64_t)blockIdx.y * p.width + lp] = key;
+  for (int g = 0; g < p.group; ++g) {
+    const u32x4 u = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head + 8 * c);
+    double s = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double q = bf16_bits_to_f32(i & 1 ? u[i / 2] >> 16 : u[i / 2] & 0xFFFF);
+      s = fma(q, mid[i], s);
+      s = fma(fabs(q), wide[i], s);
+    }
+#pragma unroll
+    for (int off = 1; off < kLanes; off <<= 1) s += __shfl_xor(s, off);
+    odd |= s != s;
+    best = fmax(best, s);
+  }
+  return score_key(odd ? INFINITY : best);
 }
 
-// The top_k largest keys of one (sequence, KV head), ties to the lowest page, in
-// ascending order: the key of the last one taken digit by digit, 8 bits at a
-// time from the top, until the pages of a digit are all taken or none is left.
-constexpr int kPickThreads = 256;
+// One workgroup a (sequence, KV head).  The scores stay in registers up to
+// kPickKeys a thread and are read again past that.
+constexpr int kPickKeys = 8;
+constexpr int kPickBins = 2048;
+constexpr int kPickFew = 256;      // pages of the window that are ranked among themselves
+constexpr int kPickChunk = 65536;  // pages of a bit map
 
-__global__ __launch_bounds__(kPickThreads) void pick_kernel(SelectParams p) {
-  __shared__ int hist[256];
-  __shared__ int wave_sum[2][kPickThreads / 64];
-  __shared__ int s_bin, s_above, s_in;
-  const int row = blockIdx.x, b = row / p.heads_k, tid = threadIdx.x;
-  const int n = select_pages(p, b);
-  int32_t* out = p.pages + (int64_t)row * p.top_k;
-  if (n <= p.top_k) {
-    for (int i = tid; i < p.top_k; i += kPickThreads) out[i] = i < n ? i : -1;
-    return;
+template <int NT>
+struct PickLds {
+  union {
+    int hist[kPickBins];
+    struct {
+      uint64_t key[kPickFew];
+      int page[kPickFew];
+    } few;
+    uint64_t map[kPickChunk / 64];
+  };
+  float red[3][NT / 64];
+  int sum[NT / 64];
+  int bin, above, in, count;
+};
+
+// Writes the pages of [c0, c0 + kPickChunk) whose bits are set, in order, from
+// place `base` of the list on; returns the next place.
+template <int NT>
+__device__ __forceinline__ int pick_write(PickLds<NT>& L, int32_t* out, int base, int c0, int n) {
+  const int words = (min(n - c0, kPickChunk) + 63) / 64, tid = threadIdx.x, w = tid >> 6, l = lane_id();
+  for (int i0 = 0; i0 < words; i0 += NT) {
+    const uint64_t m = i0 + tid < words ? L.map[i0 + tid] : 0;
+    const int incl = wave_inclusive_scan(__builtin_popcountll(m));
+    __syncthreads();  // the last round's sums are read
+    if (l == 63) L.sum[w] = incl;
+    __syncthreads();
+    int at = base + incl - __builtin_popcountll(m);
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+      if (i < w) at += L.sum[i];
+      base += L.sum[i];
+    }
+    for (uint64_t rest = m; rest; rest &= rest - 1) out[at++] = c0 + 64 * (i0 + tid) + __builtin_ctzll(rest);
   }
-  const uint64_t* keys = p.keys + (int64_t)row * p.width;
+  __syncthreads();
+  return base;
+}
+
+// All of a row in 64 bits: the key of the last page taken found digit by digit,
+// 8 bits at a time from the top, until a digit's pages are all taken or none is left.
+template <int D, int NT>
+__device__ void pick_exact(const SelectParams& p, PickLds<NT>& L, int b, int h, int n, uint64_t* keys, int32_t* out) {
+  constexpr int kLanes = D / 8;
+  const int tid = threadIdx.x, l = lane_id(), w = tid >> 6;
+  for (int lp = tid / kLanes; lp < n; lp += NT / kLanes) {
+    const uint64_t k = lp < p.sink || lp >= n - p.local ? ~0ull : exact_key<D>(p, b, h, lp, tid % kLanes);
+    if (tid % kLanes == 0) keys[lp] = k;
+  }
+  __threadfence_block();
+  __syncthreads();
   uint64_t prefix = 0;  // of the keys' bits from `shift` on
   int need = p.top_k, shift = 64;
   while (shift > 0) {
     shift -= 8;
-    hist[tid] = 0;
+    for (int i = tid; i < 256; i += NT) L.hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kPickThreads) {
+    for (int i = tid; i < n; i += NT) {
       const uint64_t k = keys[i];
-      if (shift == 56 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      if (shift == 56 || (k >> (shift + 8)) == prefix) atomicAdd(&L.hist[(k >> shift) & 255], 1);
     }
     __syncthreads();
     if (tid < 64) {  // four digits a lane, the largest first
       int v[4], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += v[i] = hist[255 - 4 * tid - i];
+      for (int i = 0; i < 4; ++i) sum += v[i] = L.hist[255 - 4 * tid - i];
       int above = wave_inclusive_scan(sum) - sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (above < need && above + v[i] >= need) {
-          s_bin = 255 - 4 * tid - i;
-          s_above = above;
-          s_in = v[i];
+          L.bin = 255 - 4 * tid - i;
+          L.above = above;
+          L.in = v[i];
         }
         above += v[i];
       }
     }
     __syncthreads();
-    prefix = prefix << 8 | (uint64_t)s_bin;
-    need -= s_above;
-    if (s_in == need) break;  // (uniform)
+    prefix = prefix << 8 | (uint64_t)L.bin;
+    need -= L.above;
+    if (L.in == need) break;  // (uniform)
   }
   // keys above `prefix` are taken, and the first `need` equal to it
-  int at = 0, equal = 0;
-  const int w = tid >> 6, l = lane_id();
-  for (int i0 = 0; i0 < n; i0 += kPickThreads) {
-    const int i = i0 + tid;
-    const uint64_t k = i < n ? keys[i] >> shift : 0;
-    const bool is = i < n && k == prefix;
-    const uint64_t eq = __builtin_amdgcn_ballot_w64(is);
-    if (l == 0) wave_sum[0][w] = __builtin_popcountll(eq);
+  int base = 0, equal = 0;
+  for (int c0 = 0; c0 < n; c0 += kPickChunk) {
     __syncthreads();
-    int rank = equal + __builtin_popcountll(eq & ((1ull << l) - 1));
-    for (int j = 0; j < kPickThreads / 64; ++j) {
-      if (j < w) rank += wave_sum[0][j];
-      equal += wave_sum[0][j];
+    for (int i0 = c0; i0 < min(n, c0 + kPickChunk); i0 += NT) {
+      const int i = i0 + tid;
+      const uint64_t k = i < n ? keys[i] >> shift : 0;
+      const bool is = i < n && k == prefix;
+      const uint64_t eq = __builtin_amdgcn_ballot_w64(is);
+      __syncthreads();
+      if (l == 0) L.sum[w] = __builtin_popcountll(eq);
+      __syncthreads();
+      int rank = equal + __builtin_popcountll(eq & ((1ull << l) - 1));
+      for (int j = 0; j < NT / 64; ++j) {
+        if (j < w) rank += L.sum[j];
+        equal += L.sum[j];
+      }
+      const uint64_t take = __builtin_amdgcn_ballot_w64(i < n && (k > prefix || (is && rank < need)));
+      if (l == 0 && i < n) L.map[(i - c0) / 64] = take;
     }
-    const bool take = i < n && (k > prefix || (is && rank < need));
-    const uint64_t tk = __builtin_amdgcn_ballot_w64(take);
-    if (l == 0) wave_sum[1][w] = __builtin_popcountll(tk);
     __syncthreads();
-    int place = at + __builtin_popcountll(tk & ((1ull << l) - 1));
-    for (int j = 0; j < kPickThreads / 64; ++j) {
-      if (j < w) place += wave_sum[1][j];
-      at += wave_sum[1][j];
+    base = pick_write<NT>(L, out, base, c0, n);
+  }
+}
+
+template <int D, int NT>
+__global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
+  __shared__ PickLds<NT> L;
+  const int row = blockIdx.x, b = row / p.heads_k, h = row % p.heads_k, tid = threadIdx.x, w = tid >> 6, l = lane_id();
+  const int n = select_pages(p, b);
+  int32_t* out = p.pages + (int64_t)row * p.top_k;
+  if (n <= p.top_k) {
+    for (int i = tid; i < p.top_k; i += NT) out[i] = i < n ? i : -1;
+    return;
+  }
+  float2* scores = p.scores + (int64_t)row * p.width;
+  const int first = p.sink, last = n - p.local;  // the pages between are chosen from
+  float key[kPickKeys];
+  float low = INFINITY, high = -INFINITY, size = 0.f;
+  auto note = [&](float2 x) {
+    low = fminf(low, x.x);
+    high = fmaxf(high, x.x);
+    size = fmaxf(size, x.y);
+  };
+#pragma unroll
+  for (int j = 0; j < kPickKeys; ++j) {
+    const int i = j * NT + tid;
+    if (i >= first && i < last) {
+      const float2 x = scores[i];
+      key[j] = x.x;
+      note(x);
     }
-    if (take) out[place] = i;
+  }
+  for (int i = kPickKeys * NT + tid; i < last; i += NT)
+    if (i >= first) note(scores[i]);
+  auto each = [&](auto f) {  // f(page, its score) over the pages to choose from
+#pragma unroll
+    for (int j = 0; j < kPickKeys; ++j) {
+      const int i = j * NT + tid;
+      if (i >= first && i < last) f(i, key[j]);
+    }
+    for (int i = kPickKeys * NT + tid; i < last; i += NT)
+      if (i >= first) f(i, scores[i].x);
+  };
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    low = fminf(low, __shfl_xor(low, off));
+    high = fmaxf(high, __shfl_xor(high, off));
+    size = fmaxf(size, __shfl_xor(size, off));
+  }
+  if (l == 0) L.red[0][w] = low, L.red[1][w] = high, L.red[2][w] = size;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) {
+    low = fminf(low, L.red[0][i]);
+    high = fmaxf(high, L.red[1][i]);
+    size = fmaxf(size, L.red[2][i]);
+  }
+  int need = p.top_k - p.sink - p.local;
+  const float margin = 3 * (kScoreError * size + kScoreRest);
+  bool exact = !(size < INFINITY);
+  // The window [low, high] that holds the need-th largest score, and how many
+  // pages lie above it: a histogram over it, then the digit that holds the score.
+  int in = INT_MAX;
+  if (need > 0 && !exact) {
+    int above = 0;  // the window's need-th largest is the (above + need)-th of all
+    for (int round = 0; round < 3; ++round) {
+      for (int i = tid; i < kPickBins; i += NT) L.hist[i] = 0;
+      __syncthreads();
+      const float scale = high > low ? kPickBins / (high - low) : 0.f;
+      auto bin = [&](float x) { return min((int)((x - low) * scale), kPickBins - 1); };
+      each([&](int, float x) {
+        if (x >= low && x <= high) atomicAdd(&L.hist[bin(x)], 1);
+      });
+      __syncthreads();
+      constexpr int kPer = kPickBins / NT;  // digits a thread, the largest first
+      int v[kPer], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sum += v[i] = L.hist[kPickBins - 1 - kPer * tid - i];
+      const int incl = wave_inclusive_scan(sum);
+      if (l == 63) L.sum[w] = incl;
+      __syncthreads();
+      int over = incl - sum;
+#pragma unroll
+      for (int i = 0; i < NT / 64; ++i)
+        if (i < w) over += L.sum[i];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (over < need && over + v[i] >= need) L.bin = kPickBins - 1 - kPer * tid - i;
+        over += v[i];
+      }
+      if (tid == 0) L.above = L.in = 0;
+      __syncthreads();
+      const float step = scale > 0.f ? 1.f / scale : high - low;
+      const float lo = fmaxf(low, low + L.bin * step - margin), hi = fminf(high, low + (L.bin + 1) * step + margin);
+      int na = 0, ni = 0;
+      each([&](int, float x) {
+        na += x > hi && x <= high;
+        ni += x >= lo && x <= hi;
+      });
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) {
+        na += __shfl_xor(na, off);
+        ni += __shfl_xor(ni, off);
+      }
+      if (l == 0) {
+        atomicAdd(&L.above, na);
+        atomicAdd(&L.in, ni);
+      }
+      __syncthreads();
+      above += L.above;
+      need -= L.above;
+      in = L.in;
+      const bool same = !(hi - lo < 0.5f * (high - low));
+      low = lo;
+      high = hi;
+      if (in <= kPickFew || same) break;  // (uniform)
+      __syncthreads();
+    }
+    exact = in > kPickFew && in != need;
+  }
+  if (exact) {  // (uniform)
+    __syncthreads();
+    pick_exact<D, NT>(p, L, b, h, n, reinterpret_cast<uint64_t*>(scores), out);
+    return;
+  }
+  // The window's pages: all of them, or the best `need` by their exact scores.
+  const bool all = need > 0 && in == need;
+  uint64_t mine = 0;
+  int page = -1;
+  if (need > 0 && !all) {
+    __syncthreads();
+    if (tid == 0) L.count = 0;
+    __syncthreads();
+    each([&](int i, float x) {
+      if (x >= low && x <= high) L.few.page[atomicAdd(&L.count, 1)] = i;
+    });
+    __syncthreads();
+    constexpr int kLanes = D / 8;
+    for (int i = tid / kLanes; i < in; i += NT / kLanes) {
+      const uint64_t k = exact_key<D>(p, b, h, L.few.page[i], tid % kLanes);
+      if (tid % kLanes == 0) L.few.key[i] = k;
+    }
+    __syncthreads();
+    if (tid < in) {
+      mine = L.few.key[tid];
+      page = L.few.page[tid];
+      int rank = 0;
+      for (int i = 0; i < in; ++i) {
+        const uint64_t k = L.few.key[i];
+        rank += k > mine || (k == mine && L.few.page[i] < page);
+      }
+      if (rank >= need) page = -1;
+    }
+  }
+  int base = 0;
+  for (int c0 = 0; c0 < n; c0 += kPickChunk) {
+    __syncthreads();
+    auto take = [&](int i, float x) {
+      return i < n && (i < first || i >= last || x > high || (all && x >= low));
+    };
+    const int end = min(n, c0 + kPickChunk);
+    if (c0 == 0) {
+#pragma unroll
+      for (int j = 0; j < kPickKeys; ++j) {
+        const int i = j * NT + tid;
+        const uint64_t m = __builtin_amdgcn_ballot_w64(take(i, key[j]));
+        if (l == 0 && i < n) L.map[i / 64] = m;
+      }
+    }
+    for (int i0 = c0 == 0 ? kPickKeys * NT : c0; i0 < end; i0 += NT) {
+      const int i = i0 + tid;
+      const float x = i >= first && i < last ? scores[i].x : 0.f;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(take(i, x));
+      if (l == 0 && i < n) L.map[(i - c0) / 64] = m;
+    }
+    __syncthreads();
+    if (page >= c0 && page < end) atomicOr((unsigned long long*)&L.map[(page - c0) / 64], 1ull << (page & 63));
+    __syncthreads();
+    base = pick_write<NT>(L, out, base, c0, n);
   }
 }
 
@@ -498,7 +818,7 @@ extern "C" int zs_paged_append(void* stream, const uint16_t* k, const uint16_t* 
 
 extern "C" size_t zs_select_kv_pages_workspace_bytes(int batch, int num_heads_k, int max_blocks_per_seq) {
   if (batch <= 0 || num_heads_k <= 0 || max_blocks_per_seq <= 0) return 0;
-  return (size_t)batch * num_heads_k * max_blocks_per_seq * sizeof(uint64_t);
+  return (size_t)batch * num_heads_k * max_blocks_per_seq * sizeof(float2);
 }
 
 extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_batch_stride, int64_t q_head_stride,
@@ -527,7 +847,7 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   p.table_stride = table_stride;
   p.seqlens = cache_seqlens;
   p.pages = pages;
-  p.keys = static_cast<uint64_t*>(workspace);
+  p.scores = static_cast<float2*>(workspace);
   p.num_blocks = num_blocks;
   p.width = max_blocks_per_seq;
   p.page = page_block_size;
@@ -538,17 +858,23 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   p.sink = sink_pages;
   p.local = local_pages;
   const hipStream_t st = (hipStream_t)stream;
-  if (max_blocks_per_seq > top_k) {
-    const int per = kScoreThreads * 8 / head_dim;
-    const dim3 grid((unsigned)(((int64_t)max_blocks_per_seq + per - 1) / per), batch * num_heads_k);
-    if (head_dim == 128)
-      hipLaunchKernelGGL(score_kernel<128>, grid, dim3(kScoreThreads), 0, st, p);
+  auto launch = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    if (max_blocks_per_seq > top_k) {
+      constexpr int kPages = 16 * kScoreTiles * kScoreWaves;
+      const dim3 grid((unsigned)(((int64_t)max_blocks_per_seq + kPages - 1) / kPages), batch * num_heads_k);
+      hipLaunchKernelGGL(score_kernel<D>, grid, dim3(kScoreWaves * 64), 0, st, p);
+    }
+    const dim3 rows(batch * num_heads_k);
+    if (max_blocks_per_seq <= kPickKeys * 256)
+      hipLaunchKernelGGL((pick_kernel<D, 256>), rows, dim3(256), 0, st, p);
     else
-      hipLaunchKernelGGL(score_kernel<64>, grid, dim3(kScoreThreads), 0, st, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-  }
-  hipLaunchKernelGGL(pick_kernel, dim3(batch * num_heads_k), dim3(kPickThreads), 0, st, p);
+      hipLaunchKernelGGL((pick_kernel<D, 1024>), rows, dim3(1024), 0, st, p);
+  };
+  if (head_dim == 128)
+    launch(std::integral_constant<int, 128>{});
+  else
+    launch(std::integral_constant<int, 64>{});
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? ZS_OK : (int)e;
 }
