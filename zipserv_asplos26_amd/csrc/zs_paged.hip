@@ -348,17 +348,35 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p)
   auto is_large = [](uint32_t x) { return (x & 0xFFFFu) >= kScoreLarge || x >> 16 >= kScoreLarge; };
   const bool large_q = __builtin_amdgcn_ballot_w64(is_large(large));
   const uint32_t no_sign = 0x7FFF7FFFu;
+  // A page's bounds, 4 D bytes, come as whole rows (an instruction reads 1 KB of
+  // them) and pass through the wave's own LDS into operand order.
+  constexpr int kRow = 4 * D, kPitch = kRow + 16, kRows = 1024 / kRow, kLoads = 2 * kC;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kScoreWaves][16 * kPitch];
+  uint8_t* lds = smem[w];
+  const int lrow = l / (kRow / 16), lcol = 16 * (l % (kRow / 16));
+  const uint8_t* from = reinterpret_cast<const uint8_t*>(p.bounds) + (int64_t)h * kRow + lcol;
+  u32x4 next[kLoads];
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int from_block = max(__shfl(block, 16 * t + i * kRows + lrow), 0);
+      next[i] = *reinterpret_cast<const u32x4*>(from + (int64_t)from_block * p.heads_k * kRow);
+    }
+  };
+  fetch(0);
   float2* out = p.scores + (int64_t)blockIdx.y * p.width + p0;
 #pragma unroll
   for (int t = 0; t < kScoreTiles; ++t) {
     if (p0 + 16 * t >= n) break;  // (uniform)
-    const int mine = __shfl(block, 16 * t + g);
-    const uint16_t* lo = p.bounds + ((int64_t)max(mine, 0) * p.heads_k + h) * 2 * D + 8 * lg;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      *reinterpret_cast<u32x4*>(lds + (i * kRows + lrow) * kPitch + lcol) = next[i];
+    if (t + 1 < kScoreTiles && p0 + 16 * (t + 1) < n) fetch(t + 1);
     u32x4 x[kC], y[kC];
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      x[c] = *reinterpret_cast<const u32x4*>(lo + 32 * c);
-      y[c] = *reinterpret_cast<const u32x4*>(lo + D + 32 * c);
+      x[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c);
+      y[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c + 2 * D);
     }
     f32x4 S = {0.f, 0.f, 0.f, 0.f}, A = {0.f, 0.f, 0.f, 0.f};
     uint32_t most = 0;
@@ -395,44 +413,32 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p)
   }
 }
 
-// The exact score of page lp as a number in its order: NaN as +inf, a page
-// outside the pool 0.  For the 16 (8) lanes of a page together.
+// The exact score of page lp for one head as a number in its order: NaN as +inf,
+// a page outside the pool 0.  For the D / 8 lanes of a page together.
 __device__ __forceinline__ uint64_t score_key(double x) {
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);  // -0 is 0
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
 template <int D>
-__device__ __forceinline__ uint64_t exact_key(const SelectParams& p, int b, int h, int lp, int c) {
+__device__ __forceinline__ uint64_t exact_key(const SelectParams& p, int b, int h, int g, int lp, int c) {
   constexpr int kLanes = D / 8;
+  const u32x4 u = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head + 8 * c);
   const int block = p.table[b * p.table_stride + lp];
   if (block < 0 || block >= p.num_blocks) return 0;
   const uint16_t* lo = p.bounds + ((int64_t)block * p.heads_k + h) * 2 * D + 8 * c;
   const u32x4 x = *reinterpret_cast<const u32x4*>(lo), y = *reinterpret_cast<const u32x4*>(lo + D);
-  double mid[8], wide[8], best = -INFINITY;
-  bool odd = false;
+  double s = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const double k0 = bf16_bits_to_f32(i & 1 ? x[i / 2] >> 16 : x[i / 2] & 0xFFFF);
-    const double k1 = bf16_bits_to_f32(i & 1 ? y[i / 2] >> 16 : y[i / 2] & 0xFFFF);
-    mid[i] = k1 + k0;
-    wide[i] = k1 - k0;
+    auto at = [&](const u32x4& v) -> double { return bf16_bits_to_f32(i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xFFFF); };
+    const double q = at(u), k0 = at(x), k1 = at(y);
+    s = fma(q, k1 + k0, s);
+    s = fma(fabs(q), k1 - k0, s);
   }
-  for (int g = 0; g < p.group; ++g) {
-    const u32x4 u = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head + 8 * c);
-    double s = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double q = bf16_bits_to_f32(i & 1 ? u[i / 2] >> 16 : u[i / 2] & 0xFFFF);
-      s = fma(q, mid[i], s);
-      s = fma(fabs(q), wide[i], s);
-    }
-#pragma unroll
-    for (int off = 1; off < kLanes; off <<= 1) s += __shfl_xor(s, off);
-    odd |= s != s;
-    best = fmax(best, s);
-  }
-  return score_key(odd ? INFINITY : best);
+  for (int off = 1; off < kLanes; off <<= 1) s += __shfl_xor(s, off);
+  return score_key(s != s ? INFINITY : s);
 }
 
 // One workgroup a (sequence, KV head).  The scores stay in registers up to
@@ -487,7 +493,9 @@ __device__ void pick_exact(const SelectParams& p, PickLds<NT>& L, int b, int h, 
   constexpr int kLanes = D / 8;
   const int tid = threadIdx.x, l = lane_id(), w = tid >> 6;
   for (int lp = tid / kLanes; lp < n; lp += NT / kLanes) {
-    const uint64_t k = lp < p.sink || lp >= n - p.local ? ~0ull : exact_key<D>(p, b, h, lp, tid % kLanes);
+    uint64_t k = lp < p.sink || lp >= n - p.local ? ~0ull : 0;
+    if (k == 0)
+      for (int g = 0; g < p.group; ++g) k = max(k, exact_key<D>(p, b, h, g, lp, tid % kLanes));
     if (tid % kLanes == 0) keys[lp] = k;
   }
   __threadfence_block();
@@ -678,13 +686,18 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     if (tid == 0) L.count = 0;
     __syncthreads();
     each([&](int i, float x) {
-      if (x >= low && x <= high) L.few.page[atomicAdd(&L.count, 1)] = i;
+      if (x >= low && x <= high) {
+        const int at = atomicAdd(&L.count, 1);
+        L.few.page[at] = i;
+        L.few.key[at] = 0;
+      }
     });
     __syncthreads();
-    constexpr int kLanes = D / 8;
-    for (int i = tid / kLanes; i < in; i += NT / kLanes) {
-      const uint64_t k = exact_key<D>(p, b, h, L.few.page[i], tid % kLanes);
-      if (tid % kLanes == 0) L.few.key[i] = k;
+    constexpr int kLanes = D / 8;  // of a page and a head
+    for (int i = tid / kLanes; i < in * p.group; i += NT / kLanes) {
+      const int at = i / p.group;
+      const uint64_t k = exact_key<D>(p, b, h, i - at * p.group, L.few.page[at], tid % kLanes);
+      if (tid % kLanes == 0) atomicMax((unsigned long long*)&L.few.key[at], k);
     }
     __syncthreads();
     if (tid < in) {
