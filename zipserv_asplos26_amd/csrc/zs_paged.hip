@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -296,8 +297,11 @@ __device__ __forceinline__ int select_pages(const SelectParams& p, int b) {
 constexpr float kScoreError = 1.02f / (1 << 14), kScoreRest = 0x1p-50f;
 constexpr uint32_t kScoreLarge = 0x5D80;  // 2^60 in bf16: from there on the rest is no bound
 
+// A wave scores 16 pages for one KV head.  The heads of the same pages run next to
+// one another, so a page's bounds are read from memory as one piece (32 sequences
+// to 64000 tokens, 64 / 8 heads, 271 MB: selection 81.5 -> 71.3 us; with 16 pages a
+// wave in place of 64 69.5, one sequence of 32000 tokens 17.0 -> 12.7).
 constexpr int kScoreWaves = 4;
-constexpr int kScoreTiles = 4;  // 16-page tiles of a wave
 
 // max over the 16 lanes of a row, in all of them
 __device__ __forceinline__ float row_max16(float x) {
@@ -320,34 +324,17 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
 template <int D>
 __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p) {
   constexpr int kC = D / 32;
-  const int b = blockIdx.y / p.heads_k, h = blockIdx.y % p.heads_k;
+  const int b = blockIdx.y;
   const int n = select_pages(p, b);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l & 15, lg = l >> 4;
-  const int p0 = (blockIdx.x * kScoreWaves + w) * 16 * kScoreTiles;
+  const int64_t item = (int64_t)blockIdx.x * kScoreWaves + w;
+  const int h = (int)(item % p.heads_k);
+  const int64_t p0 = item / p.heads_k * 16;
   if (n <= p.top_k || p0 >= n) return;
-  // lane i: the place of the wave's i-th page, -1 without one
+  // lane i: the place of the wave's page i%16, -1 without one
   int block = -1;
-  if (l < 16 * kScoreTiles && p0 + l < n) block = p.table[b * p.table_stride + p0 + l];
+  if (p0 + g < n) block = p.table[b * p.table_stride + p0 + g];
   if (block >= p.num_blocks) block = -1;
-  // the B operands (lane l: head l%16, dims 32c + 8*(l/16)..+7): q's positive and
-  // negative parts
-  u32x4 qp[kC], qn[kC];
-  uint32_t large = 0;
-  const uint16_t* qrow = p.q + b * p.q_batch + (h * p.group + (g < p.group ? g : 0)) * p.q_head + 8 * lg;
-#pragma unroll
-  for (int c = 0; c < kC; ++c) {
-    const u32x4 x = *reinterpret_cast<const u32x4*>(qrow + 32 * c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t neg = ((x[i] >> 15) & 0x00010001u) * 0xFFFFu;
-      qp[c][i] = x[i] & ~neg;
-      qn[c][i] = x[i] & neg;
-      large = max_u16x2(large, x[i] & 0x7FFF7FFFu);
-    }
-  }
-  auto is_large = [](uint32_t x) { return (x & 0xFFFFu) >= kScoreLarge || x >> 16 >= kScoreLarge; };
-  const bool large_q = __builtin_amdgcn_ballot_w64(is_large(large));
-  const uint32_t no_sign = 0x7FFF7FFFu;
   // A page's bounds, 4 D bytes, come as whole rows (an instruction reads 1 KB of
   // them) and pass through the wave's own LDS into operand order.
   constexpr int kRow = 4 * D, kPitch = kRow + 16, kRows = 1024 / kRow, kLoads = 2 * kC;
@@ -355,62 +342,68 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p)
   uint8_t* lds = smem[w];
   const int lrow = l / (kRow / 16), lcol = 16 * (l % (kRow / 16));
   const uint8_t* from = reinterpret_cast<const uint8_t*>(p.bounds) + (int64_t)h * kRow + lcol;
-  u32x4 next[kLoads];
-  auto fetch = [&](int t) {
+  u32x4 x[kC], y[kC], in[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int from_block = max(__shfl(block, 16 * t + i * kRows + lrow), 0);
-      next[i] = *reinterpret_cast<const u32x4*>(from + (int64_t)from_block * p.heads_k * kRow);
+  for (int i = 0; i < kLoads; ++i)
+    in[i] = *reinterpret_cast<const u32x4*>(from + (int64_t)max(__shfl(block, i * kRows + lrow), 0) * p.heads_k * kRow);
+  // the B operands (lane l: head l%16, dims 32c + 8*(l/16)..+7): q's positive and
+  // negative parts
+  u32x4 qp[kC], qn[kC];
+  uint32_t most = 0;
+  const uint16_t* qrow = p.q + b * p.q_batch + (h * p.group + (g < p.group ? g : 0)) * p.q_head + 8 * lg;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const u32x4 q = *reinterpret_cast<const u32x4*>(qrow + 32 * c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t neg = ((q[i] >> 15) & 0x00010001u) * 0xFFFFu;
+      qp[c][i] = q[i] & ~neg;
+      qn[c][i] = q[i] & neg;
+      most = max_u16x2(most, q[i] & 0x7FFF7FFFu);
     }
-  };
-  fetch(0);
-  float2* out = p.scores + (int64_t)blockIdx.y * p.width + p0;
-#pragma unroll
-  for (int t = 0; t < kScoreTiles; ++t) {
-    if (p0 + 16 * t >= n) break;  // (uniform)
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      *reinterpret_cast<u32x4*>(lds + (i * kRows + lrow) * kPitch + lcol) = next[i];
-    if (t + 1 < kScoreTiles && p0 + 16 * (t + 1) < n) fetch(t + 1);
-    u32x4 x[kC], y[kC];
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      x[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c);
-      y[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c + 2 * D);
-    }
-    f32x4 S = {0.f, 0.f, 0.f, 0.f}, A = {0.f, 0.f, 0.f, 0.f};
-    uint32_t most = 0;
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c]), as_bf16x8(qn[c]), S, 0, 0, 0);
-      S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c]), as_bf16x8(qp[c]), S, 0, 0, 0);
-      u32x4 an;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[c][i] &= no_sign;
-        y[c][i] &= no_sign;
-        an[i] = qn[c][i] & no_sign;
-        most = max_u16x2(most, max_u16x2(x[c][i], y[c][i]));
-      }
-      A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c]), as_bf16x8(an), A, 0, 0, 0);
-      A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c]), as_bf16x8(qp[c]), A, 0, 0, 0);
-    }
-    // lane l: head l%16, pages 4*(l/16)..+3 of S and A
-    uint64_t wide = __builtin_amdgcn_ballot_w64(is_large(most));  // of page l%16, in each of its four lanes
-    wide |= wide >> 32;
-    wide |= wide >> 16;
-    float s = 0.f, a = 0.f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float sr = row_max16(S[r]), ar = row_max16(A[r]);
-      if (g == r) s = sr, a = ar;
-    }
-    const int at = 4 * lg + (g & 3);  // the page whose score lanes with g < 4 have now
-    const bool gone = __shfl(block, 16 * t + at) < 0;
-    // an infinite sum of sizes says that the score is not to be gone by
-    if (large_q || gone || (wide >> at & 1)) a = INFINITY;
-    if (g < 4 && p0 + 16 * t + at < n) out[16 * t + at] = float2{s, a};
   }
+  auto is_large = [](uint32_t v) { return (v & 0xFFFFu) >= kScoreLarge || v >> 16 >= kScoreLarge; };
+  const bool large_q = __builtin_amdgcn_ballot_w64(is_large(most));
+  const uint32_t no_sign = 0x7FFF7FFFu;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(lds + (i * kRows + lrow) * kPitch + lcol) = in[i];
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    x[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c);
+    y[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c + 2 * D);
+  }
+  f32x4 S = {0.f, 0.f, 0.f, 0.f}, A = {0.f, 0.f, 0.f, 0.f};
+  most = 0;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c]), as_bf16x8(qn[c]), S, 0, 0, 0);
+    S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c]), as_bf16x8(qp[c]), S, 0, 0, 0);
+    u32x4 an;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[c][i] &= no_sign;
+      y[c][i] &= no_sign;
+      an[i] = qn[c][i] & no_sign;
+      most = max_u16x2(most, max_u16x2(x[c][i], y[c][i]));
+    }
+    A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c]), as_bf16x8(an), A, 0, 0, 0);
+    A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c]), as_bf16x8(qp[c]), A, 0, 0, 0);
+  }
+  // lane l: head l%16, pages 4*(l/16)..+3 of S and A
+  uint64_t wide = __builtin_amdgcn_ballot_w64(is_large(most));  // of page l%16, in each of its four lanes
+  wide |= wide >> 32;
+  wide |= wide >> 16;
+  float s = 0.f, a = 0.f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float sr = row_max16(S[r]), ar = row_max16(A[r]);
+    if (g == r) s = sr, a = ar;
+  }
+  const int at = 4 * lg + (g & 3);  // the page whose score lanes with g < 4 have now
+  const bool gone = __shfl(block, at) < 0;
+  // an infinite sum of sizes says that the score is not to be gone by
+  if (large_q || gone || (wide >> at & 1)) a = INFINITY;
+  if (g < 4 && p0 + at < n) p.scores[((int64_t)b * p.heads_k + h) * p.width + p0 + at] = float2{s, a};
 }
 
 // The exact score of page lp for one head as a number in its order: NaN as +inf,
@@ -441,48 +434,50 @@ __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, int b, int 
   return score_key(s != s ? INFINITY : s);
 }
 
-// One workgroup a (sequence, KV head).  The scores stay in registers up to
-// kPickKeys a thread and are read again past that.
+// One workgroup a (sequence, KV head).  What it takes is a chain of short steps, each
+// ended by a barrier: so scores are loaded before the row's length is known and stay
+// in registers (kPickKeys a thread; the rest of longer rows is read again), sums
+// and maxima run over DPP and ballots, and one pass does all that goes by the window.
 constexpr int kPickKeys = 8;
 constexpr int kPickBins = 2048;
 constexpr int kPickFew = 256;      // pages of the window that are ranked among themselves
 constexpr int kPickChunk = 65536;  // pages of a bit map
 
+__device__ __forceinline__ float wave_max(float x) { return wave_max16(row_max16(x)); }
+
 template <int NT>
 struct PickLds {
   union {
     int hist[kPickBins];
-    struct {
-      uint64_t key[kPickFew];
-      int page[kPickFew];
-    } few;
     uint64_t map[kPickChunk / 64];
   };
-  float red[3][NT / 64];
+  uint64_t few_key[kPickFew];
+  int few_page[kPickFew];
+  float red[3][16];
   int sum[NT / 64];
   int bin, above, in, count;
+  float low, high;
 };
 
 // Writes the pages of [c0, c0 + kPickChunk) whose bits are set, in order, from
 // place `base` of the list on; returns the next place.
 template <int NT>
 __device__ __forceinline__ int pick_write(PickLds<NT>& L, int32_t* out, int base, int c0, int n) {
-  const int words = (min(n - c0, kPickChunk) + 63) / 64, tid = threadIdx.x, w = tid >> 6, l = lane_id();
+  const int words = (min(n - c0, kPickChunk) + 63) / 64, tid = threadIdx.x, l = lane_id();
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll 1
   for (int i0 = 0; i0 < words; i0 += NT) {
-    const uint64_t m = i0 + tid < words ? L.map[i0 + tid] : 0;
+    uint64_t m = i0 + tid < words ? L.map[i0 + tid] : 0;
     const int incl = wave_inclusive_scan(__builtin_popcountll(m));
-    __syncthreads();  // the last round's sums are read
     if (l == 63) L.sum[w] = incl;
     __syncthreads();
-    int at = base + incl - __builtin_popcountll(m);
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) {
-      if (i < w) at += L.sum[i];
-      base += L.sum[i];
-    }
-    for (uint64_t rest = m; rest; rest &= rest - 1) out[at++] = c0 + 64 * (i0 + tid) + __builtin_ctzll(rest);
+    const int s = l < NT / 64 ? L.sum[l] : 0;
+    const int upto = wave_inclusive_scan(s);
+    int at = base + incl - __builtin_popcountll(m) + __builtin_amdgcn_readlane(upto - s, w);
+    base += __builtin_amdgcn_readlane(upto, 63);
+    for (; m; m &= m - 1) out[at++] = c0 + 64 * (i0 + tid) + __builtin_ctzll(m);
+    __syncthreads();  // the sums and the map are read
   }
-  __syncthreads();
   return base;
 }
 
@@ -558,181 +553,196 @@ __device__ void pick_exact(const SelectParams& p, PickLds<NT>& L, int b, int h, 
 
 template <int D, int NT>
 __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
+  constexpr int kWaves = NT / 64;
   __shared__ PickLds<NT> L;
-  const int row = blockIdx.x, b = row / p.heads_k, h = row % p.heads_k, tid = threadIdx.x, w = tid >> 6, l = lane_id();
+  const int row = blockIdx.x, b = row / p.heads_k, h = row % p.heads_k, tid = threadIdx.x, l = lane_id();
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  float2* scores = p.scores + (int64_t)row * p.width;
+  float2 own[kPickKeys];
+#pragma unroll
+  for (int j = 0; j < kPickKeys; ++j)  // (what lies behind the row's end is not looked at)
+    own[j] = j * NT + tid < p.width ? scores[j * NT + tid] : float2{0.f, 0.f};
   const int n = select_pages(p, b);
   int32_t* out = p.pages + (int64_t)row * p.top_k;
   if (n <= p.top_k) {
     for (int i = tid; i < p.top_k; i += NT) out[i] = i < n ? i : -1;
     return;
   }
-  float2* scores = p.scores + (int64_t)row * p.width;
   const int first = p.sink, last = n - p.local;  // the pages between are chosen from
-  float key[kPickKeys];
-  float low = INFINITY, high = -INFINITY, size = 0.f;
-  auto note = [&](float2 x) {
-    low = fminf(low, x.x);
-    high = fmaxf(high, x.x);
-    size = fmaxf(size, x.y);
-  };
+  const int need = p.top_k - p.sink - p.local;
+  const bool whole = n <= kPickKeys * NT;
+  // A page's score: NaN for one that is always taken, -inf behind the last one.
+  auto marked = [&](int i, float x) { return i >= first && i < last ? x : i < n ? NAN : -INFINITY; };
+  float key[kPickKeys], size = 0.f;
 #pragma unroll
   for (int j = 0; j < kPickKeys; ++j) {
     const int i = j * NT + tid;
-    if (i >= first && i < last) {
-      const float2 x = scores[i];
-      key[j] = x.x;
-      note(x);
-    }
+    key[j] = marked(i, own[j].x);
+    size = fmaxf(size, i >= first && i < last ? own[j].y : 0.f);
   }
-  for (int i = kPickKeys * NT + tid; i < last; i += NT)
-    if (i >= first) note(scores[i]);
-  auto each = [&](auto f) {  // f(page, its score) over the pages to choose from
+  if (!whole)
+    for (int i = kPickKeys * NT + tid; i < last; i += NT) size = fmaxf(size, i >= first ? scores[i].y : 0.f);
+  size = wave_max(size);
+  if (l == 0) L.red[2][w] = size;
+  auto each = [&](auto f) {
 #pragma unroll
-    for (int j = 0; j < kPickKeys; ++j) {
-      const int i = j * NT + tid;
-      if (i >= first && i < last) f(i, key[j]);
-    }
-    for (int i = kPickKeys * NT + tid; i < last; i += NT)
-      if (i >= first) f(i, scores[i].x);
+    for (int j = 0; j < kPickKeys; ++j) f(key[j]);
+    if (!whole)
+      for (int i = kPickKeys * NT + tid; i < n; i += NT) f(marked(i, scores[i].x));
   };
+
+  // The window [low, high] that holds the need-th largest score.  A window of too
+  // many pages is cut again.
+  float low = -FLT_MAX, high = FLT_MAX;
+  int page = -1;  // of the window's, if this thread's one is taken
+  bool exact = false;
+  for (int round = 0;; ++round) {
+    float lo = INFINITY, hi = -INFINITY;
+    each([&](float x) {
+      const bool in = x >= low && x <= high;
+      lo = fminf(lo, in ? x : INFINITY);
+      hi = fmaxf(hi, in ? x : -INFINITY);
+    });
+    lo = -wave_max(-lo);
+    hi = wave_max(hi);
+    __syncthreads();  // the last round's maxima and map are read
+    if (l == 0) L.red[0][w] = lo, L.red[1][w] = hi;
+    if (tid == 0) L.above = L.count = 0;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    low = fminf(low, __shfl_xor(low, off));
-    high = fmaxf(high, __shfl_xor(high, off));
-    size = fmaxf(size, __shfl_xor(size, off));
-  }
-  if (l == 0) L.red[0][w] = low, L.red[1][w] = high, L.red[2][w] = size;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < NT / 64; ++i) {
-    low = fminf(low, L.red[0][i]);
-    high = fmaxf(high, L.red[1][i]);
-    size = fmaxf(size, L.red[2][i]);
-  }
-  int need = p.top_k - p.sink - p.local;
-  const float margin = 3 * (kScoreError * size + kScoreRest);
-  bool exact = !(size < INFINITY);
-  // The window [low, high] that holds the need-th largest score, and how many
-  // pages lie above it: a histogram over it, then the digit that holds the score.
-  int in = INT_MAX;
-  if (need > 0 && !exact) {
-    int above = 0;  // the window's need-th largest is the (above + need)-th of all
-    for (int round = 0; round < 3; ++round) {
-      for (int i = tid; i < kPickBins; i += NT) L.hist[i] = 0;
-      __syncthreads();
-      const float scale = high > low ? kPickBins / (high - low) : 0.f;
-      auto bin = [&](float x) { return min((int)((x - low) * scale), kPickBins - 1); };
-      each([&](int, float x) {
-        if (x >= low && x <= high) atomicAdd(&L.hist[bin(x)], 1);
+    for (int i = 4 * tid; i < kPickBins; i += 4 * NT) *reinterpret_cast<u32x4*>(&L.hist[i]) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    lo = -row_max16(-L.red[0][l % kWaves]);
+    hi = row_max16(L.red[1][l % kWaves]);
+    size = row_max16(L.red[2][l % kWaves]);
+    if (!(size < INFINITY && hi - lo < INFINITY)) {  // (uniform) some page's score is not to be gone by
+      exact = true;
+      break;
+    }
+    if (need > 0) {
+      const float scale = hi > lo ? kPickBins / (hi - lo) : 0.f;
+      const int rest = need;
+      each([&](float x) {
+        if (x >= lo && x <= hi) atomicAdd(&L.hist[min((int)((x - lo) * scale), kPickBins - 1)], 1);
       });
+      // (in a later round: how many lie above the range)
+      int above = 0;
+      if (round > 0) {
+        each([&](float x) { above += x > hi; });
+        above = __builtin_amdgcn_readlane(wave_inclusive_scan(above), 63);
+        if (l == 0) atomicAdd(&L.above, above);
+      }
       __syncthreads();
-      constexpr int kPer = kPickBins / NT;  // digits a thread, the largest first
+      above = L.above;
+      constexpr int kPer = kPickBins / NT;  // digits a thread, from the largest
+      const int mine = kPickBins - kPer * (tid + 1);
       int v[kPer], sum = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += v[i] = L.hist[kPickBins - 1 - kPer * tid - i];
+      for (int i = 0; i < kPer; ++i) sum += v[i] = L.hist[mine + i];
       const int incl = wave_inclusive_scan(sum);
       if (l == 63) L.sum[w] = incl;
       __syncthreads();
-      int over = incl - sum;
+      const int s = l < kWaves ? L.sum[l] : 0;
+      int over = above + incl - sum + __builtin_amdgcn_readlane(wave_inclusive_scan(s) - s, w);
+      if (over < rest && over + sum >= rest) {
+        int at = mine;
 #pragma unroll
-      for (int i = 0; i < NT / 64; ++i)
-        if (i < w) over += L.sum[i];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (over < need && over + v[i] >= need) L.bin = kPickBins - 1 - kPer * tid - i;
-        over += v[i];
+        for (int i = kPer - 1; i >= 0; --i) {
+          if (over < rest) at = mine + i;
+          over += v[i];
+        }
+        // the digit's ends, the margin and what the digits' own rounding may be off by
+        const float step = scale > 0.f ? 1.f / scale : 0.f;
+        const float margin = 3 * (kScoreError * size + kScoreRest) + 0.01f * step;
+        L.low = fmaxf(lo, lo + at * step - margin);
+        L.high = fminf(hi, lo + (at + 1) * step + margin);
       }
-      if (tid == 0) L.above = L.in = 0;
+      if (tid == 0) L.above = 0;
       __syncthreads();
-      const float step = scale > 0.f ? 1.f / scale : high - low;
-      const float lo = fmaxf(low, low + L.bin * step - margin), hi = fminf(high, low + (L.bin + 1) * step + margin);
-      int na = 0, ni = 0;
-      each([&](int, float x) {
-        na += x > hi && x <= high;
-        ni += x >= lo && x <= hi;
-      });
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) {
-        na += __shfl_xor(na, off);
-        ni += __shfl_xor(ni, off);
-      }
-      if (l == 0) {
-        atomicAdd(&L.above, na);
-        atomicAdd(&L.in, ni);
-      }
-      __syncthreads();
-      above += L.above;
-      need -= L.above;
-      in = L.in;
-      const bool same = !(hi - lo < 0.5f * (high - low));
-      low = lo;
-      high = hi;
-      if (in <= kPickFew || same) break;  // (uniform)
-      __syncthreads();
+      low = L.low;
+      high = L.high;
+    } else {
+      low = high = INFINITY;  // nothing but the pages that are always taken
     }
-    exact = in > kPickFew && in != need;
+    // Taken pages into the map, the window's into the list.
+    int taken = 0;
+    auto put = [&](int i, float x) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64(!(x <= high));
+      if (l == 0) L.map[i / 64] = m;
+      taken += __builtin_popcountll(m);
+      if (x >= low && x <= high) {
+        const int at = atomicAdd(&L.count, 1);
+        if (at < kPickFew) {
+          L.few_page[at] = i;
+          L.few_key[at] = 0;
+        }
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < kPickKeys; ++j) put(j * NT + tid, key[j]);
+    if (!whole)
+      for (int i = kPickKeys * NT + tid; i - l < n; i += NT) {
+        const float x = i < n ? marked(i, scores[i].x) : -INFINITY;
+        const uint64_t m = __builtin_amdgcn_ballot_w64(!(x <= high));
+        if (i < kPickChunk) {
+          if (l == 0) L.map[i / 64] = m;
+        }
+        taken += __builtin_popcountll(m);
+        if (x >= low && x <= high) {
+          const int at = atomicAdd(&L.count, 1);
+          if (at < kPickFew) {
+            L.few_page[at] = i;
+            L.few_key[at] = 0;
+          }
+        }
+      }
+    if (l == 0) atomicAdd(&L.above, taken);
+    __syncthreads();
+    const int in = L.count, left = p.top_k - L.above;
+    if (in <= kPickFew) {  // (uniform)
+      if (in == left) {
+        if (tid < in) page = L.few_page[tid];
+        break;
+      }
+      constexpr int kLanes = D / 8;  // of a page and a head
+      for (int i = tid / kLanes; i < in * p.group; i += NT / kLanes) {
+        const int at = i / p.group;
+        const uint64_t k = exact_key<D>(p, b, h, i - at * p.group, L.few_page[at], tid % kLanes);
+        if (tid % kLanes == 0) atomicMax((unsigned long long*)&L.few_key[at], k);
+      }
+      __syncthreads();
+      if (tid < in) {
+        const uint64_t k = L.few_key[tid];
+        page = L.few_page[tid];
+        int rank = 0;
+        for (int i = 0; i < in; ++i) {
+          const uint64_t o = L.few_key[i];
+          rank += o > k || (o == k && L.few_page[i] < page);
+        }
+        if (rank >= left) page = -1;
+      }
+      break;
+    }
+    if (round == 2) {
+      exact = true;
+      break;
+    }
   }
   if (exact) {  // (uniform)
     __syncthreads();
     pick_exact<D, NT>(p, L, b, h, n, reinterpret_cast<uint64_t*>(scores), out);
     return;
   }
-  // The window's pages: all of them, or the best `need` by their exact scores.
-  const bool all = need > 0 && in == need;
-  uint64_t mine = 0;
-  int page = -1;
-  if (need > 0 && !all) {
-    __syncthreads();
-    if (tid == 0) L.count = 0;
-    __syncthreads();
-    each([&](int i, float x) {
-      if (x >= low && x <= high) {
-        const int at = atomicAdd(&L.count, 1);
-        L.few.page[at] = i;
-        L.few.key[at] = 0;
-      }
-    });
-    __syncthreads();
-    constexpr int kLanes = D / 8;  // of a page and a head
-    for (int i = tid / kLanes; i < in * p.group; i += NT / kLanes) {
-      const int at = i / p.group;
-      const uint64_t k = exact_key<D>(p, b, h, i - at * p.group, L.few.page[at], tid % kLanes);
-      if (tid % kLanes == 0) atomicMax((unsigned long long*)&L.few.key[at], k);
-    }
-    __syncthreads();
-    if (tid < in) {
-      mine = L.few.key[tid];
-      page = L.few.page[tid];
-      int rank = 0;
-      for (int i = 0; i < in; ++i) {
-        const uint64_t k = L.few.key[i];
-        rank += k > mine || (k == mine && L.few.page[i] < page);
-      }
-      if (rank >= need) page = -1;
-    }
-  }
   int base = 0;
   for (int c0 = 0; c0 < n; c0 += kPickChunk) {
-    __syncthreads();
-    auto take = [&](int i, float x) {
-      return i < n && (i < first || i >= last || x > high || (all && x >= low));
-    };
     const int end = min(n, c0 + kPickChunk);
-    if (c0 == 0) {
-#pragma unroll
-      for (int j = 0; j < kPickKeys; ++j) {
-        const int i = j * NT + tid;
-        const uint64_t m = __builtin_amdgcn_ballot_w64(take(i, key[j]));
-        if (l == 0 && i < n) L.map[i / 64] = m;
+    if (c0 > 0) {
+      for (int i0 = c0; i0 < end; i0 += NT) {
+        const int i = i0 + tid;
+        const uint64_t m = __builtin_amdgcn_ballot_w64(i < n && !(marked(i, scores[i < n ? i : 0].x) <= high));
+        if (l == 0 && i < n) L.map[(i - c0) / 64] = m;
       }
+      __syncthreads();
     }
-    for (int i0 = c0 == 0 ? kPickKeys * NT : c0; i0 < end; i0 += NT) {
-      const int i = i0 + tid;
-      const float x = i >= first && i < last ? scores[i].x : 0.f;
-      const uint64_t m = __builtin_amdgcn_ballot_w64(take(i, x));
-      if (l == 0 && i < n) L.map[(i - c0) / 64] = m;
-    }
-    __syncthreads();
     if (page >= c0 && page < end) atomicOr((unsigned long long*)&L.map[(page - c0) / 64], 1ull << (page & 63));
     __syncthreads();
     base = pick_write<NT>(L, out, base, c0, n);
@@ -874,8 +884,8 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   auto launch = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
     if (max_blocks_per_seq > top_k) {
-      constexpr int kPages = 16 * kScoreTiles * kScoreWaves;
-      const dim3 grid((unsigned)(((int64_t)max_blocks_per_seq + kPages - 1) / kPages), batch * num_heads_k);
+      const int64_t items = ((int64_t)max_blocks_per_seq + 15) / 16 * num_heads_k;
+      const dim3 grid((unsigned)((items + kScoreWaves - 1) / kScoreWaves), batch);
       hipLaunchKernelGGL(score_kernel<D>, grid, dim3(kScoreWaves * 64), 0, st, p);
     }
     const dim3 rows(batch * num_heads_k);
