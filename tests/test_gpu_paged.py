@@ -327,7 +327,7 @@ def test_select_long_sequence(torch_cuda, width, top_k):
 
 
 @pytest.mark.parametrize("kind", ["equal", "few values", "crowd and one far", "two crowds", "one page far below",
-                                  "large", "nearly equal", "stranger"])
+                                  "large", "small queries", "nearly equal", "stranger"])
 @pytest.mark.parametrize("width,top_k", [(1500, 400), (5000, 90), (70000, 9000)])
 def test_select_score_distributions(torch_cuda, kind, width, top_k):
     # the scores themselves, as the first channel of bounds that are 0 elsewhere: crowds that a first look cannot
@@ -350,6 +350,9 @@ def test_select_score_distributions(torch_cuda, kind, width, top_k):
         x[width // 3] = -1e7
     elif kind == "large":
         x *= 1e30
+    elif kind == "small queries":
+        q *= 2.0 ** -130  # below the normal range, against bounds that make up for it
+        x *= 2.0 ** 120
     elif kind == "nearly equal":
         bounds[:, 0, 1, 2] = x.to(T.bfloat16)  # 2^-20 of it counts
         x.fill_(0.75)

@@ -285,6 +285,7 @@ struct SelectParams {
   int32_t* pages;           // [B][Hkv][top_k]
   float2* scores;           // [B][Hkv][width]: the fp32 score and the sum of its terms' sizes
   int num_blocks, width, page, batch, heads_k, group, top_k, sink, local;
+  FastDiv over_heads;
 };
 
 __device__ __forceinline__ int select_pages(const SelectParams& p, int b) {
@@ -292,10 +293,12 @@ __device__ __forceinline__ int select_pages(const SelectParams& p, int b) {
   return min(len / p.page + (len % p.page != 0), p.width);
 }
 
-// 2 D 2^-22 of the sizes, rounded up (D = 128), and an absolute rest for operands
-// and products below the normal range, which an instruction may take as 0.
+// 2 D 2^-22 of the sizes, rounded up (D = 128), and an absolute rest for bounds and
+// products below the normal range, which an instruction may take as 0.  The rest
+// is one for queries of 0 or 2^-126..2^60; pick_kernel looks for others.  (A bound
+// that is not finite makes every sum of sizes not finite.)
 constexpr float kScoreError = 1.02f / (1 << 14), kScoreRest = 0x1p-50f;
-constexpr uint32_t kScoreLarge = 0x5D80;  // 2^60 in bf16: from there on the rest is no bound
+constexpr uint32_t kQuerySmall = 0x0080, kQueryLarge = 0x5D80;  // 2^-126 and 2^60 in bf16
 
 // A wave scores 16 pages for one KV head.  The heads of the same pages run next to
 // one another, so a page's bounds are read from memory as one piece (32 sequences
@@ -316,9 +319,20 @@ __device__ __forceinline__ float row_max16(float x) {
   return x;
 }
 
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+// The largest of each of v's four values over the 16 lanes of a row, the one of
+// value 2 (l & 1) + (l >> 1 & 1) in lane l: two exchanges that halve the values,
+// two that keep one (5 maxima where four whole reductions take 16).
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), kCtrl, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float row_max16x4(f32x4 v, int l) {
+  const bool odd = l & 1, up = l & 2;
+  const float a = fmaxf(odd ? v[2] : v[0], dpp<0xB1>(odd ? v[0] : v[2]));  // quad_perm:[1,0,3,2]
+  const float b = fmaxf(odd ? v[3] : v[1], dpp<0xB1>(odd ? v[1] : v[3]));
+  float x = fmaxf(up ? b : a, dpp<0x4E>(up ? a : b));  // quad_perm:[2,3,0,1]
+  x = fmaxf(x, dpp<0x124>(x));                         // row_ror:4
+  return fmaxf(x, dpp<0x128>(x));
 }
 
 template <int D>
@@ -327,9 +341,8 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p)
   const int b = blockIdx.y;
   const int n = select_pages(p, b);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l & 15, lg = l >> 4;
-  const int64_t item = (int64_t)blockIdx.x * kScoreWaves + w;
-  const int h = (int)(item % p.heads_k);
-  const int64_t p0 = item / p.heads_k * 16;
+  const int item = blockIdx.x * kScoreWaves + w, tile = (int)p.over_heads.div((uint32_t)item);
+  const int h = item - tile * p.heads_k, p0 = 16 * tile;
   if (n <= p.top_k || p0 >= n) return;
   // lane i: the place of the wave's page i%16, -1 without one
   int block = -1;
@@ -349,21 +362,14 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p)
   // the B operands (lane l: head l%16, dims 32c + 8*(l/16)..+7): q's positive and
   // negative parts
   u32x4 qp[kC], qn[kC];
-  uint32_t most = 0;
   const uint16_t* qrow = p.q + b * p.q_batch + (h * p.group + (g < p.group ? g : 0)) * p.q_head + 8 * lg;
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
     const u32x4 q = *reinterpret_cast<const u32x4*>(qrow + 32 * c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t neg = ((q[i] >> 15) & 0x00010001u) * 0xFFFFu;
-      qp[c][i] = q[i] & ~neg;
-      qn[c][i] = q[i] & neg;
-      most = max_u16x2(most, q[i] & 0x7FFF7FFFu);
-    }
+    const u32x4 neg = __builtin_bit_cast(u32x4, __builtin_bit_cast(i16x8, q) >> 15);
+    qp[c] = q & ~neg;
+    qn[c] = q & neg;
   }
-  auto is_large = [](uint32_t v) { return (v & 0xFFFFu) >= kScoreLarge || v >> 16 >= kScoreLarge; };
-  const bool large_q = __builtin_amdgcn_ballot_w64(is_large(most));
   const uint32_t no_sign = 0x7FFF7FFFu;
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(lds + (i * kRows + lrow) * kPitch + lcol) = in[i];
@@ -373,36 +379,19 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p)
     y[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c + 2 * D);
   }
   f32x4 S = {0.f, 0.f, 0.f, 0.f}, A = {0.f, 0.f, 0.f, 0.f};
-  most = 0;
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
     S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c]), as_bf16x8(qn[c]), S, 0, 0, 0);
     S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c]), as_bf16x8(qp[c]), S, 0, 0, 0);
-    u32x4 an;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[c][i] &= no_sign;
-      y[c][i] &= no_sign;
-      an[i] = qn[c][i] & no_sign;
-      most = max_u16x2(most, max_u16x2(x[c][i], y[c][i]));
-    }
-    A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c]), as_bf16x8(an), A, 0, 0, 0);
-    A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c]), as_bf16x8(qp[c]), A, 0, 0, 0);
+    A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x[c] & no_sign), as_bf16x8(qn[c] & no_sign), A, 0, 0, 0);
+    A = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(y[c] & no_sign), as_bf16x8(qp[c]), A, 0, 0, 0);
   }
   // lane l: head l%16, pages 4*(l/16)..+3 of S and A
-  uint64_t wide = __builtin_amdgcn_ballot_w64(is_large(most));  // of page l%16, in each of its four lanes
-  wide |= wide >> 32;
-  wide |= wide >> 16;
-  float s = 0.f, a = 0.f;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const float sr = row_max16(S[r]), ar = row_max16(A[r]);
-    if (g == r) s = sr, a = ar;
-  }
-  const int at = 4 * lg + (g & 3);  // the page whose score lanes with g < 4 have now
-  const bool gone = __shfl(block, at) < 0;
+  const float s = row_max16x4(S, l);
+  float a = row_max16x4(A, l);
+  const int at = 4 * lg + 2 * (l & 1) + (l >> 1 & 1);
   // an infinite sum of sizes says that the score is not to be gone by
-  if (large_q || gone || (wide >> at & 1)) a = INFINITY;
+  if (__shfl(block, at) < 0 || !(a < INFINITY)) a = INFINITY;
   if (g < 4 && p0 + at < n) p.scores[((int64_t)b * p.heads_k + h) * p.width + p0 + at] = float2{s, a};
 }
 
@@ -582,6 +571,16 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   }
   if (!whole)
     for (int i = kPickKeys * NT + tid; i < last; i += NT) size = fmaxf(size, i >= first ? scores[i].y : 0.f);
+  for (int i = tid; i < p.group * (D / 8); i += NT) {
+    const int g = i / (D / 8);
+    const u32x4 q = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head +
+                                                    8 * (i - g * (D / 8)));
+    const u16x8 u = __builtin_bit_cast(u16x8, q) & (uint16_t)0x7FFF;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) odd |= u[j] >= kQueryLarge || (u[j] != 0 && u[j] < kQuerySmall);
+    if (odd) size = INFINITY;
+  }
   size = wave_max(size);
   if (l == 0) L.red[2][w] = size;
   auto each = [&](auto f) {
@@ -861,6 +860,8 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   if (num_heads / num_heads_k > 16 || (int64_t)batch * num_heads_k > 65535) return ZS_E_UNSUPPORTED;
   if (workspace_bytes < zs_select_kv_pages_workspace_bytes(batch, num_heads_k, max_blocks_per_seq))
     return ZS_E_INVAL;
+  const int64_t score_items = ((int64_t)max_blocks_per_seq + 15) / 16 * num_heads_k;
+  if (score_items > INT_MAX / 16) return ZS_E_OVERFLOW;
   SelectParams p{};
   p.q = q;
   p.q_batch = q_batch_stride;
@@ -878,14 +879,14 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   p.heads_k = num_heads_k;
   p.group = num_heads / num_heads_k;
   p.top_k = top_k;
+  p.over_heads = FastDiv::of(num_heads_k);
   p.sink = sink_pages;
   p.local = local_pages;
   const hipStream_t st = (hipStream_t)stream;
   auto launch = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
     if (max_blocks_per_seq > top_k) {
-      const int64_t items = ((int64_t)max_blocks_per_seq + 15) / 16 * num_heads_k;
-      const dim3 grid((unsigned)((items + kScoreWaves - 1) / kScoreWaves), batch);
+      const dim3 grid((unsigned)((score_items + kScoreWaves - 1) / kScoreWaves), batch);
       hipLaunchKernelGGL(score_kernel<D>, grid, dim3(kScoreWaves * 64), 0, st, p);
     }
     const dim3 rows(batch * num_heads_k);
