@@ -369,32 +369,35 @@ def flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cach
     without tokens gives zeros and lse -inf."""
     torch = _torch()
     shape = q.shape
-    q3 = q[:, 0] if q.dim() == 4 and q.shape[1] == 1 else q
-    paged._check(q3, "q", torch.bfloat16, (None,) * 3, contiguous=False)
+    q3 = paged._query(q)
+    on = paged._elsewhere(q3)
+    if on is not None:
+        with on:
+            return flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cache_seqlens,
+                                                  softmax_scale, num_splits, return_softmax_lse)
     B, H, D = q3.shape
-    device = q3.device
+    device = q3.get_device()
     paged._check(k_cache, "k_cache", torch.bfloat16, (None, None, None, D), device)
-    paged._check(v_cache, "v_cache", torch.bfloat16, k_cache.shape, device)
-    nblocks, page, Hkv, _ = k_cache.shape
-    table = paged._table(block_table, B, device)
+    size = k_cache.shape
+    paged._check(v_cache, "v_cache", torch.bfloat16, size, device)
+    nblocks, page, Hkv, _ = size
+    table, stride, width = paged._table(block_table, B, device)
+    lens = paged._lengths(cache_seqlens, B, device)
     paged._check(pages, "pages", torch.int32, (B, Hkv, None), device)
     top_k = pages.shape[2]
     if Hkv == 0 or H % Hkv:
         raise ValueError(f"{H} query heads do not share {Hkv} KV heads evenly")
     scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
-    with paged._device_of(q3):
-        lens = paged._lengths(cache_seqlens, B, device)
-        q3 = paged._rows(q3)
-        out = torch.empty((B, H, D), dtype=torch.bfloat16, device=device)
-        lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_softmax_lse else None
-        L = lib()
-        wsb = int(L.zs_decode_attention_sparse_workspace_bytes(B, H, Hkv, D, top_k, page, num_splits))
-        ws = torch.empty(wsb, dtype=torch.uint8, device=device) if wsb else None
-        check("zs_decode_attention_sparse_paged", L.zs_decode_attention_sparse_paged(
-            _stream(), q3.data_ptr(), q3.stride(0), q3.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), nblocks,
-            page, table.data_ptr(), table.stride(0), table.shape[1], pages.data_ptr(), top_k, lens.data_ptr(), B, H,
-            Hkv, D, scale, out.data_ptr(), _dptr(lse), _dptr(ws), wsb, int(num_splits)))
-    out = out.view(shape)
+    splits, at = int(num_splits), q3.device
+    q3, q0, q1 = paged._rows(q3)
+    out = torch.empty(shape, dtype=torch.bfloat16, device=at)
+    lse = torch.empty((B, H), dtype=torch.float32, device=at) if return_softmax_lse else None
+    wsb = paged._bytes("zs_decode_attention_sparse_workspace_bytes", B, H, Hkv, D, top_k, page, splits)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=at) if wsb else None
+    check("zs_decode_attention_sparse_paged", lib().zs_decode_attention_sparse_paged(
+        _stream(), q3.data_ptr(), q0, q1, k_cache.data_ptr(), v_cache.data_ptr(), nblocks, page, table.data_ptr(),
+        stride, width, pages.data_ptr(), top_k, lens.data_ptr(), B, H, Hkv, D, scale, out.data_ptr(), _dptr(lse),
+        _dptr(ws), wsb, splits))
     return (out, lse) if return_softmax_lse else out
 
 

@@ -17,53 +17,87 @@ outputs and workspace.
 """
 from __future__ import annotations
 
-import contextlib
+import functools
 from dataclasses import dataclass
 
 from ._lib import check, lib
 from .codec import _dptr, _stream, _torch
 
-_here = contextlib.nullcontext()
 
-
-def _device_of(t):
-    """A context in which t's device is the current one, whose current stream
-    the call goes to."""
+def _elsewhere(t):
+    """None where t's device is the current one, whose current stream a call goes
+    to, else the context that makes it so."""
     cuda = _torch().cuda
-    return _here if t.device.index == cuda.current_device() else cuda.device(t.device)
+    return None if t.get_device() == cuda.current_device() else cuda.device(t.device)
 
 
 def _check(t, name, dtype, shape, device=None, contiguous=True):
-    """`shape`: the sizes asked for, None where any will do."""
+    """Raises where t is not a GPU tensor of these (shape: None where any size will
+    do; device: its index)."""
+    try:  # (what a right tensor costs is 0.6 us)
+        if t.dtype is dtype and t.is_cuda and (device is None or t.get_device() == device) and \
+                (not contiguous or t.is_contiguous()):
+            got = t.shape
+            if got == shape or (len(got) == len(shape) and all(n is None or n == m for n, m in zip(shape, got))):
+                return
+    except AttributeError:
+        pass
     torch = _torch()
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        want = ", ".join("*" if n is None else str(n) for n in shape)
-        raise ValueError(f"{name} must be ({want}), got {tuple(t.shape)}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} must be on cuda:{device}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+    want = ", ".join("*" if n is None else str(n) for n in shape)
+    raise ValueError(f"{name} must be ({want}), got {tuple(t.shape)}")
 
 
 def _rows(t):
-    """t (rows, heads, dim) as the kernels take it: 16-byte pieces of contiguous
-    heads at any stride between rows and heads (a slice of a fused projection is
-    one), a copy otherwise."""
+    """t (rows, heads, dim) and its strides as the kernels take it: 16-byte pieces
+    of contiguous heads at any stride between rows and heads (a slice of a fused
+    projection is one), a copy otherwise."""
     s0, s1, s2 = t.stride()
     if s2 != 1 or s0 % 8 or s1 % 8 or t.data_ptr() % 16:
-        return t.clone(memory_format=_torch().contiguous_format)
-    return t
+        t = t.clone(memory_format=_torch().contiguous_format)
+        s0, s1, _ = t.stride()
+    return t, s0, s1
 
 
 def _table(block_table, batch, device):
+    """A block table that is read, its row stride and its width."""
     _check(block_table, "block_table", _torch().int32, (batch, None), device, contiguous=False)
-    inner, width = block_table.stride(1), block_table.shape[1]
-    apart = block_table.stride(0) >= width and (inner == 1 or width == 1)
-    return block_table if apart else block_table.contiguous()
+    width = block_table.shape[1]
+    s0, s1 = block_table.stride()
+    if s0 < width or (s1 != 1 and width > 1):
+        block_table = block_table.contiguous()
+        s0 = max(width, 1)
+    return block_table, s0, width
+
+
+def _lengths(cache_seqlens, batch, device):
+    torch = _torch()
+    if isinstance(cache_seqlens, int):
+        return torch.full((batch,), cache_seqlens, dtype=torch.int32, device=f"cuda:{device}")
+    _check(cache_seqlens, "cache_seqlens", torch.int32, (batch,), device)
+    return cache_seqlens
+
+
+def _query(q):
+    """(B, 1, H, D) or (B, H, D) -> (B, H, D)."""
+    torch = _torch()
+    if isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[1] == 1:
+        q = q[:, 0]
+    _check(q, "q", torch.bfloat16, (None, None, None), contiguous=False)
+    return q
+
+
+@functools.lru_cache(maxsize=4096)
+def _bytes(query, *sizes):
+    """What a workspace query answers."""
+    return int(getattr(lib(), query)(*sizes))
 
 
 @dataclass
@@ -95,28 +129,34 @@ def plan_paged_step(context_lens, new_lens, block_table, free_pages, num_free, p
     need them get slot -1, and seqlens and counts say so: counts[0] against
     cu_new[-1] shows tokens left out, counts[2] the pages missing."""
     torch = _torch()
-    _check(context_lens, "context_lens", torch.int32, (None,))
-    device, batch = context_lens.device, context_lens.shape[0]
-    _check(new_lens, "new_lens", torch.int32, (batch,), device)
-    _check(block_table, "block_table", torch.int32, (batch, None), device, contiguous=False)
+    i32 = torch.int32
+    _check(context_lens, "context_lens", i32, (None,))
+    on = _elsewhere(context_lens)
+    if on is not None:
+        with on:
+            return plan_paged_step(context_lens, new_lens, block_table, free_pages, num_free, page_block_size,
+                                   max_tokens)
+    device, batch = context_lens.get_device(), context_lens.shape[0]
+    _check(new_lens, "new_lens", i32, (batch,), device)
+    _check(block_table, "block_table", i32, (batch, None), device, contiguous=False)
     width = block_table.shape[1]
-    stride = block_table.stride(0) if batch > 1 else width
-    if (block_table.stride(1) != 1 and width > 1) or stride < width:
+    stride, inner = block_table.stride()
+    if batch == 1:
+        stride = max(width, 1)
+    if (inner != 1 and width > 1) or stride < width:
         raise ValueError("block_table is written in place: its rows must be contiguous and apart")
-    _check(free_pages, "free_pages", torch.int32, (None,), device)
-    _check(num_free, "num_free", torch.int32, (1,), device)
-    page, most = int(page_block_size), int(max_tokens)
+    _check(free_pages, "free_pages", i32, (None,), device)
+    _check(num_free, "num_free", i32, (1,), device)
+    most = int(max_tokens)
     if most < 0:
         raise ValueError("max_tokens must not be negative")
-    with _device_of(context_lens):
-        out = torch.empty(3 * most + 2 * batch + 5, dtype=torch.int32, device=device)
-        plan = PagedPlan(*out.split([most, most, most, batch, batch + 1, 4]))
-        at = out.data_ptr()
-        check("zs_paged_plan", lib().zs_paged_plan(
-            _stream(), context_lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), stride, width,
-            free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), page, most, at, at + 4 * most,
-            at + 8 * most, at + 12 * most, at + 12 * most + 4 * batch, at + 12 * most + 8 * batch + 4))
-    return plan
+    out = torch.empty(3 * most + 2 * batch + 5, dtype=i32, device=context_lens.device)
+    at = out.data_ptr()
+    check("zs_paged_plan", lib().zs_paged_plan(
+        _stream(), context_lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), stride, width,
+        free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), int(page_block_size), most, at,
+        at + 4 * most, at + 8 * most, at + 12 * most, at + 12 * most + 4 * batch, at + 12 * most + 8 * batch + 4))
+    return PagedPlan(*torch.split_with_sizes(out, (most, most, most, batch, batch + 1, 4)))
 
 
 def append_paged_kv(k, v, k_cache, v_cache, slots, page_bounds=None) -> None:
@@ -129,22 +169,26 @@ def append_paged_kv(k, v, k_cache, v_cache, slots, page_bounds=None) -> None:
     of one page stand next to one another, as a plan puts them, and no slot
     occurs twice."""
     torch = _torch()
-    _check(k_cache, "k_cache", torch.bfloat16, (None,) * 4)
-    device = k_cache.device
-    blocks, page, heads_k, dim = k_cache.shape
-    _check(v_cache, "v_cache", torch.bfloat16, k_cache.shape, device)
+    bf16 = torch.bfloat16
+    _check(k_cache, "k_cache", bf16, (None, None, None, None))
+    on = _elsewhere(k_cache)
+    if on is not None:
+        with on:
+            return append_paged_kv(k, v, k_cache, v_cache, slots, page_bounds)
+    device, size = k_cache.get_device(), k_cache.shape
+    blocks, page, heads_k, dim = size
+    _check(v_cache, "v_cache", bf16, size, device)
     _check(slots, "slots", torch.int32, (None,), device)
     n = slots.shape[0]
-    _check(k, "k", torch.bfloat16, (n, heads_k, dim), device, contiguous=False)
-    _check(v, "v", torch.bfloat16, (n, heads_k, dim), device, contiguous=False)
+    _check(k, "k", bf16, (n, heads_k, dim), device, contiguous=False)
+    _check(v, "v", bf16, (n, heads_k, dim), device, contiguous=False)
     if page_bounds is not None:
-        _check(page_bounds, "page_bounds", torch.bfloat16, (blocks, heads_k, 2, dim), device)
-    with _device_of(k_cache):
-        k, v = _rows(k), _rows(v)
-        check("zs_paged_append", lib().zs_paged_append(
-            _stream(), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-            slots.data_ptr(), n, k_cache.data_ptr(), v_cache.data_ptr(), _dptr(page_bounds), blocks, page, heads_k,
-            dim))
+        _check(page_bounds, "page_bounds", bf16, (blocks, heads_k, 2, dim), device)
+    k, k0, k1 = _rows(k)
+    v, v0, v1 = _rows(v)
+    check("zs_paged_append", lib().zs_paged_append(
+        _stream(), k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, k_cache.data_ptr(),
+        v_cache.data_ptr(), _dptr(page_bounds), blocks, page, heads_k, dim))
 
 
 def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size: int, top_k: int,
@@ -160,35 +204,30 @@ def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size:
     local_pages of a sequence are always taken, the others by score, ties to the
     lowest page; sequences of at most top_k pages keep them all."""
     torch = _torch()
-    if isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[1] == 1:
-        q = q[:, 0]
-    _check(q, "q", torch.bfloat16, (None,) * 3, contiguous=False)
+    q = _query(q)
+    on = _elsewhere(q)
+    if on is not None:
+        with on:
+            return select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size, top_k, sink_pages,
+                                   local_pages)
     batch, heads, dim = q.shape
-    device = q.device
+    device = q.get_device()
     _check(page_bounds, "page_bounds", torch.bfloat16, (None, None, 2, dim), device)
     blocks, heads_k = page_bounds.shape[:2]
-    table = _table(block_table, batch, device)
-    width, page, top_k = table.shape[1], int(page_block_size), int(top_k)
-    if top_k <= 0 or sink_pages < 0 or local_pages < 0 or sink_pages + local_pages > top_k:
+    table, stride, width = _table(block_table, batch, device)
+    lens = _lengths(cache_seqlens, batch, device)
+    top_k, sink, local = int(top_k), int(sink_pages), int(local_pages)
+    if top_k <= 0 or sink < 0 or local < 0 or sink + local > top_k:
         raise ValueError("top_k must be positive and hold sink_pages and local_pages")
     if heads_k == 0 or heads % heads_k:
         raise ValueError(f"{heads} query heads do not share {heads_k} KV heads evenly")
-    with _device_of(q):
-        lens = _lengths(cache_seqlens, batch, device)
-        q = _rows(q)
-        pages = torch.empty((batch, heads_k, top_k), dtype=torch.int32, device=device)
-        need = int(lib().zs_select_kv_pages_workspace_bytes(batch, heads_k, width))
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        check("zs_select_kv_pages", lib().zs_select_kv_pages(
-            _stream(), q.data_ptr(), q.stride(0), q.stride(1), page_bounds.data_ptr(), blocks, page,
-            table.data_ptr(), table.stride(0), width, lens.data_ptr(), batch, heads, heads_k, dim, top_k,
-            int(sink_pages), int(local_pages), pages.data_ptr(), ws.data_ptr(), need))
+    q, q0, q1 = _rows(q)
+    at = q.device
+    pages = torch.empty((batch, heads_k, top_k), dtype=torch.int32, device=at)
+    need = _bytes("zs_select_kv_pages_workspace_bytes", batch, heads_k, width)
+    ws = torch.empty(need, dtype=torch.uint8, device=at)
+    check("zs_select_kv_pages", lib().zs_select_kv_pages(
+        _stream(), q.data_ptr(), q0, q1, page_bounds.data_ptr(), blocks, int(page_block_size), table.data_ptr(),
+        stride, width, lens.data_ptr(), batch, heads, heads_k, dim, top_k, sink, local, pages.data_ptr(),
+        ws.data_ptr(), need))
     return pages
-
-
-def _lengths(cache_seqlens, batch, device):
-    torch = _torch()
-    if isinstance(cache_seqlens, int):
-        return torch.full((batch,), cache_seqlens, dtype=torch.int32, device=device)
-    _check(cache_seqlens, "cache_seqlens", torch.int32, (batch,), device)
-    return cache_seqlens
