@@ -30,7 +30,7 @@ namespace zs {
 // from L2) and then places its 256 tokens by a search over the first sum.  A
 // table entry is written by the token that opens its page and read only for
 // pages that the sequence had before, so no workgroup waits for another.
-constexpr int kPlanThreads = 256;
+constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxBatch = 4096;
 
 struct PlanParams {
@@ -50,22 +50,25 @@ struct PlanParams {
   FastDiv page;
 };
 
-// Inclusive sum over the workgroup of one value a thread, and the total.
-__device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t* wave_sum, int64_t& total) {
-  const int l = lane_id(), w = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(x, off);
-    if (l >= off) x += y;
-  }
-  __syncthreads();  // the last scan's sums are read
-  if (l == 63) wave_sum[w] = x;
+// Inclusive sum of a value of 0..2^31 - 1 over the lanes of a wave: two sums of
+// 16 bits over DPP, which 32 bits hold.
+__device__ __forceinline__ int64_t plan_wave_scan(int x) {
+  return ((int64_t)wave_inclusive_scan(x >> 16) << 16) + wave_inclusive_scan(x & 0xFFFF);
+}
+
+// The same over the workgroup, and the total.  `sums` is one call's own until the
+// workgroup's next barrier but one.
+__device__ __forceinline__ int64_t plan_scan(int v, int64_t* sums, int64_t& total) {
+  const int w = threadIdx.x >> 6;
+  int64_t x = plan_wave_scan(v);
+  if (lane_id() == 63) sums[w] = x;
   __syncthreads();
   total = 0;
 #pragma unroll
   for (int i = 0; i < kPlanThreads / 64; ++i) {
-    if (i < w) x += wave_sum[i];
-    total += wave_sum[i];
+    const int64_t y = sums[i];
+    x += i < w ? y : 0;
+    total += y;
   }
   return x;
 }
@@ -79,32 +82,34 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanParams p) {
   __shared__ int first_page[kPlanMaxBatch];     // how many pages the ones before it take
   __shared__ int held[kPlanMaxBatch];           // pages that it had
   __shared__ int had[kPlanMaxBatch];            // tokens that it had
-  __shared__ int64_t sums[kPlanThreads / 64];
+  __shared__ int64_t sums[4][kPlanThreads / 64];
   const int page = (int)p.page.d;
   const int64_t F = min(max(*p.num_free, 0), p.free_capacity);
-  int64_t asked = 0, tokens = 0, taken = 0, wanted = 0;  // of the sequences so far
+  int64_t tokens = 0, taken = 0;    // of the sequences so far
+  int64_t asked = 0, wanted = 0;    // of this thread's
   const bool lead = blockIdx.x == 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+  auto pages_of = [&](uint32_t n) {
+    const uint32_t q = p.page.div(n);
+    return (int)(q + (q * page != n));
+  };
+  for (int b0 = 0, i = 0; b0 < p.batch; b0 += kPlanThreads, i ^= 2) {
     const int b = b0 + threadIdx.x;
     const bool live = b < p.batch;
     const int c = live ? max(p.context[b], 0) : 0;
     const int n_asked = live ? max(p.fresh[b], 0) : 0;
     int n = min(n_asked, INT_MAX - c);
     int64_t total;
-    const int64_t end = tokens + plan_scan(n, sums, total);
+    const int64_t end = tokens + plan_scan(n, sums[i], total);
     const int start = (int)min(end - n, (int64_t)p.max_tokens);
     n = (int)min((int64_t)n, p.max_tokens - (int64_t)start);
     tokens += total;
-    plan_scan(n_asked, sums, total);
-    asked += total;
-    const int have = (int)p.page.div((uint32_t)c) + (p.page.div((uint32_t)c) * page != (uint32_t)c);
     const uint32_t all = (uint32_t)c + (uint32_t)n;
-    const int need = (int)(p.page.div(all) + (p.page.div(all) * page != all));
+    const int have = pages_of(c), need = pages_of(all);
     const int more = max(min(need, p.width) - have, 0);
-    const int64_t before = taken + plan_scan(more, sums, total) - more;
+    const int64_t before = taken + plan_scan(more, sums[i + 1], total) - more;
     taken += total;
-    plan_scan(need - have, sums, total);
-    wanted += total;
+    asked += n_asked;
+    wanted += need - have;
     if (live) {
       first[b] = start;
       first_page[b] = plan_saturate(before);
@@ -119,14 +124,23 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanParams p) {
     }
   }
   const int used = (int)min(tokens, (int64_t)p.max_tokens);
-  if (threadIdx.x == 0) {
-    first[p.batch] = used;
-    if (lead) {
+  if (threadIdx.x == 0) first[p.batch] = used;
+  if (lead) {  // (uniform)
+    int64_t a = 0, m = 0, unused;
+    // (each in halves that a scan takes)
+    for (int half = 0; half < 2; ++half) {
+      __syncthreads();
+      plan_scan((int)(asked >> (half ? 31 : 0) & INT_MAX), sums[0], unused);
+      a += half ? unused << 31 : unused;
+      plan_scan((int)(wanted >> (half ? 31 : 0) & INT_MAX), sums[1], unused);
+      m += half ? unused << 31 : unused;
+    }
+    if (threadIdx.x == 0) {
       const int64_t given = min(taken, F);
       p.cu_new[p.batch] = used;
-      p.counts[0] = plan_saturate(asked);
+      p.counts[0] = plan_saturate(a);
       p.counts[1] = (int)given;
-      p.counts[2] = plan_saturate(wanted - given);
+      p.counts[2] = plan_saturate(m - given);
       p.counts[3] = (int)(F - given);
     }
   }
