@@ -390,7 +390,7 @@ def flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cach
     scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
     splits, at = int(num_splits), q3.device
     q3, q0, q1 = paged._rows(q3)
-    out = torch.empty(shape, dtype=torch.bfloat16, device=at)
+    out = paged._new_like(q3, shape)
     lse = torch.empty((B, H), dtype=torch.float32, device=at) if return_softmax_lse else None
     wsb = paged._bytes("zs_decode_attention_sparse_workspace_bytes", B, H, Hkv, D, top_k, page, splits)
     ws = torch.empty(wsb, dtype=torch.uint8, device=at) if wsb else None

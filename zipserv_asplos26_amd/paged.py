@@ -34,12 +34,18 @@ def _elsewhere(t):
 def _check(t, name, dtype, shape, device=None, contiguous=True):
     """Raises where t is not a GPU tensor of these (shape: None where any size will
     do; device: its index)."""
-    try:  # (what a right tensor costs is 0.6 us)
-        if t.dtype is dtype and t.is_cuda and (device is None or t.get_device() == device) and \
+    try:  # (a right tensor takes 0.4 us)
+        if t.dtype is dtype and (t.is_cuda if device is None else t.get_device() == device) and \
                 (not contiguous or t.is_contiguous()):
             got = t.shape
-            if got == shape or (len(got) == len(shape) and all(n is None or n == m for n, m in zip(shape, got))):
+            if got == shape:
                 return
+            if len(got) == len(shape):
+                for n, m in zip(shape, got):
+                    if n is not None and n != m:
+                        break
+                else:
+                    return
     except AttributeError:
         pass
     torch = _torch()
@@ -88,10 +94,20 @@ def _lengths(cache_seqlens, batch, device):
 def _query(q):
     """(B, 1, H, D) or (B, H, D) -> (B, H, D)."""
     torch = _torch()
-    if isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[1] == 1:
-        q = q[:, 0]
+    if isinstance(q, torch.Tensor):
+        if q.dim() == 4 and q.shape[1] == 1:
+            q = q[:, 0]
+        if q.dtype is torch.bfloat16 and q.is_cuda and q.dim() == 3:
+            return q
     _check(q, "q", torch.bfloat16, (None, None, None), contiguous=False)
     return q
+
+
+def _new_like(q, shape):
+    """A contiguous tensor of q's type and place (empty_like takes two thirds of
+    the time of empty)."""
+    torch = _torch()
+    return torch.empty_like(q) if q.shape == shape and q.is_contiguous() else q.new_empty(shape)
 
 
 @functools.lru_cache(maxsize=4096)
