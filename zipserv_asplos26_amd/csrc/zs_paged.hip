@@ -479,6 +479,14 @@ __device__ __forceinline__ uint64_t score_key(double x) {
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
+template <int kCtrl>
+__device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)u, kCtrl, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(u >> 32), kCtrl, 0xF, 0xF, true);
+  return x + __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo));
+}
+
 template <int D>
 __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, int b, int h, int g, int lp, int c) {
   constexpr int kLanes = D / 8;
@@ -495,8 +503,10 @@ __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, int b, int 
     s = fma(q, k1 + k0, s);
     s = fma(fabs(q), k1 - k0, s);
   }
-#pragma unroll
-  for (int off = 1; off < kLanes; off <<= 1) s += __shfl_xor(s, off);
+  s = dpp_add<0xB1>(s);   // quad_perm:[1,0,3,2]
+  s = dpp_add<0x4E>(s);   // quad_perm:[2,3,0,1]
+  s = dpp_add<0x141>(s);  // row_half_mirror: eight lanes
+  if constexpr (kLanes == 16) s = dpp_add<0x140>(s);  // row_mirror
   return score_key(s != s ? INFINITY : s);
 }
 
@@ -628,6 +638,13 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
 #pragma unroll
   for (int j = 0; j < kPickKeys; ++j)  // (what lies behind the row's end is not looked at)
     own[j] = j * NT + tid < p.width ? scores[j * NT + tid] : float2{0.f, 0.f};
+  // (a group has at most 16 heads: 256 pieces of 8 values)
+  static_assert(NT >= 256, "a piece a thread");
+  u32x4 query = {0, 0, 0, 0};
+  if (tid < p.group * (D / 8)) {
+    const int g = tid / (D / 8);
+    query = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head + 8 * (tid % (D / 8)));
+  }
   const int n = select_pages(p, b);
   int32_t* out = p.pages + (int64_t)row * p.top_k;
   if (n <= p.top_k) {
@@ -639,21 +656,23 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   const bool whole = n <= kPickKeys * NT;
   // A page's score: NaN for one that is always taken, -inf behind the last one.
   auto marked = [&](int i, float x) { return i >= first && i < last ? x : i < n ? NAN : -INFINITY; };
-  float key[kPickKeys], size = 0.f;
+  float key[kPickKeys], size = 0.f, lo = INFINITY, hi = -INFINITY;
+  auto note = [&](int i, float2 x) {  // the first round's range
+    const bool in = i >= first && i < last;
+    size = fmaxf(size, in ? x.y : 0.f);
+    lo = fminf(lo, in ? x.x : INFINITY);
+    hi = fmaxf(hi, in ? x.x : -INFINITY);
+  };
 #pragma unroll
   for (int j = 0; j < kPickKeys; ++j) {
-    const int i = j * NT + tid;
-    key[j] = marked(i, own[j].x);
-    size = fmaxf(size, i >= first && i < last ? own[j].y : 0.f);
+    note(j * NT + tid, own[j]);
+    key[j] = marked(j * NT + tid, own[j].x);
   }
   if (!whole)
-    for (int i = kPickKeys * NT + tid; i < last; i += NT) size = fmaxf(size, i >= first ? scores[i].y : 0.f);
-  for (int i = tid; i < p.group * (D / 8); i += NT) {
-    const int g = i / (D / 8);
-    const u32x4 q = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head +
-                                                    8 * (i - g * (D / 8)));
-    const u16x8 u = __builtin_bit_cast(u16x8, q) & (uint16_t)0x7FFF;
-    uint32_t odd = 0;
+    for (int i = kPickKeys * NT + tid; i < last; i += NT) note(i, scores[i]);
+  {
+    const u16x8 u = __builtin_bit_cast(u16x8, query) & (uint16_t)0x7FFF;
+    bool odd = false;
 #pragma unroll
     for (int j = 0; j < 8; ++j) odd |= u[j] >= kQueryLarge || (u[j] != 0 && u[j] < kQuerySmall);
     if (odd) size = INFINITY;
@@ -673,15 +692,17 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   int page = -1;  // of the window's, if this thread's one is taken
   bool exact = false;
   for (int round = 0;; ++round) {
-    float lo = INFINITY, hi = -INFINITY;
-    each([&](float x) {
-      const bool in = x >= low && x <= high;
-      lo = fminf(lo, in ? x : INFINITY);
-      hi = fmaxf(hi, in ? x : -INFINITY);
-    });
+    if (round > 0) {
+      lo = INFINITY, hi = -INFINITY;
+      each([&](float x) {
+        const bool in = x >= low && x <= high;
+        lo = fminf(lo, in ? x : INFINITY);
+        hi = fmaxf(hi, in ? x : -INFINITY);
+      });
+      __syncthreads();  // the last round's maxima and map are read
+    }
     lo = -wave_max(-lo);
     hi = wave_max(hi);
-    __syncthreads();  // the last round's maxima and map are read
     if (l == 0) L.red[0][w] = lo, L.red[1][w] = hi;
     if (tid == 0) L.above = L.count = 0;
 #pragma unroll
@@ -712,8 +733,19 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
       constexpr int kPer = kPickBins / NT;  // digits a thread, from the largest
       const int mine = kPickBins - kPer * (tid + 1);
       int v[kPer], sum = 0;
+      if constexpr (kPer >= 4) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += v[i] = L.hist[mine + i];
+        for (int i = 0; i < kPer; i += 4) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(&L.hist[mine + i]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[i + j] = (int)x[j];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = L.hist[mine + i];
+      }
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sum += v[i];
       const int incl = wave_inclusive_scan(sum);
       if (l == 63) L.sum[w] = incl;
       __syncthreads();
@@ -741,10 +773,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     }
     // Taken pages into the map, the window's into the list.
     int taken = 0;
-    auto put = [&](int i, float x) {
-      const uint64_t m = __builtin_amdgcn_ballot_w64(!(x <= high));
-      if (l == 0) L.map[i / 64] = m;
-      taken += __builtin_popcountll(m);
+    auto put = [&](int i, float x) {  // the wave's taken pages, a bit each
       if (x >= low && x <= high) {
         const int at = atomicAdd(&L.count, 1);
         if (at < kPickFew) {
@@ -752,24 +781,21 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
           L.few_key[at] = 0;
         }
       }
+      const uint64_t m = __builtin_amdgcn_ballot_w64(!(x <= high));
+      taken += __builtin_popcountll(m);
+      return m;
     };
+    uint64_t word = 0;  // lane j: of the wave's j-th 64 pages
 #pragma unroll
-    for (int j = 0; j < kPickKeys; ++j) put(j * NT + tid, key[j]);
+    for (int j = 0; j < kPickKeys; ++j) {
+      const uint64_t m = put(j * NT + tid, key[j]);
+      word = l == j ? m : word;
+    }
+    if (l < kPickKeys) L.map[l * kWaves + w] = word;
     if (!whole)
       for (int i = kPickKeys * NT + tid; i - l < n; i += NT) {
-        const float x = i < n ? marked(i, scores[i].x) : -INFINITY;
-        const uint64_t m = __builtin_amdgcn_ballot_w64(!(x <= high));
-        if (i < kPickChunk) {
-          if (l == 0) L.map[i / 64] = m;
-        }
-        taken += __builtin_popcountll(m);
-        if (x >= low && x <= high) {
-          const int at = atomicAdd(&L.count, 1);
-          if (at < kPickFew) {
-            L.few_page[at] = i;
-            L.few_key[at] = 0;
-          }
-        }
+        const uint64_t m = put(i, i < n ? marked(i, scores[i].x) : -INFINITY);
+        if (i < kPickChunk && l == 0) L.map[i / 64] = m;
       }
     if (l == 0) atomicAdd(&L.above, taken);
     __syncthreads();
@@ -790,6 +816,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
         const uint64_t k = L.few_key[tid];
         page = L.few_page[tid];
         int rank = 0;
+#pragma unroll 4
         for (int i = 0; i < in; ++i) {
           const uint64_t o = L.few_key[i];
           rank += o > k || (o == k && L.few_page[i] < page);
@@ -806,6 +833,33 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   if (exact) {  // (uniform)
     __syncthreads();
     pick_exact<D, NT>(p, L, b, h, n, reinterpret_cast<uint64_t*>(scores), out);
+    return;
+  }
+  if (whole) {
+    // every wave sums the bits of all words, and writes its own ones' pages
+    if (page >= 0) atomicOr((unsigned long long*)&L.map[page / 64], 1ull << (page & 63));
+    __syncthreads();
+    constexpr int kPer = kPickKeys * kWaves > 64 ? 2 : 1;  // words a lane
+    static_assert(kPickKeys * kWaves <= 64 * kPer, "");
+    uint64_t m[kPer];
+    int c[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      m[i] = kPer * l + i < kPickKeys * kWaves ? L.map[kPer * l + i] : 0;
+      sum += c[i] = __builtin_popcountll(m[i]);
+    }
+    const int before = wave_inclusive_scan(sum) - sum;
+#pragma unroll
+    for (int j = 0; j < kPickKeys; ++j) {
+      const int at = j * kWaves + w, of = at / kPer, i = at % kPer;
+      int base = __builtin_amdgcn_readlane(before, of);
+      if (kPer == 2 && i) base += __builtin_amdgcn_readlane(c[0], of);
+      const uint64_t mine = kPer == 2 && i ? m[kPer - 1] : m[0];
+      const uint32_t lo32 = __builtin_amdgcn_readlane((uint32_t)mine, of);
+      const uint32_t hi32 = __builtin_amdgcn_readlane((uint32_t)(mine >> 32), of);
+      const uint64_t bits = (uint64_t)hi32 << 32 | lo32;
+      if (bits >> l & 1) out[base + __builtin_popcountll(bits & ((1ull << l) - 1))] = j * NT + tid;
+    }
     return;
   }
   int base = 0;
@@ -972,6 +1026,8 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
     const dim3 rows(batch * num_heads_k);
     if (max_blocks_per_seq <= kPickKeys * 256)
       hipLaunchKernelGGL((pick_kernel<D, 256>), rows, dim3(256), 0, st, p);
+    else if (max_blocks_per_seq <= kPickKeys * 512)
+      hipLaunchKernelGGL((pick_kernel<D, 512>), rows, dim3(512), 0, st, p);
     else
       hipLaunchKernelGGL((pick_kernel<D, 1024>), rows, dim3(1024), 0, st, p);
   };

@@ -408,7 +408,8 @@ extern "C" int zs_decode_attention_sparse_paged(void* stream, const uint16_t* q,
         reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
       ((q_batch_stride | q_head_stride) & 7))
     return ZS_E_INVAL;
-  if (num_heads / num_heads_k > 16 || batch > 65535) return ZS_E_UNSUPPORTED;
+  if (num_heads / num_heads_k > 16 || batch > 65535 || (int64_t)batch * num_heads > INT_MAX)
+    return ZS_E_UNSUPPORTED;
   const int64_t tiles = (int64_t)top_k * (page_block_size / 16);
   if (tiles > INT_MAX / 2) return ZS_E_OVERFLOW;
   SparseParams p{};
