@@ -270,6 +270,8 @@ def test_select_values_that_are_no_numbers(torch_cuda):
     bounds[table[0, 30].long(), 1] = nan
     q[1, 5, 2] = nan        # every page of one KV head is a tie
     q[2] = 0.0              # every score is 0
+    q[1, 0, 5] = inf        # -inf for pages whose bounds are below 0 there
+    bounds[table[1, ::2].long(), 0, :, 5] = -T.tensor([2.0, 1.0], dtype=T.bfloat16)
     q[3, 0] = T.full((128,), 3e38, dtype=T.bfloat16)
     bounds[table[3].long()] *= 1e38  # products past the range of 32 bits
     check_select(T, q, bounds, table, [950] * 4, 16, 9)
@@ -363,6 +365,17 @@ def test_select_score_distributions(torch_cuda, kind, width, top_k):
     table = T.randperm(width, device="cuda", generator=g).to(T.int32).view(1, width)
     check_select_many(T, q, bounds, table, width * 16, 16, top_k)
     check_select_many(T, q, bounds, table, width * 16, 16, top_k, 0, 0)
+
+
+def test_select_bounds_far_apart(torch_cuda):
+    # a channel whose smallest key is 2^80 times its largest, and of the other sign of what is asked for
+    T = torch_cuda
+    q, bounds, table = make_select(T, 9, 2, 4, 2, 128, 16, 300)
+    q.abs_()
+    bounds[:, :, 0, 7] = -2.0 ** 80
+    bounds[:, 1, 0, 9] = -2.0 ** 40
+    bounds[::3, 0, 1] *= 2.0 ** 70
+    check_select(T, q, bounds, table, [4800, 4000], 16, 31, sink_pages=0, local_pages=0)
 
 
 @pytest.mark.parametrize("how", ["row", "heads", "offset", "four"])

@@ -348,10 +348,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendParams p) 
 // and ranked, ties to the lowest page.  Rows where that cannot be told from a
 // bound (scores or operands so large that products or sums leave fp32's range,
 // values that are no numbers, hundreds of equal scores) are scored in 64 bits as a
-// whole.
-//
-// In 64 bits: 2 score = sum_d q_d (kmax + kmin) + |q_d| (kmax - kmin), each sum
-// off by 2^-53.
+// whole: products are exact there and each of D additions is off by 2^-53.
 struct SelectParams {
   const uint16_t* q;
   int64_t q_batch, q_head;  // strides in elements
@@ -473,7 +470,8 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p)
 }
 
 // The exact score of page lp for one head as a number in its order: NaN as +inf,
-// a page outside the pool 0.  For the D / 8 lanes of a page together.
+// a page outside the pool 0.  For the D / 8 lanes of a page together.  A channel's
+// other product is 0 times its bound: nothing, or NaN where that is not finite.
 __device__ __forceinline__ uint64_t score_key(double x) {
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);  // -0 is 0
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
@@ -496,13 +494,15 @@ __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, int b, int 
   const uint16_t* lo = p.bounds + ((int64_t)block * p.heads_k + h) * 2 * D + 8 * c;
   const u32x4 x = *reinterpret_cast<const u32x4*>(lo), y = *reinterpret_cast<const u32x4*>(lo + D);
   double s = 0;
+  bool odd = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    auto at = [&](const u32x4& v) -> double { return bf16_bits_to_f32(i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xFFFF); };
-    const double q = at(u), k0 = at(x), k1 = at(y);
-    s = fma(q, k1 + k0, s);
-    s = fma(fabs(q), k1 - k0, s);
+    auto at = [&](const u32x4& v) { return i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xFFFF; };
+    const uint32_t q = at(u), k0 = at(x), k1 = at(y);
+    odd |= (k0 & 0x7F80) == 0x7F80 || (k1 & 0x7F80) == 0x7F80;
+    s = fma((double)bf16_bits_to_f32(q), (double)bf16_bits_to_f32(q >> 15 ? k0 : k1), s);
   }
+  if (odd) s = NAN;
   s = dpp_add<0xB1>(s);   // quad_perm:[1,0,3,2]
   s = dpp_add<0x4E>(s);   // quad_perm:[2,3,0,1]
   s = dpp_add<0x141>(s);  // row_half_mirror: eight lanes
