@@ -374,12 +374,12 @@ __device__ __forceinline__ int select_pages(const SelectParams& p, int b) {
 constexpr float kScoreError = 1.02f / (1 << 14), kScoreRest = 0x1p-50f;
 constexpr uint32_t kQuerySmall = 0x0080, kQueryLarge = 0x5D80;  // 2^-126 and 2^60 in bf16
 
-// A wave scores 16 pages for one KV head.  The heads of the same pages run next to
-// one another, so a page's bounds are read from memory as one piece (32 sequences
-// to 64000 tokens, 64 / 8 heads, 271 MB: selection 81.5 -> 71.3 us; with 16 pages a
-// wave in place of 64 69.5, one sequence of 32000 tokens 17.0 -> 12.7).
-constexpr int kScoreWaves = 4;
-
+// A workgroup of one wave scores 16 pages for one KV head.  The heads of the same
+// pages run next to one another, so a page's bounds are read from memory as one
+// piece (32 sequences to 64000 tokens, 64 / 8 heads, 271 MB: selection 81.5 -> 71.3
+// us; with 16 pages a wave in place of 64 69.5).  Workgroups of four waves take 11.1
+// and 64.8 us where these take 10.4 and 65.4 (one sequence of 32000 tokens, the 32 to
+// 64000), 69.5 and 68.3 us with the attention of 16 to 40000.
 // max over the 16 lanes of a row, in all of them
 __device__ __forceinline__ float row_max16(float x) {
   auto step = [&](auto ctrl) {
@@ -410,29 +410,31 @@ __device__ __forceinline__ float row_max16x4(f32x4 v, int l) {
 }
 
 template <int D>
-__global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p) {
+__global__ __launch_bounds__(64) void score_kernel(SelectParams p) {
   constexpr int kC = D / 32;
   const int b = blockIdx.y;
   const int n = select_pages(p, b);
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), g = l & 15, lg = l >> 4;
-  const int item = blockIdx.x * kScoreWaves + w, tile = (int)p.over_heads.div((uint32_t)item);
-  const int h = item - tile * p.heads_k, p0 = 16 * tile;
+  const int l = lane_id(), g = l & 15, lg = l >> 4;
+  const int tile = (int)p.over_heads.div(blockIdx.x), h = blockIdx.x - tile * p.heads_k, p0 = 16 * tile;
   if (n <= p.top_k || p0 >= n) return;
   // lane i: the place of the wave's page i%16, -1 without one
   int block = -1;
   if (p0 + g < n) block = p.table[b * p.table_stride + p0 + g];
   if (block >= p.num_blocks) block = -1;
-  // A page's bounds, 4 D bytes, come as whole rows (an instruction reads 1 KB of
-  // them) and pass through the wave's own LDS into operand order.
-  constexpr int kRow = 4 * D, kPitch = kRow + 16, kRows = 1024 / kRow, kLoads = 2 * kC;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[kScoreWaves][16 * kPitch];
-  uint8_t* lds = smem[w];
+  // A page's bounds, 2 D bytes each, come as whole rows (an instruction reads 1 KB of
+  // them) and pass through LDS into operand order, one after the other (twice the
+  // LDS for both together left the CU fewer waves: 66.8 us for 66.0).
+  constexpr int kRow = 2 * D, kPitch = kRow + 16, kRows = 1024 / kRow;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[16 * kPitch];
   const int lrow = l / (kRow / 16), lcol = 16 * (l % (kRow / 16));
-  const uint8_t* from = reinterpret_cast<const uint8_t*>(p.bounds) + (int64_t)h * kRow + lcol;
-  u32x4 x[kC], y[kC], in[kLoads];
+  const uint8_t* from = reinterpret_cast<const uint8_t*>(p.bounds) + (int64_t)h * 2 * kRow + lcol;
+  u32x4 x[kC], y[kC], in[2 * kC];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i)
-    in[i] = *reinterpret_cast<const u32x4*>(from + (int64_t)max(__shfl(block, i * kRows + lrow), 0) * p.heads_k * kRow);
+  for (int i = 0; i < kC; ++i) {
+    const uint8_t* at = from + (int64_t)max(__shfl(block, i * kRows + lrow), 0) * p.heads_k * (2 * kRow);
+    in[i] = *reinterpret_cast<const u32x4*>(at);
+    in[kC + i] = *reinterpret_cast<const u32x4*>(at + kRow);
+  }
   // the B operands (lane l: head l%16, dims 32c + 8*(l/16)..+7): q's positive and
   // negative parts
   u32x4 qp[kC], qn[kC];
@@ -446,12 +448,13 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_kernel(SelectParams p)
   }
   const uint32_t no_sign = 0x7FFF7FFFu;
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(lds + (i * kRows + lrow) * kPitch + lcol) = in[i];
+  for (int i = 0; i < kC; ++i) *reinterpret_cast<u32x4*>(lds + (i * kRows + lrow) * kPitch + lcol) = in[i];
 #pragma unroll
-  for (int c = 0; c < kC; ++c) {
-    x[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c);
-    y[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c + 2 * D);
-  }
+  for (int c = 0; c < kC; ++c) x[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c);
+#pragma unroll
+  for (int i = 0; i < kC; ++i) *reinterpret_cast<u32x4*>(lds + (i * kRows + lrow) * kPitch + lcol) = in[kC + i];
+#pragma unroll
+  for (int c = 0; c < kC; ++c) y[c] = *reinterpret_cast<const u32x4*>(lds + g * kPitch + 16 * lg + 64 * c);
   f32x4 S = {0.f, 0.f, 0.f, 0.f}, A = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
@@ -1020,8 +1023,8 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   auto launch = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
     if (max_blocks_per_seq > top_k) {
-      const dim3 grid((unsigned)((score_items + kScoreWaves - 1) / kScoreWaves), batch);
-      hipLaunchKernelGGL(score_kernel<D>, grid, dim3(kScoreWaves * 64), 0, st, p);
+      const dim3 grid((unsigned)score_items, batch);
+      hipLaunchKernelGGL(score_kernel<D>, grid, dim3(64), 0, st, p);
     }
     const dim3 rows(batch * num_heads_k);
     if (max_blocks_per_seq <= kPickKeys * 256)
