@@ -21,6 +21,12 @@
 // the output's rounding to bf16 is the only one that shows.  The second one is
 // never 0, or an infinite V would meet it as inf * 0.
 //
+// HBM bounds it where there is enough to read: 64 sequences' 4096 tokens at 5.8 TB/s,
+// and a plain reader of random pages gets 5.65.  One pair of tiles in flight a wave
+// is enough for that; loading the next pair ahead, more waves a workgroup and more
+// splits were slower.  One sequence's 2048 tokens of 8 heads take 6 us and 2.5 for
+// the merge.
+//
 // Tokens at or past the sequence's length, pages that are not in the sequence
 // and table entries outside the pool count for nothing: their scores are masked
 // and their rows are not read (a tile's last valid row is read in their place,
