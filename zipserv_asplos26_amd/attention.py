@@ -368,8 +368,8 @@ def flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cach
     16.  Returns out shaped like q (and softmax_lse [B, H] when asked); a row
     without tokens gives zeros and lse -inf."""
     torch = _torch()
-    shape = q.shape
     q3 = paged._query(q)
+    shape = q.shape
     on = paged._elsewhere(q3)
     if on is not None:
         with on:

@@ -379,12 +379,6 @@ __device__ __forceinline__ int select_pages(const SelectParams& p, int b) {
 constexpr float kScoreError = 1.02f / (1 << 14), kScoreRest = 0x1p-50f;
 constexpr uint32_t kQuerySmall = 0x0080, kQueryLarge = 0x5D80;  // 2^-126 and 2^60 in bf16
 
-// A workgroup of one wave scores 16 pages for one KV head.  The heads of the same
-// pages run next to one another, so a page's bounds are read from memory as one
-// piece (32 sequences to 64000 tokens, 64 / 8 heads, 271 MB: selection 81.5 -> 71.3
-// us; with 16 pages a wave in place of 64 69.5).  Workgroups of four waves take 11.1
-// and 64.8 us where these take 10.4 and 65.4 (one sequence of 32000 tokens, the 32 to
-// 64000), 69.5 and 68.3 us with the attention of 16 to 40000.
 // max over the 16 lanes of a row, in all of them
 __device__ __forceinline__ float row_max16(float x) {
   auto step = [&](auto ctrl) {
@@ -414,6 +408,12 @@ __device__ __forceinline__ float row_max16x4(f32x4 v, int l) {
   return fmaxf(x, dpp<0x128>(x));
 }
 
+// A workgroup of one wave scores 16 pages for one KV head.  The heads of the same
+// pages run next to one another, so a page's bounds are read from memory as one
+// piece (32 sequences to 64000 tokens, 64 / 8 heads, 271 MB: selection 81.5 -> 71.3
+// us; with 16 pages a wave in place of 64 69.5).  Workgroups of four waves take 11.1
+// and 64.8 us where these take 10.4 and 65.4 (one sequence of 32000 tokens, the 32 to
+// 64000), 69.5 and 68.3 us with the attention of 16 to 40000.
 template <int D>
 __global__ __launch_bounds__(64) void score_kernel(SelectParams p) {
   constexpr int kC = D / 32;
@@ -473,13 +473,11 @@ __global__ __launch_bounds__(64) void score_kernel(SelectParams p) {
   float a = row_max16x4(A, l);
   const int at = 4 * lg + 2 * (l & 1) + (l >> 1 & 1);
   // an infinite sum of sizes says that the score is not to be gone by
-  if (__shfl(block, at) < 0 || !(a < INFINITY)) a = INFINITY;
+  if (__shfl(block, at) < 0 || !(a < INFINITY && fabsf(s) < INFINITY)) a = INFINITY;
   if (g < 4 && p0 + at < n) p.scores[((int64_t)b * p.heads_k + h) * p.width + p0 + at] = float2{s, a};
 }
 
-// The exact score of page lp for one head as a number in its order: NaN as +inf,
-// a page outside the pool 0.  For the D / 8 lanes of a page together.  A channel's
-// other product is 0 times its bound: nothing, or NaN where that is not finite.
+// An exact score as a number in its order.
 __device__ __forceinline__ uint64_t score_key(double x) {
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);  // -0 is 0
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
@@ -493,29 +491,47 @@ __device__ __forceinline__ double dpp_add(double x) {
   return x + __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo));
 }
 
+// A page's bounds, eight channels in each of its D / 8 lanes.
+struct PageBounds {
+  u32x4 low, high;
+  bool gone, odd;  // outside the pool; some bound of the lane's is not finite
+};
+
 template <int D>
-__device__ __forceinline__ uint64_t exact_key(const SelectParams& p, int b, int h, int g, int lp, int c) {
-  constexpr int kLanes = D / 8;
-  const u32x4 u = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head + 8 * c);
+__device__ __forceinline__ PageBounds load_bounds(const SelectParams& p, int b, int h, int lp, int c) {
+  PageBounds r;
   const int block = p.table[b * p.table_stride + lp];
-  if (block < 0 || block >= p.num_blocks) return 0;
-  const uint16_t* lo = p.bounds + ((int64_t)block * p.heads_k + h) * 2 * D + 8 * c;
-  const u32x4 x = *reinterpret_cast<const u32x4*>(lo), y = *reinterpret_cast<const u32x4*>(lo + D);
-  double s = 0;
-  bool odd = false;
+  r.gone = block < 0 || block >= p.num_blocks;
+  const uint16_t* at = p.bounds + ((int64_t)(r.gone ? 0 : block) * p.heads_k + h) * 2 * D + 8 * c;
+  r.low = *reinterpret_cast<const u32x4*>(at);
+  r.high = *reinterpret_cast<const u32x4*>(at + D);
+  r.odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    auto bad = [](uint32_t x) { return (x & 0x7F80) == 0x7F80 || (x & 0x7F800000) == 0x7F800000; };
+    r.odd |= bad(r.low[i]) || bad(r.high[i]);
+  }
+  return r;
+}
+
+// The exact score of a page for one head, in all of its lanes: NaN as +inf, a page
+// outside the pool 0.  A channel's other product is 0 times its bound: nothing, or
+// NaN where that is not finite.
+template <int D>
+__device__ __forceinline__ uint64_t exact_key(const SelectParams& p, const PageBounds& k, int b, int h, int g, int c) {
+  const u32x4 u = *reinterpret_cast<const u32x4*>(p.q + b * p.q_batch + (h * p.group + g) * p.q_head + 8 * c);
+  double s = k.odd ? NAN : 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     auto at = [&](const u32x4& v) { return i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xFFFF; };
-    const uint32_t q = at(u), k0 = at(x), k1 = at(y);
-    odd |= (k0 & 0x7F80) == 0x7F80 || (k1 & 0x7F80) == 0x7F80;
-    s = fma((double)bf16_bits_to_f32(q), (double)bf16_bits_to_f32(q >> 15 ? k0 : k1), s);
+    const uint32_t q = at(u);
+    s = fma((double)bf16_bits_to_f32(q), (double)bf16_bits_to_f32(q >> 15 ? at(k.low) : at(k.high)), s);
   }
-  if (odd) s = NAN;
-  s = dpp_add<0xB1>(s);   // quad_perm:[1,0,3,2]
-  s = dpp_add<0x4E>(s);   // quad_perm:[2,3,0,1]
-  s = dpp_add<0x141>(s);  // row_half_mirror: eight lanes
-  if constexpr (kLanes == 16) s = dpp_add<0x140>(s);  // row_mirror
-  return score_key(s != s ? INFINITY : s);
+  s = dpp_add<0xB1>(s);                              // quad_perm:[1,0,3,2]
+  s = dpp_add<0x4E>(s);                              // quad_perm:[2,3,0,1]
+  s = dpp_add<0x141>(s);                             // row_half_mirror: eight lanes
+  if constexpr (D == 128) s = dpp_add<0x140>(s);     // row_mirror
+  return k.gone ? 0 : score_key(s != s ? INFINITY : s);
 }
 
 // One workgroup a (sequence, KV head).  What it takes is a chain of short steps, each
@@ -575,8 +591,10 @@ __device__ void pick_exact(const SelectParams& p, PickLds<NT>& L, int b, int h, 
   const int tid = threadIdx.x, l = lane_id(), w = tid >> 6;
   for (int lp = tid / kLanes; lp < n; lp += NT / kLanes) {
     uint64_t k = lp < p.sink || lp >= n - p.local ? ~0ull : 0;
-    if (k == 0)
-      for (int g = 0; g < p.group; ++g) k = max(k, exact_key<D>(p, b, h, g, lp, tid % kLanes));
+    if (k == 0) {
+      const PageBounds bounds = load_bounds<D>(p, b, h, lp, tid % kLanes);
+      for (int g = 0; g < p.group; ++g) k = max(k, exact_key<D>(p, bounds, b, h, g, tid % kLanes));
+    }
     if (tid % kLanes == 0) keys[lp] = k;
   }
   __threadfence_block();
@@ -818,7 +836,8 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
       constexpr int kLanes = D / 8;  // of a page and a head
       for (int i = tid / kLanes; i < in * p.group; i += NT / kLanes) {
         const int at = i / p.group;
-        const uint64_t k = exact_key<D>(p, b, h, i - at * p.group, L.few_page[at], tid % kLanes);
+        const PageBounds bounds = load_bounds<D>(p, b, h, L.few_page[at], tid % kLanes);
+        const uint64_t k = exact_key<D>(p, bounds, b, h, i - at * p.group, tid % kLanes);
         if (tid % kLanes == 0) atomicMax((unsigned long long*)&L.few_key[at], k);
       }
       __syncthreads();
