@@ -536,11 +536,11 @@ __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, const PageB
 
 // One workgroup a (sequence, KV head).  What it takes is a chain of short steps, each
 // ended by a barrier: so scores are loaded before the row's length is known and stay
-// in registers (kPickKeys a thread; the rest of longer rows is read again), sums
+// in registers (kKeys a thread; the rest of longer rows is read again), sums
 // and maxima run over DPP and ballots, and one pass does all that goes by the window.
-// 8 rows of 2000 pages 8 us, of 8188 10 us, 256 rows of 125..4000 12 us; the same
-// in rolled loops over scores in LDS 9.6 us for the first.
-constexpr int kPickKeys = 8;
+// 8 rows of 2000 pages 7 us, of 8188 10 us, 256 rows of 125..4000 11.5 us.  For the
+// first, eight scores a thread took 8 us and sixteen 9.7, the same steps in rolled
+// loops over scores in LDS 9.6.
 constexpr int kPickBins = 2048;
 constexpr int kPickFew = 256;      // pages of the window that are ranked among themselves
 constexpr int kPickChunk = 65536;  // pages of a bit map
@@ -655,16 +655,16 @@ __device__ void pick_exact(const SelectParams& p, PickLds<NT>& L, int b, int h, 
   }
 }
 
-template <int D, int NT>
+template <int D, int NT, int kKeys>
 __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   constexpr int kWaves = NT / 64;
   __shared__ PickLds<NT> L;
   const int row = blockIdx.x, b = row / p.heads_k, h = row % p.heads_k, tid = threadIdx.x, l = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   float2* scores = p.scores + (int64_t)row * p.width;
-  float2 own[kPickKeys];
+  float2 own[kKeys];
 #pragma unroll
-  for (int j = 0; j < kPickKeys; ++j)  // (what lies behind the row's end is not looked at)
+  for (int j = 0; j < kKeys; ++j)  // (what lies behind the row's end is not looked at)
     own[j] = j * NT + tid < p.width ? scores[j * NT + tid] : float2{0.f, 0.f};
   // (a group has at most 16 heads: 256 pieces of 8 values)
   static_assert(NT >= 256, "a piece a thread");
@@ -681,10 +681,10 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   }
   const int first = p.sink, last = n - p.local;  // the pages between are chosen from
   const int need = p.top_k - p.sink - p.local;
-  const bool whole = n <= kPickKeys * NT;
+  const bool whole = n <= kKeys * NT;
   // A page's score: NaN for one that is always taken, -inf behind the last one.
   auto marked = [&](int i, float x) { return i >= first && i < last ? x : i < n ? NAN : -INFINITY; };
-  float key[kPickKeys], size = 0.f, lo = INFINITY, hi = -INFINITY;
+  float key[kKeys], size = 0.f, lo = INFINITY, hi = -INFINITY;
   auto note = [&](int i, float2 x) {  // the first round's range
     const bool in = i >= first && i < last;
     size = fmaxf(size, in ? x.y : 0.f);
@@ -692,12 +692,12 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     hi = fmaxf(hi, in ? x.x : -INFINITY);
   };
 #pragma unroll
-  for (int j = 0; j < kPickKeys; ++j) {
+  for (int j = 0; j < kKeys; ++j) {
     note(j * NT + tid, own[j]);
     key[j] = marked(j * NT + tid, own[j].x);
   }
   if (!whole)
-    for (int i = kPickKeys * NT + tid; i < last; i += NT) note(i, scores[i]);
+    for (int i = kKeys * NT + tid; i < last; i += NT) note(i, scores[i]);
   {
     const u16x8 u = __builtin_bit_cast(u16x8, query) & (uint16_t)0x7FFF;
     bool odd = false;
@@ -709,9 +709,9 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   if (l == 0) L.red[2][w] = size;
   auto each = [&](auto f) {
 #pragma unroll
-    for (int j = 0; j < kPickKeys; ++j) f(key[j]);
+    for (int j = 0; j < kKeys; ++j) f(key[j]);
     if (!whole)
-      for (int i = kPickKeys * NT + tid; i < n; i += NT) f(marked(i, scores[i].x));
+      for (int i = kKeys * NT + tid; i < n; i += NT) f(marked(i, scores[i].x));
   };
 
   // The window [low, high] that holds the need-th largest score.  A window of too
@@ -815,13 +815,13 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     };
     uint64_t word = 0;  // lane j: of the wave's j-th 64 pages
 #pragma unroll
-    for (int j = 0; j < kPickKeys; ++j) {
+    for (int j = 0; j < kKeys; ++j) {
       const uint64_t m = put(j * NT + tid, key[j]);
       word = l == j ? m : word;
     }
-    if (l < kPickKeys) L.map[l * kWaves + w] = word;
+    if (l < kKeys) L.map[l * kWaves + w] = word;
     if (!whole)
-      for (int i = kPickKeys * NT + tid; i - l < n; i += NT) {
+      for (int i = kKeys * NT + tid; i - l < n; i += NT) {
         const uint64_t m = put(i, i < n ? marked(i, scores[i].x) : -INFINITY);
         if (i < kPickChunk && l == 0) L.map[i / 64] = m;
       }
@@ -868,18 +868,18 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     // every wave sums the bits of all words, and writes its own ones' pages
     if (page >= 0) atomicOr((unsigned long long*)&L.map[page / 64], 1ull << (page & 63));
     __syncthreads();
-    constexpr int kPer = kPickKeys * kWaves > 64 ? 2 : 1;  // words a lane
-    static_assert(kPickKeys * kWaves <= 64 * kPer, "");
+    constexpr int kPer = kKeys * kWaves > 64 ? 2 : 1;  // words a lane
+    static_assert(kKeys * kWaves <= 64 * kPer, "");
     uint64_t m[kPer];
     int c[kPer], sum = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      m[i] = kPer * l + i < kPickKeys * kWaves ? L.map[kPer * l + i] : 0;
+      m[i] = kPer * l + i < kKeys * kWaves ? L.map[kPer * l + i] : 0;
       sum += c[i] = __builtin_popcountll(m[i]);
     }
     const int before = wave_inclusive_scan(sum) - sum;
 #pragma unroll
-    for (int j = 0; j < kPickKeys; ++j) {
+    for (int j = 0; j < kKeys; ++j) {
       const int at = j * kWaves + w, of = at / kPer, i = at % kPer;
       int base = __builtin_amdgcn_readlane(before, of);
       if (kPer == 2 && i) base += __builtin_amdgcn_readlane(c[0], of);
@@ -1053,12 +1053,19 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
       hipLaunchKernelGGL(score_kernel<D>, grid, dim3(64), 0, st, p);
     }
     const dim3 rows(batch * num_heads_k);
-    if (max_blocks_per_seq <= kPickKeys * 256)
-      hipLaunchKernelGGL((pick_kernel<D, 256>), rows, dim3(256), 0, st, p);
-    else if (max_blocks_per_seq <= kPickKeys * 512)
-      hipLaunchKernelGGL((pick_kernel<D, 512>), rows, dim3(512), 0, st, p);
+    auto pick = [&](auto threads, auto keys) {
+      constexpr int NT = decltype(threads)::value;
+      hipLaunchKernelGGL((pick_kernel<D, NT, decltype(keys)::value>), rows, dim3(NT), 0, st, p);
+    };
+    using Four = std::integral_constant<int, 4>;
+    if (max_blocks_per_seq <= 4 * 256)
+      pick(std::integral_constant<int, 256>{}, Four{});
+    else if (max_blocks_per_seq <= 4 * 512)
+      pick(std::integral_constant<int, 512>{}, Four{});
+    else if (max_blocks_per_seq <= 4 * 1024)
+      pick(std::integral_constant<int, 1024>{}, Four{});
     else
-      hipLaunchKernelGGL((pick_kernel<D, 1024>), rows, dim3(1024), 0, st, p);
+      pick(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
   };
   if (head_dim == 128)
     launch(std::integral_constant<int, 128>{});
