@@ -522,7 +522,7 @@ int zs_paged_append(void* stream, const uint16_t* k, const uint16_t* v, int64_t 
  * local_pages of the sequence's ceil(len / page_block_size) pages are taken, then
  * the largest scores, ties to the lowest page.  pages [batch][num_heads_k][top_k]
  * gets them in ascending order, -1 behind.  sink_pages + local_pages <= top_k;
- * at most 16 query heads a KV head, batch * num_heads_k at most 65535.  q:
+ * at most 16 query heads a KV head, batch and num_heads_k at most 65535.  q:
  * [batch][num_heads][head_dim], strides in elements, multiples of 8; q and
  * page_bounds 16-byte aligned.  workspace: the queried bytes, 8-byte aligned. */
 size_t zs_select_kv_pages_workspace_bytes(int batch, int num_heads_k, int max_blocks_per_seq);

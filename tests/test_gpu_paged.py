@@ -378,6 +378,34 @@ def test_select_bounds_far_apart(torch_cuda):
     check_select(T, q, bounds, table, [4800, 4000], 16, 31, sink_pages=0, local_pages=0)
 
 
+def test_many_rows(torch_cuda):
+    # more (sequence, KV head) rows than a dimension of a grid but the first holds
+    T = torch_cuda
+    g = T.Generator(device="cuda").manual_seed(3)
+    batch, heads_k, dim, page, width, top_k = 4500, 16, 64, 16, 6, 3
+    blocks = 400
+    kc, vc = (T.randn(blocks, page, heads_k, dim, device="cuda", generator=g).to(T.bfloat16) for _ in range(2))
+    bounds = T.stack([kc.amin(1), kc.amax(1)], 2)
+    table = T.randint(0, blocks, (batch, width), device="cuda", generator=g, dtype=T.int32)
+    lens = T.randint(0, width * page + 1, (batch,), device="cuda", generator=g, dtype=T.int32)
+    q = T.randn(batch, heads_k, dim, device="cuda", generator=g).to(T.bfloat16)
+    pages = paged.select_kv_pages(q, bounds, table, lens, page, top_k, 0, 0)
+    b, x = bounds[table.long()].double(), q.double()[:, None]
+    s = (b[:, :, :, 1] * x.clamp(min=0) + b[:, :, :, 0] * x.clamp(max=0)).sum(3).transpose(1, 2)  # (batch, heads, width)
+    n = ((lens + page - 1) // page)[:, None, None]
+    s = s.masked_fill(T.arange(width, device="cuda") >= n, -float("inf"))
+    best = s.sort(descending=True, stable=True).indices[..., :top_k]
+    best = best.masked_fill(best >= n, width).sort().values
+    assert T.equal(pages.long(), best.masked_fill(best == width, -1))
+    out, lse = attention.flash_attn_with_kvcache_sparse(q, kc, vc, table, pages, lens, return_softmax_lse=True)
+    some = T.tensor([0, 1, 77, 2222, 4095, 4096, 4499])
+    want, want_lse, tol, lse_tol = ref.attend(q[some].cpu(), kc.cpu(), vc.cpu(), table[some].cpu(), pages[some].cpu(),
+                                              lens[some].tolist())
+    assert ((out[some].cpu().double() - want).abs() <= tol).all()
+    live = (lens[some] > 0).cpu()
+    assert ((lse[some].cpu().double() - want_lse).abs() <= lse_tol)[live].all()
+
+
 @pytest.mark.parametrize("how", ["row", "heads", "offset", "four"])
 def test_select_of_other_strides(torch_cuda, how):
     T = torch_cuda

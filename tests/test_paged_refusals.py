@@ -58,7 +58,7 @@ SELECT = dict(q=P, qb=4096, qh=128, bounds=P, blocks=8, page=16, table=P, stride
     (dict(qh=130), INVAL), (dict(stride=7), INVAL), (dict(heads=30), INVAL), (dict(sink=-1), INVAL),
     (dict(local=-1), INVAL), (dict(sink=2, local=3), INVAL), (dict(sink=2147483647, local=2147483647), INVAL),
     (dict(ws_bytes=2 * 8 * 8 * 8 - 1), INVAL), (dict(page=40), UNSUPPORTED), (dict(dim=80), UNSUPPORTED),
-    (dict(heads=136), UNSUPPORTED), (dict(batch=8192, ws_bytes=1 << 40), UNSUPPORTED),
+    (dict(heads=136), UNSUPPORTED), (dict(batch=65536, ws_bytes=1 << 40), UNSUPPORTED),
     (dict(blocks=1 << 27), OVERFLOW), (dict(width=2 ** 31 - 1, stride=1 << 31, ws_bytes=1 << 50), OVERFLOW)])
 def test_select_refuses(changed, status):
     assert call("zs_select_kv_pages", SELECT, **changed) == status

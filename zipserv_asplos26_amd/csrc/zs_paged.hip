@@ -1020,7 +1020,8 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   if (top_k <= 0 || sink_pages < 0 || local_pages < 0 || (int64_t)sink_pages + local_pages > top_k) return ZS_E_INVAL;
   if (!aligned16(q) || !aligned16(page_bounds) || ((q_batch_stride | q_head_stride) & 7)) return ZS_E_INVAL;
   if (reinterpret_cast<uintptr_t>(workspace) & 7) return ZS_E_INVAL;
-  if (num_heads / num_heads_k > 16 || (int64_t)batch * num_heads_k > 65535) return ZS_E_UNSUPPORTED;
+  if (num_heads / num_heads_k > 16 || batch > 65535 || (int64_t)batch * num_heads_k > INT_MAX)
+    return ZS_E_UNSUPPORTED;
   if (workspace_bytes < zs_select_kv_pages_workspace_bytes(batch, num_heads_k, max_blocks_per_seq))
     return ZS_E_INVAL;
   const int64_t score_items = ((int64_t)max_blocks_per_seq + 15) / 16 * num_heads_k;
