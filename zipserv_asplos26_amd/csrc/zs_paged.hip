@@ -696,8 +696,22 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     note(j * NT + tid, own[j]);
     key[j] = marked(j * NT + tid, own[j].x);
   }
-  if (!whole)
-    for (int i = kKeys * NT + tid; i < last; i += NT) note(i, scores[i]);
+  // The pages past the registers', f(page, its score) for all lanes of a wave that
+  // has one: four loads in flight.
+  auto rest = [&](auto f) {
+    if (whole) return;
+    for (int i0 = kKeys * NT + tid; i0 - l < n; i0 += 4 * NT) {
+      float2 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = scores[min(i0 + j * NT, n - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i0 + j * NT - l >= n) break;  // (uniform)
+        f(i0 + j * NT, x[j]);
+      }
+    }
+  };
+  rest(note);
   {
     const u16x8 u = __builtin_bit_cast(u16x8, query) & (uint16_t)0x7FFF;
     bool odd = false;
@@ -710,8 +724,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   auto each = [&](auto f) {
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) f(key[j]);
-    if (!whole)
-      for (int i = kKeys * NT + tid; i < n; i += NT) f(marked(i, scores[i].x));
+    rest([&](int i, float2 x) { f(marked(i, x.x)); });
   };
 
   // The window [low, high] that holds the need-th largest score.  A window of too
@@ -745,7 +758,6 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     }
     if (need > 0) {
       const float scale = hi > lo ? kPickBins / (hi - lo) : 0.f;
-      const int rest = need;
       each([&](float x) {
         if (x >= lo && x <= hi) atomicAdd(&L.hist[min((int)((x - lo) * scale), kPickBins - 1)], 1);
       });
@@ -779,11 +791,11 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
       __syncthreads();
       const int s = l < kWaves ? L.sum[l] : 0;
       int over = above + incl - sum + __builtin_amdgcn_readlane(wave_inclusive_scan(s) - s, w);
-      if (over < rest && over + sum >= rest) {
+      if (over < need && over + sum >= need) {
         int at = mine;
 #pragma unroll
         for (int i = kPer - 1; i >= 0; --i) {
-          if (over < rest) at = mine + i;
+          if (over < need) at = mine + i;
           over += v[i];
         }
         // the digit's ends, the margin and what the digits' own rounding may be off by
@@ -820,11 +832,10 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
       word = l == j ? m : word;
     }
     if (l < kKeys) L.map[l * kWaves + w] = word;
-    if (!whole)
-      for (int i = kKeys * NT + tid; i - l < n; i += NT) {
-        const uint64_t m = put(i, i < n ? marked(i, scores[i].x) : -INFINITY);
-        if (i < kPickChunk && l == 0) L.map[i / 64] = m;
-      }
+    rest([&](int i, float2 x) {
+      const uint64_t m = put(i, marked(i, x.x));
+      if (i < kPickChunk && l == 0) L.map[i / 64] = m;
+    });
     if (l == 0) atomicAdd(&L.above, taken);
     __syncthreads();
     const int in = L.count, left = p.top_k - L.above;
@@ -897,7 +908,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     if (c0 > 0) {
       for (int i0 = c0; i0 < end; i0 += NT) {
         const int i = i0 + tid;
-        const uint64_t m = __builtin_amdgcn_ballot_w64(i < n && !(marked(i, scores[i < n ? i : 0].x) <= high));
+        const uint64_t m = __builtin_amdgcn_ballot_w64(!(marked(i, scores[min(i, n - 1)].x) <= high));
         if (l == 0 && i < n) L.map[(i - c0) / 64] = m;
       }
       __syncthreads();
