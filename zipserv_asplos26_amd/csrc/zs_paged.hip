@@ -350,10 +350,11 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendParams p) 
 // pick_kernel finds a narrow window that holds the top_k-th largest fp32 score,
 // 2 E wider on both sides: scores above it are taken and scores below it are not,
 // whatever their errors.  What lies in it, a few pages, is scored again in 64 bits
-// and ranked, ties to the lowest page.  Rows where that cannot be told from a
-// bound (scores or operands so large that products or sums leave fp32's range,
-// values that are no numbers, hundreds of equal scores) are scored in 64 bits as a
-// whole: products are exact there and each of D additions is off by 2^-53.
+// and ranked, ties to the lowest page; where it holds hundreds (long rows cut in
+// their middle, equal scores) the choice runs over 64-bit keys.  Rows where the
+// bound says nothing (scores or operands so large that products or sums leave
+// fp32's range, values that are no numbers) are scored in 64 bits as a whole:
+// products are exact there and each of D additions is off by 2^-53.
 struct SelectParams {
   const uint16_t* q;
   int64_t q_batch, q_head;  // strides in elements
@@ -543,6 +544,7 @@ __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, const PageB
 // loops over scores in LDS 9.6.
 constexpr int kPickBins = 2048;
 constexpr int kPickFew = 256;      // pages of the window that are ranked among themselves
+constexpr int kPickList = 4096;    // that are scored by themselves and chosen from with the row
 constexpr int kPickChunk = 65536;  // pages of a bit map
 
 __device__ __forceinline__ float wave_max(float x) { return wave_max16(row_max16(x)); }
@@ -552,6 +554,7 @@ struct PickLds {
   union {
     int hist[kPickBins];
     uint64_t map[kPickChunk / 64];
+    int list[kPickList];
   };
   uint64_t few_key[kPickFew];
   int few_page[kPickFew];
@@ -583,13 +586,33 @@ __device__ __forceinline__ int pick_write(PickLds<NT>& L, int32_t* out, int base
   return base;
 }
 
-// All of a row in 64 bits: the key of the last page taken found digit by digit,
-// 8 bits at a time from the top, until a digit's pages are all taken or none is left.
+// A row by keys of 64 bits: the key of the last page taken found digit by digit, 8
+// bits at a time from the top, until a digit's pages are all taken or none is left.
+// Keys are the exact scores of the pages whose fp32 scores lie in [low, high], at
+// most kPickList of them, and the most or least for those above or below; or of
+// all pages (`window` false).
 template <int D, int NT>
-__device__ void pick_exact(const SelectParams& p, PickLds<NT>& L, int b, int h, int n, uint64_t* keys, int32_t* out) {
+__device__ void pick_exact(const SelectParams& p, PickLds<NT>& L, int b, int h, int n, float2* scores, int32_t* out,
+                           bool window, float low, float high) {
   constexpr int kLanes = D / 8;
   const int tid = threadIdx.x, l = lane_id(), w = tid >> 6;
-  for (int lp = tid / kLanes; lp < n; lp += NT / kLanes) {
+  uint64_t* keys = reinterpret_cast<uint64_t*>(scores);
+  if (tid == 0) L.count = 0;
+  __syncthreads();
+  if (window) {
+    for (int i = tid; i < n; i += NT) {
+      const float x = scores[i].x;
+      const bool always = i < p.sink || i >= n - p.local;
+      if (always || x > high || x < low)
+        keys[i] = always || x > high ? ~0ull : 0;
+      else
+        L.list[min(atomicAdd(&L.count, 1), kPickList - 1)] = i;
+    }
+    __syncthreads();
+  }
+  const int count = window ? L.count : n;
+  for (int i = tid / kLanes; i < count; i += NT / kLanes) {
+    const int lp = window ? L.list[i] : i;
     uint64_t k = lp < p.sink || lp >= n - p.local ? ~0ull : 0;
     if (k == 0) {
       const PageBounds bounds = load_bounds<D>(p, b, h, lp, tid % kLanes);
@@ -731,7 +754,7 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   // many pages is cut again.
   float low = -FLT_MAX, high = FLT_MAX;
   int page = -1;  // of the window's, if this thread's one is taken
-  bool exact = false;
+  bool exact = false, window = false;  // by 64-bit keys; of the window's pages alone
   for (int round = 0;; ++round) {
     if (round > 0) {
       lo = INFINITY, hi = -INFINITY;
@@ -867,12 +890,13 @@ __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
     }
     if (round == 2) {
       exact = true;
+      window = in <= kPickList;
       break;
     }
   }
   if (exact) {  // (uniform)
     __syncthreads();
-    pick_exact<D, NT>(p, L, b, h, n, reinterpret_cast<uint64_t*>(scores), out);
+    pick_exact<D, NT>(p, L, b, h, n, scores, out, window, low, high);
     return;
   }
   if (whole) {
