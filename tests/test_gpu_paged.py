@@ -316,7 +316,8 @@ def check_select_many(T, q, bounds, table, length, page, top_k, sink=1, local=1)
 
 
 @pytest.mark.parametrize("width,top_k", [(2048, 100), (2049, 1000), (8192, 8191), (8200, 64), (40000, 700),
-                                         (65536, 300), (70001, 5000), (140000, 64)])
+                                         (65536, 300), (70001, 5000), (140000, 64), (62500, 30000),
+                                         (140000, 70000)])
 def test_select_long_sequence(torch_cuda, width, top_k):
     # more pages than a workgroup holds in registers, and than one bit map of them
     T = torch_cuda
