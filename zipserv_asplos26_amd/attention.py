@@ -370,18 +370,18 @@ def flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cach
     torch = _torch()
     q3 = paged._query(q)
     shape = q.shape
-    on = paged._elsewhere(q3)
-    if on is not None:
-        with on:
+    here = paged._here(q3)
+    if here is None:
+        with torch.cuda.device(q3.device):
             return flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cache_seqlens,
                                                   softmax_scale, num_splits, return_softmax_lse)
+    device, stream = here
     B, H, D = q3.shape
-    device = q3.get_device()
     paged._check(k_cache, "k_cache", torch.bfloat16, (None, None, None, D), device)
     size = k_cache.shape
     paged._check(v_cache, "v_cache", torch.bfloat16, size, device)
     nblocks, page, Hkv, _ = size
-    table, stride, width = paged._table(block_table, B, device)
+    table, row, width = paged._table(block_table, B, device)
     lens = paged._lengths(cache_seqlens, B, device)
     paged._check(pages, "pages", torch.int32, (B, Hkv, None), device)
     top_k = pages.shape[2]
@@ -395,8 +395,8 @@ def flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cach
     wsb = paged._bytes("zs_decode_attention_sparse_workspace_bytes", B, H, Hkv, D, top_k, page, splits)
     ws = torch.empty(wsb, dtype=torch.uint8, device=at) if wsb else None
     check("zs_decode_attention_sparse_paged", lib().zs_decode_attention_sparse_paged(
-        _stream(), q3.data_ptr(), q0, q1, k_cache.data_ptr(), v_cache.data_ptr(), nblocks, page, table.data_ptr(),
-        stride, width, pages.data_ptr(), top_k, lens.data_ptr(), B, H, Hkv, D, scale, out.data_ptr(), _dptr(lse),
+        stream, q3.data_ptr(), q0, q1, k_cache.data_ptr(), v_cache.data_ptr(), nblocks, page, table.data_ptr(),
+        row, width, pages.data_ptr(), top_k, lens.data_ptr(), B, H, Hkv, D, scale, out.data_ptr(), _dptr(lse),
         _dptr(ws), wsb, splits))
     return (out, lse) if return_softmax_lse else out
 

@@ -24,11 +24,15 @@ from ._lib import check, lib
 from .codec import _dptr, _stream, _torch
 
 
-def _elsewhere(t):
-    """None where t's device is the current one, whose current stream a call goes
-    to, else the context that makes it so."""
-    cuda = _torch().cuda
-    return None if t.get_device() == cuda.current_device() else cuda.device(t.device)
+def _here(t):
+    """The index of t's device and its current stream, which a call goes to; None
+    where another device is the current one."""
+    torch = _torch()
+    device = t.get_device()
+    if device != torch.cuda.current_device():
+        return None
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return device, _stream() if raw is None else raw(device)
 
 
 def _check(t, name, dtype, shape, device=None, contiguous=True):
@@ -147,12 +151,13 @@ def plan_paged_step(context_lens, new_lens, block_table, free_pages, num_free, p
     torch = _torch()
     i32 = torch.int32
     _check(context_lens, "context_lens", i32, (None,))
-    on = _elsewhere(context_lens)
-    if on is not None:
-        with on:
+    here = _here(context_lens)
+    if here is None:
+        with torch.cuda.device(context_lens.device):
             return plan_paged_step(context_lens, new_lens, block_table, free_pages, num_free, page_block_size,
                                    max_tokens)
-    device, batch = context_lens.get_device(), context_lens.shape[0]
+    device, stream = here
+    batch = context_lens.shape[0]
     _check(new_lens, "new_lens", i32, (batch,), device)
     _check(block_table, "block_table", i32, (batch, None), device, contiguous=False)
     width = block_table.shape[1]
@@ -169,7 +174,7 @@ def plan_paged_step(context_lens, new_lens, block_table, free_pages, num_free, p
     out = torch.empty(3 * most + 2 * batch + 5, dtype=i32, device=context_lens.device)
     at = out.data_ptr()
     check("zs_paged_plan", lib().zs_paged_plan(
-        _stream(), context_lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), stride, width,
+        stream, context_lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), stride, width,
         free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), int(page_block_size), most, at,
         at + 4 * most, at + 8 * most, at + 12 * most, at + 12 * most + 4 * batch, at + 12 * most + 8 * batch + 4))
     return PagedPlan(*torch.split_with_sizes(out, (most, most, most, batch, batch + 1, 4)))
@@ -187,12 +192,12 @@ def append_paged_kv(k, v, k_cache, v_cache, slots, page_bounds=None) -> None:
     torch = _torch()
     bf16 = torch.bfloat16
     _check(k_cache, "k_cache", bf16, (None, None, None, None))
-    on = _elsewhere(k_cache)
-    if on is not None:
-        with on:
+    here = _here(k_cache)
+    if here is None:
+        with torch.cuda.device(k_cache.device):
             return append_paged_kv(k, v, k_cache, v_cache, slots, page_bounds)
-    device, size = k_cache.get_device(), k_cache.shape
-    blocks, page, heads_k, dim = size
+    device, stream = here
+    blocks, page, heads_k, dim = size = k_cache.shape
     _check(v_cache, "v_cache", bf16, size, device)
     _check(slots, "slots", torch.int32, (None,), device)
     n = slots.shape[0]
@@ -203,7 +208,7 @@ def append_paged_kv(k, v, k_cache, v_cache, slots, page_bounds=None) -> None:
     k, k0, k1 = _rows(k)
     v, v0, v1 = _rows(v)
     check("zs_paged_append", lib().zs_paged_append(
-        _stream(), k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, k_cache.data_ptr(),
+        stream, k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, k_cache.data_ptr(),
         v_cache.data_ptr(), _dptr(page_bounds), blocks, page, heads_k, dim))
 
 
@@ -221,16 +226,16 @@ def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size:
     lowest page; sequences of at most top_k pages keep them all."""
     torch = _torch()
     q = _query(q)
-    on = _elsewhere(q)
-    if on is not None:
-        with on:
+    here = _here(q)
+    if here is None:
+        with torch.cuda.device(q.device):
             return select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size, top_k, sink_pages,
                                    local_pages)
+    device, stream = here
     batch, heads, dim = q.shape
-    device = q.get_device()
     _check(page_bounds, "page_bounds", torch.bfloat16, (None, None, 2, dim), device)
     blocks, heads_k = page_bounds.shape[:2]
-    table, stride, width = _table(block_table, batch, device)
+    table, row, width = _table(block_table, batch, device)
     lens = _lengths(cache_seqlens, batch, device)
     top_k, sink, local = int(top_k), int(sink_pages), int(local_pages)
     if top_k <= 0 or sink < 0 or local < 0 or sink + local > top_k:
@@ -243,7 +248,7 @@ def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size:
     need = _bytes("zs_select_kv_pages_workspace_bytes", batch, heads_k, width)
     ws = torch.empty(need, dtype=torch.uint8, device=at)
     check("zs_select_kv_pages", lib().zs_select_kv_pages(
-        _stream(), q.data_ptr(), q0, q1, page_bounds.data_ptr(), blocks, int(page_block_size), table.data_ptr(),
-        stride, width, lens.data_ptr(), batch, heads, heads_k, dim, top_k, sink, local, pages.data_ptr(),
+        stream, q.data_ptr(), q0, q1, page_bounds.data_ptr(), blocks, int(page_block_size), table.data_ptr(),
+        row, width, lens.data_ptr(), batch, heads, heads_k, dim, top_k, sink, local, pages.data_ptr(),
         ws.data_ptr(), need))
     return pages
