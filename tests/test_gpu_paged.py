@@ -128,7 +128,8 @@ def run_slots(rng, blocks, page, runs):
     (8, 128, 16, [(0, 1)], 0), (8, 128, 16, [(15, 1), (3, 1), (0, 1)], 2), (8, 128, 16, [(5, 40), (0, 16), (9, 7)], 0),
     (1, 64, 16, [(5, 40), (0, 33), (9, 7)], 70), (16, 64, 128, [(100, 300), (0, 128), (1, 1)], 0),
     (2, 128, 64, [(63, 130)], 1), (3, 128, 48, [(0, 48), (47, 1), (46, 2), (20, 60)], 0),
-    (5, 64, 256, [(250, 520), (0, 1), (17, 239)], 5), (8, 128, 16, [(i % 16, 1) for i in range(65)], 0)])
+    (5, 64, 256, [(250, 520), (0, 1), (17, 239)], 5), (1, 128, 1040, [(1000, 2200), (3, 900)], 0),
+    (8, 128, 16, [(i % 16, 1) for i in range(65)], 0)])
 @pytest.mark.parametrize("with_bounds", [True, False])
 def test_append(torch_cuda, heads_k, dim, page, runs, tail, with_bounds):
     T = torch_cuda
@@ -234,7 +235,8 @@ def check_select(T, q, bounds, table, lens, page, top_k, **kw):
 @pytest.mark.parametrize("heads,heads_k,dim,page,width,top_k,sink,local", [
     (8, 8, 128, 16, 40, 5, 1, 1), (32, 8, 128, 16, 300, 20, 1, 1), (64, 8, 64, 16, 70, 7, 0, 0),
     (16, 1, 128, 32, 33, 32, 4, 4), (28, 4, 64, 48, 90, 1, 0, 1), (5, 5, 128, 16, 20, 2, 2, 0),
-    (40, 8, 128, 64, 257, 64, 1, 3), (2, 2, 64, 16, 3, 8, 1, 1), (30, 2, 128, 256, 65, 3, 0, 0)])
+    (40, 8, 128, 64, 257, 64, 1, 3), (2, 2, 64, 16, 3, 8, 1, 1), (30, 2, 128, 256, 65, 3, 0, 0), (16, 1, 64, 1040, 40, 6, 1, 2),
+    (3, 3, 128, 16, 2100, 30, 1, 1), (4, 2, 64, 16, 4200, 9, 0, 1)])
 def test_select(torch_cuda, heads, heads_k, dim, page, width, top_k, sink, local):
     T = torch_cuda
     most = width * page

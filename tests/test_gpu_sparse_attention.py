@@ -65,7 +65,8 @@ def check(T, q, kc, vc, table, pages, lens, scale=None, q_dev=None, **kw):
 @pytest.mark.parametrize("splits", [1, 0, 3])
 @pytest.mark.parametrize("heads,heads_k,dim,page,width,top_k", [
     (1, 1, 128, 16, 3, 1), (8, 8, 64, 16, 9, 4), (32, 8, 128, 16, 70, 60), (16, 1, 128, 32, 20, 18),
-    (28, 4, 64, 48, 12, 12), (64, 8, 128, 64, 9, 7), (30, 2, 64, 256, 3, 3), (5, 5, 128, 128, 4, 3)])
+    (28, 4, 64, 48, 12, 12), (64, 8, 128, 64, 9, 7), (30, 2, 64, 256, 3, 3), (5, 5, 128, 128, 4, 3),
+    (16, 1, 64, 1040, 2, 2)])
 def test_sparse_attention(torch_cuda, heads, heads_k, dim, page, width, top_k, splits):
     T = torch_cuda
     rng = random.Random(width * page + splits)
@@ -174,6 +175,29 @@ def test_splits(torch_cuda, splits):
     pages = some_pages(T, random.Random(5), lens, 1, 16, 561, 563)
     poison(T, kc, vc, table, pages, lens)
     check(T, q, kc, vc, table, pages, lens, num_splits=splits)
+
+
+@pytest.mark.parametrize("how", ["slice", "transposed", "shared"])
+def test_tables_of_other_strides(torch_cuda, how):
+    # a part of a wider table, one that is laid out by columns, one row for all; lengths past the table's pages
+    T = torch_cuda
+    q, kc, vc, table = make(T, 12, 3, 4, 2, 64, 16, 6)
+    lens, dev = [96, 200, 50], table.cuda()
+    if how == "slice":
+        dev = T.full((3, 20), 10 ** 6, dtype=T.int32, device="cuda")
+        dev[:, 4:10] = table.cuda()
+        dev = dev[:, 4:10]
+    elif how == "transposed":
+        dev = dev.t().contiguous().t()
+    else:
+        table = table[:1].expand(3, 6)
+        dev = dev[:1].expand(3, 6)
+    pages = some_pages(T, random.Random(3), lens, 2, 16, 4, 6)
+    want, want_lse, tol, lse_tol = ref.attend(q, kc, vc, table, pages, lens)
+    got, lse = attention.flash_attn_with_kvcache_sparse(q.cuda(), kc.cuda(), vc.cuda(), dev, pages.cuda(),
+                                                        T.tensor(lens, dtype=T.int32, device="cuda"),
+                                                        return_softmax_lse=True)
+    assert ((got.cpu().double() - want).abs() <= tol).all() and ((lse.cpu().double() - want_lse).abs() <= lse_tol).all()
 
 
 @pytest.mark.parametrize("how", ["row", "heads", "offset", "four"])
