@@ -264,3 +264,79 @@ def test_sparse_attention_refuses(torch_cuda):
         d = {**dict(q=q, kc=kc, vc=vc, table=table, pages=pages, lens=lens), **a}
         with pytest.raises(ValueError):
             attention.flash_attn_with_kvcache_sparse(d["q"], d["kc"], d["vc"], d["table"], d["pages"], d["lens"])
+
+
+def one_channel(T, batch, heads_k, dim, score, v):
+    """A page of tokens with given scores q.k, exact in fp32 (q is 1 in channel 0 alone): score (batch, heads_k,
+    tokens), v (batch, heads_k, tokens, dim)."""
+    n = score.shape[2]
+    q = T.zeros(batch, heads_k, dim, dtype=T.bfloat16)
+    q[..., 0] = 1
+    kc = T.zeros(batch, 16, heads_k, dim, dtype=T.bfloat16)
+    vc = T.zeros_like(kc)
+    kc[:, :n, :, 0] = score.transpose(1, 2).to(T.bfloat16)
+    vc[:, :n] = v.transpose(1, 2).to(T.bfloat16)
+    table = T.arange(batch, dtype=T.int32).view(batch, 1)
+    pages = T.zeros(batch, heads_k, 1, dtype=T.int32)
+    return q, kc, vc, table, pages, [n] * batch
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_enter_the_product_as_fp32(torch_cuda, dim):
+    # four tokens whose weighted values cancel: each of the last three takes away what its forerunners leave, to 8
+    # bits, so 2^-27 of them is left and the output's rounding hides nothing.  What may be left of the sizes: a
+    # weight is off by 2^-24 for the scale, as much for its product with the score (below 1 in size) and 2^-23 for
+    # the exponential, 4 in all; 12 additions (a weight is at most 3 bf16) by 2^-23 each, 24.  A weight of 16 bits
+    # is off by up to 2^-16, half of that in relation to both sizes.
+    T = torch_cuda
+    g = T.Generator().manual_seed(dim)
+    batch, heads_k = 16, 8
+    score = -T.rand(batch, heads_k, 4, generator=g).to(T.bfloat16)
+    score[..., 0] = 0
+    w = score.double().exp()
+    v = T.zeros(batch, heads_k, 4, dim, dtype=T.bfloat16)
+    v[..., 1, :] = (1 + T.rand(batch, heads_k, dim, generator=g)).to(T.bfloat16)
+    for t in (0, 2, 3):
+        left = (w[..., None] * v.double()).sum(2)
+        v[..., t, :] = (-left / w[..., t, None]).to(T.bfloat16)
+    q, kc, vc, table, pages, lens = one_channel(T, batch, heads_k, dim, score, v)
+    out = attention.flash_attn_with_kvcache_sparse(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), pages.cuda(), 4,
+                                                   softmax_scale=1.0).cpu().double()
+    w = w / w.sum(2, keepdim=True)
+    want = (w[..., None] * v.double()).sum(2)
+    sizes = (w[..., None] * v.double().abs()).sum(2)
+    far = (out - want).abs() - want.abs() * (2.0 ** -8 + 2.0 ** -20)
+    assert (far <= 28 * 2.0 ** -24 * sizes).all(), float((far / sizes).max() * 2 ** 24)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_of_nothing(torch_cuda, dim):
+    # a weight that underflows (e^-200) takes nothing of the largest value, and no other weight more than its part
+    T = torch_cuda
+    score = T.tensor([0.0, -200.0, -75.0]).expand(3, 2, 3)
+    v = T.zeros(3, 2, 3, dim)
+    v[..., 0, :] = 1.0
+    v[..., 1, :] = 3.0e38
+    v[1, :, 2] = 2.0e32  # e^-75 of it: 0.5
+    v[2, :, 1] *= -1
+    want, _, tol, _ = ref.attend(*(x := one_channel(T, 3, 2, dim, score, v)), scale=1.0)
+    out = attention.flash_attn_with_kvcache_sparse(*(y.cuda() for y in x[:5]), 3, softmax_scale=1.0).cpu().double()
+    assert ((out - want).abs() <= tol).all(), (out - want).abs().max()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinite_values_with_small_weights_show(torch_cuda, dim):
+    # weights of 2^-n, which one bf16 holds, and others, down to the smallest normal number
+    T = torch_cuda
+    for scale, scores in ((0.6931471805599453, [-1, -7, -30, -64, -100, -110, -120, -125]),
+                          (1.0, [-0.5, -3.3, -40.0, -60.0, -70.0, -76.0, -82.0, -86.5])):
+        score = T.zeros(8, 1, 2)
+        score[:, 0, 1] = T.tensor(scores)
+        v = T.ones(8, 1, 2, dim)
+        v[:, :, 1, 1] = float("inf")
+        v[:, :, 1, 5] = -float("inf")
+        x = one_channel(T, 8, 1, dim, score, v)
+        out = attention.flash_attn_with_kvcache_sparse(*(y.cuda() for y in x[:5]), 2, softmax_scale=scale).cpu()
+        assert (out[..., 1] == float("inf")).all() and (out[..., 5] == -float("inf")).all(), out[..., 0, :8]
+        rest = [i for i in range(dim) if i not in (1, 5)]
+        assert (out[..., rest] == 1).all()

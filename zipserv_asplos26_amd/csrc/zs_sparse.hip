@@ -17,9 +17,11 @@
 //   l the weights of head l%16 for tokens 4*(l/16)..+3 of both tiles, which is
 //   the B operand if k index 8*(l/16) + j stands for token 4*(l/16) + j%4 of
 //   tile j/4; V^T in that order are two ds_read_b64_tr_b16 of the V tiles.
-// A weight enters the product as the sum of two bf16, so it keeps 16 bits, and
-// the output's rounding to bf16 is the only one that shows.  The second one is
-// never 0, or an infinite V would meet it as inf * 0.
+// A weight enters the product as the sum of three bf16, all of its 24 bits, so
+// the output's rounding to bf16 is the only one that shows.  None of the three is 0
+// unless the weight is, or an infinite V would meet it as inf * 0: a part is what
+// stands above one step less than the number, which leaves a rest, and 2^-133 (the
+// smallest bf16, of a weight of 2^-126 or more) where that is less.
 //
 // HBM bounds it where there is enough to read: 64 sequences' 4096 tokens at 5.8 TB/s,
 // and a plain reader of random pages gets 5.65.  One pair of tiles in flight a wave
@@ -34,7 +36,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -66,6 +67,8 @@ struct SparseParams {
   FastDiv tiles;            // 16-token tiles of a page
   float scale_log2;
 };
+
+constexpr uint32_t kLeastPart = 0x00010000;  // 2^-133 in fp32: the smallest bf16
 
 template <int D, int W>
 struct SparseLds {
@@ -189,15 +192,23 @@ __global__ __launch_bounds__(W * 64) void sparse_attn_kernel(SparseParams p) {
         for (int k = 0; k < kO; ++k) O[k] *= alpha;
       }
       m_run = m_new;
-      // the weights as a sum of two bf16 each: the upper half cut off, the rest
-      // (exact in fp32) rounded
-      u32x4 hi, lo;
+      // the weights as a sum of three bf16 each: the upper half of one fp32 step less,
+      // the same of the rest, and what is left (eight bits at most, exact)
+      u32x4 hi, mid, lo;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t x = __float_as_uint(e[2 * j]), y = __float_as_uint(e[2 * j + 1]);
-        hi[j] = __builtin_amdgcn_perm(y, x, 0x07060302);
-        lo[j] = pack_bf16x2(fmaxf(e[2 * j] - __uint_as_float(x & 0xFFFF0000u), FLT_MIN),
-                            fmaxf(e[2 * j + 1] - __uint_as_float(y & 0xFFFF0000u), FLT_MIN));
+        uint32_t a[2], c[2], d[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t u = __float_as_uint(e[2 * j + i]), least = min(u, kLeastPart);
+          a[i] = __builtin_elementwise_sub_sat(u, 1u) & 0xFFFF0000u;
+          const float r = e[2 * j + i] - __uint_as_float(a[i]);
+          c[i] = max(__builtin_elementwise_sub_sat(__float_as_uint(r), 1u), least) & 0xFFFF0000u;
+          d[i] = (uint32_t)max((int)__float_as_uint(r - __uint_as_float(c[i])), (int)least);
+        }
+        hi[j] = __builtin_amdgcn_perm(a[1], a[0], 0x07060302);
+        mid[j] = __builtin_amdgcn_perm(c[1], c[0], 0x07060302);
+        lo[j] = __builtin_amdgcn_perm(d[1], d[0], 0x07060302);
       }
       if (n0 + n1 < 32) {  // (uniform)
 #pragma unroll
@@ -218,6 +229,7 @@ __global__ __launch_bounds__(W * 64) void sparse_attn_kernel(SparseParams p) {
         const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(t_lds + 16 * kPitch + vrd + 32 * k));
         const bf16x8 A = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
         O[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, as_bf16x8(hi), O[k], 0, 0, 0);
+        O[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, as_bf16x8(mid), O[k], 0, 0, 0);
         O[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, as_bf16x8(lo), O[k], 0, 0, 0);
       }
     }
