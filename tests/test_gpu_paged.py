@@ -558,3 +558,27 @@ def test_two_streams_at_once(torch_cuda):
         for g in got:
             for x, y in zip(g[1:], want[1:]):
                 assert T.equal(x, y)
+
+
+# ------------------------------------------------------------------------------------------------------------
+# Numbers that a C int does not hold
+# ------------------------------------------------------------------------------------------------------------
+def test_numbers_past_32_bits_are_refused(torch_cuda):
+    # each is a small, valid number modulo 2^32
+    T, big = torch_cuda, 2 ** 32
+    q, bounds, table = (x.cuda() for x in make_select(T, 9, 3, 4, 2, 64, 16, 5))
+    kc = T.zeros(len(bounds), 16, 2, 64, dtype=T.bfloat16, device="cuda")
+    i3, wide = ints(T, [1, 2, 3]), table[:, :1].expand(3, big + 1)
+    pages = T.zeros(3, 2, 2, dtype=T.int32, device="cuda")
+    plan = lambda page, most: paged.plan_paged_step(i3, i3, table, i3, i3[2:], page, most)  # noqa: E731
+    select = lambda q, table, page, top_k: paged.select_kv_pages(q, bounds, table, i3, page, top_k)  # noqa: E731
+    attend = lambda q, table, splits: attention.flash_attn_with_kvcache_sparse(  # noqa: E731
+        q, kc, kc, table, pages, i3, num_splits=splits)
+    many = q[:, :1].expand(3, big + 4, 64)
+    for call in [lambda: plan(16, big + 4), lambda: plan(big + 16, 4), lambda: select(q, table, big + 16, 2),
+                 lambda: select(q, table, 16, big + 2), lambda: select(q, wide, 16, 2), lambda: select(many, table, 16, 2),
+                 lambda: attend(q, table, big + 1), lambda: attend(q, table, 1 - big), lambda: attend(q, wide, 1),
+                 lambda: attend(many, table, 1),
+                 lambda: paged.plan_paged_step(i3, i3, wide, i3, i3[2:], 16, 4)]:
+        with pytest.raises(ValueError):
+            call()

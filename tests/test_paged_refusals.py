@@ -121,3 +121,10 @@ def test_reference_bound_is_a_bound():
     for h, p in itertools.product(range(2), range(3)):
         most = (q[0, 2 * h:2 * h + 2].double() @ keys[p, :, h].double().t()).max()
         assert most <= s[h, p]
+
+
+def test_python_refuses_numbers_that_a_c_int_does_not_hold():
+    assert [paged._whole(n, "n") for n in (0, -1, 2 ** 31 - 1, True, 7.0)] == [0, -1, 2 ** 31 - 1, 1, 7]
+    for n in (2 ** 31, 2 ** 32 + 4, -2 ** 31, -2 ** 32 + 1):
+        with pytest.raises(ValueError, match="2\\^31"):
+            paged._whole(n, "n")

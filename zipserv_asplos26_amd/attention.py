@@ -388,7 +388,7 @@ def flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cach
     if Hkv == 0 or H % Hkv:
         raise ValueError(f"{H} query heads do not share {Hkv} KV heads evenly")
     scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
-    splits, at = int(num_splits), q3.device
+    splits, at = paged._whole(num_splits, "num_splits"), q3.device
     q3, q0, q1 = paged._rows(q3)
     out = paged._new_like(q3, shape)
     lse = torch.empty((B, H), dtype=torch.float32, device=at) if return_softmax_lse else None

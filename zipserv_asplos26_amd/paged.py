@@ -35,9 +35,20 @@ def _here(t):
     return device, _stream() if raw is None else raw(device)
 
 
+_MOST = 2 ** 31 - 1  # of a number that goes to the library as a C int (which takes others modulo 2^32)
+
+
+def _whole(n, name):
+    """n as a whole number that a C int holds."""
+    n = int(n)
+    if not -_MOST <= n <= _MOST:
+        raise ValueError(f"{name} must be less than 2^31, got {n}")
+    return n
+
+
 def _check(t, name, dtype, shape, device=None, contiguous=True):
-    """Raises where t is not a GPU tensor of these (shape: None where any size will
-    do; device: its index)."""
+    """Raises where t is not a GPU tensor of these (shape: None where any size that
+    a C int holds will do; device: its index)."""
     try:  # (a right tensor takes 0.4 us)
         if t.dtype is dtype and (t.is_cuda if device is None else t.get_device() == device) and \
                 (not contiguous or t.is_contiguous()):
@@ -46,7 +57,7 @@ def _check(t, name, dtype, shape, device=None, contiguous=True):
                 return
             if len(got) == len(shape):
                 for n, m in zip(shape, got):
-                    if n is not None and n != m:
+                    if m > _MOST if n is None else n != m:
                         break
                 else:
                     return
@@ -61,6 +72,8 @@ def _check(t, name, dtype, shape, device=None, contiguous=True):
         raise ValueError(f"{name} must be on cuda:{device}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+    if t.shape and max(t.shape) > _MOST:
+        raise ValueError(f"{name} must have less than 2^31 entries a dimension, got {tuple(t.shape)}")
     want = ", ".join("*" if n is None else str(n) for n in shape)
     raise ValueError(f"{name} must be ({want}), got {tuple(t.shape)}")
 
@@ -101,7 +114,7 @@ def _query(q):
     if isinstance(q, torch.Tensor):
         if q.dim() == 4 and q.shape[1] == 1:
             q = q[:, 0]
-        if q.dtype is torch.bfloat16 and q.is_cuda and q.dim() == 3:
+        if q.dtype is torch.bfloat16 and q.is_cuda and q.dim() == 3 and q.shape[0] <= _MOST and q.shape[1] <= _MOST:
             return q
     _check(q, "q", torch.bfloat16, (None, None, None), contiguous=False)
     return q
@@ -168,14 +181,14 @@ def plan_paged_step(context_lens, new_lens, block_table, free_pages, num_free, p
         raise ValueError("block_table is written in place: its rows must be contiguous and apart")
     _check(free_pages, "free_pages", i32, (None,), device)
     _check(num_free, "num_free", i32, (1,), device)
-    most = int(max_tokens)
+    page, most = _whole(page_block_size, "page_block_size"), _whole(max_tokens, "max_tokens")
     if most < 0:
         raise ValueError("max_tokens must not be negative")
     out = torch.empty(3 * most + 2 * batch + 5, dtype=i32, device=context_lens.device)
     at = out.data_ptr()
     check("zs_paged_plan", lib().zs_paged_plan(
         stream, context_lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), stride, width,
-        free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), int(page_block_size), most, at,
+        free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), page, most, at,
         at + 4 * most, at + 8 * most, at + 12 * most, at + 12 * most + 4 * batch, at + 12 * most + 8 * batch + 4))
     return PagedPlan(*torch.split_with_sizes(out, (most, most, most, batch, batch + 1, 4)))
 
@@ -237,7 +250,8 @@ def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size:
     blocks, heads_k = page_bounds.shape[:2]
     table, row, width = _table(block_table, batch, device)
     lens = _lengths(cache_seqlens, batch, device)
-    top_k, sink, local = int(top_k), int(sink_pages), int(local_pages)
+    page, top_k = _whole(page_block_size, "page_block_size"), _whole(top_k, "top_k")
+    sink, local = int(sink_pages), int(local_pages)  # (not below 0, and top_k at most together)
     if top_k <= 0 or sink < 0 or local < 0 or sink + local > top_k:
         raise ValueError("top_k must be positive and hold sink_pages and local_pages")
     if heads_k == 0 or heads % heads_k:
@@ -248,7 +262,7 @@ def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size:
     need = _bytes("zs_select_kv_pages_workspace_bytes", batch, heads_k, width)
     ws = torch.empty(need, dtype=torch.uint8, device=at)
     check("zs_select_kv_pages", lib().zs_select_kv_pages(
-        stream, q.data_ptr(), q0, q1, page_bounds.data_ptr(), blocks, int(page_block_size), table.data_ptr(),
+        stream, q.data_ptr(), q0, q1, page_bounds.data_ptr(), blocks, page, table.data_ptr(),
         row, width, lens.data_ptr(), batch, heads, heads_k, dim, top_k, sink, local, pages.data_ptr(),
         ws.data_ptr(), need))
     return pages
