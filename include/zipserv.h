@@ -476,7 +476,13 @@ int zs_decode_attention_dense_paged(void* stream, const uint16_t* q, const uint1
 /* many for V; token t of sequence b is row t % page_block_size of page     */
 /* block_table[b * table_stride + t / page_block_size], its slot that page  */
 /* times page_block_size plus the row.  Pages are a multiple of 16 tokens,  */
-/* num_blocks * page_block_size at most 2^31 - 1, head_dim 64 or 128.       */
+/* num_blocks * page_block_size at most 2^31 - 1, head_dim 64 or 128.  A    */
+/* call that takes 2^32 threads or more is refused with ZS_E_OVERFLOW       */
+/* before any launch: an append of 2^28 rows of 128 (tokens x KV heads) or  */
+/* 2^29 of 64; a selection for 2^24 (sequence, KV head) rows, 2^23 of       */
+/* tables wider than 1024 pages, 2^22 wider than 2048, or for width / 16 x  */
+/* KV heads of 2^26; attention over 2^24 splits, or 2^24 (sequence, head)   */
+/* rows of more than one.                                                   */
 /* ---------------------------------------------------------------------- */
 
 /* The tables of one step, from the lengths of its requests (device int32):

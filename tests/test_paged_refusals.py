@@ -128,3 +128,23 @@ def test_python_refuses_numbers_that_a_c_int_does_not_hold():
     for n in (2 ** 31, 2 ** 32 + 4, -2 ** 31, -2 ** 32 + 1):
         with pytest.raises(ValueError, match="2\\^31"):
             paged._whole(n, "n")
+
+
+@pytest.mark.parametrize("fn,defaults,changed", [
+    # 2^24 workgroups of 256 threads, 2^25
+    ("zs_paged_append", APPEND, dict(n=1 << 20, heads=256)),
+    ("zs_paged_append", APPEND, dict(n=1 << 30, dim=64, heads=1)),
+    # 2^26 workgroups of one wave, and 2^22 rows of 1024 threads, 2^23 of 512, 2^24 of 256
+    ("zs_select_kv_pages", SELECT, dict(width=1 << 27, stride=1 << 27, ws_bytes=1 << 50)),
+    ("zs_select_kv_pages", SELECT, dict(batch=1 << 14, heads=256, heads_k=256, width=2049, stride=2049,
+                                        ws_bytes=1 << 50)),
+    ("zs_select_kv_pages", SELECT, dict(batch=1 << 14, heads=512, heads_k=512, width=1025, stride=1025,
+                                        ws_bytes=1 << 50)),
+    ("zs_select_kv_pages", SELECT, dict(batch=1 << 14, heads=1024, heads_k=1024, width=8, ws_bytes=1 << 50)),
+    # 2^24 splits of 256 threads; 2^24 (sequence, head) rows of the merge
+    ("zs_decode_attention_sparse_paged", SPARSE, dict(top_k=1 << 27, splits=1 << 24, ws=P, ws_bytes=1 << 50)),
+    ("zs_decode_attention_sparse_paged", SPARSE, dict(batch=1 << 14, heads=1024, heads_k=1024, top_k=64, splits=2,
+                                                      ws=P, ws_bytes=1 << 50))])
+def test_grids_of_2_to_the_32_threads_are_refused(fn, defaults, changed):
+    # (a launch refuses them too, after others of the same call, and with a code of its own)
+    assert call(fn, defaults, **changed) == OVERFLOW

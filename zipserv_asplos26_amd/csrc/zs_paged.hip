@@ -955,6 +955,10 @@ int paged_checks(int num_blocks, int page, int heads_k, int head_dim) {
   return ZS_OK;
 }
 
+// Whether a launch takes this many workgroups of so many threads: fewer than 2^32
+// threads in all.
+bool grid_fits(int64_t groups, int threads) { return groups * threads <= UINT32_MAX; }
+
 }  // namespace zs
 
 using namespace zs;
@@ -1027,7 +1031,7 @@ extern "C" int zs_paged_append(void* stream, const uint16_t* k, const uint16_t* 
   p.over_heads = FastDiv::of(num_heads_k);
   const int rows = kAppendThreads * 8 / head_dim;
   const int64_t items = ((int64_t)num_tokens + rows - 1) / rows * num_heads_k;
-  if (items > INT_MAX) return ZS_E_OVERFLOW;
+  if (!grid_fits(items, kAppendThreads)) return ZS_E_OVERFLOW;
   const dim3 grid((unsigned)items);
   if (head_dim == 128)
     hipLaunchKernelGGL(append_kernel<128>, grid, dim3(kAppendThreads), 0, (hipStream_t)stream, p);
@@ -1056,12 +1060,13 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   if (top_k <= 0 || sink_pages < 0 || local_pages < 0 || (int64_t)sink_pages + local_pages > top_k) return ZS_E_INVAL;
   if (!aligned16(q) || !aligned16(page_bounds) || ((q_batch_stride | q_head_stride) & 7)) return ZS_E_INVAL;
   if (reinterpret_cast<uintptr_t>(workspace) & 7) return ZS_E_INVAL;
-  if (num_heads / num_heads_k > 16 || batch > 65535 || (int64_t)batch * num_heads_k > INT_MAX)
-    return ZS_E_UNSUPPORTED;
+  if (num_heads / num_heads_k > 16 || batch > 65535) return ZS_E_UNSUPPORTED;
   if (workspace_bytes < zs_select_kv_pages_workspace_bytes(batch, num_heads_k, max_blocks_per_seq))
     return ZS_E_INVAL;
   const int64_t score_items = ((int64_t)max_blocks_per_seq + 15) / 16 * num_heads_k;
-  if (score_items > INT_MAX / 16) return ZS_E_OVERFLOW;
+  const int64_t pick_rows = (int64_t)batch * num_heads_k;
+  const int pick_threads = max_blocks_per_seq <= 4 * 256 ? 256 : max_blocks_per_seq <= 4 * 512 ? 512 : 1024;
+  if (!grid_fits(score_items, 64) || !grid_fits(pick_rows, pick_threads)) return ZS_E_OVERFLOW;
   SelectParams p{};
   p.q = q;
   p.q_batch = q_batch_stride;
@@ -1089,15 +1094,15 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
       const dim3 grid((unsigned)score_items, batch);
       hipLaunchKernelGGL(score_kernel<D>, grid, dim3(64), 0, st, p);
     }
-    const dim3 rows(batch * num_heads_k);
+    const dim3 rows((unsigned)pick_rows);
     auto pick = [&](auto threads, auto keys) {
       constexpr int NT = decltype(threads)::value;
       hipLaunchKernelGGL((pick_kernel<D, NT, decltype(keys)::value>), rows, dim3(NT), 0, st, p);
     };
     using Four = std::integral_constant<int, 4>;
-    if (max_blocks_per_seq <= 4 * 256)
+    if (pick_threads == 256)
       pick(std::integral_constant<int, 256>{}, Four{});
-    else if (max_blocks_per_seq <= 4 * 512)
+    else if (pick_threads == 512)
       pick(std::integral_constant<int, 512>{}, Four{});
     else if (max_blocks_per_seq <= 4 * 1024)
       pick(std::integral_constant<int, 1024>{}, Four{});

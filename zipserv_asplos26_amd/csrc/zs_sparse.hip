@@ -46,6 +46,7 @@ namespace zs {
 
 int device_cu_count();                                                 // zs_gemm.hip
 int paged_checks(int num_blocks, int page, int heads_k, int head_dim);  // zs_paged.hip
+bool grid_fits(int64_t groups, int threads);                           // zs_paged.hip
 
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 typedef short v8i16 __attribute__((ext_vector_type(8)));
@@ -433,6 +434,9 @@ extern "C" int zs_decode_attention_sparse_paged(void* stream, const uint16_t* q,
   SparseParams p{};
   const SparseCut cut = sparse_cut(batch, num_heads_k, tiles, num_splits);
   p.splits = cut.splits;
+  if (!grid_fits(p.splits, cut.waves * 64) ||
+      (p.splits > 1 && !grid_fits((int64_t)batch * num_heads, kMergeWaves * 64)))
+    return ZS_E_OVERFLOW;
   if (workspace_bytes < sparse_ws_bytes(batch, num_heads, head_dim, p.splits) || (p.splits > 1 && !workspace))
     return ZS_E_INVAL;
   p.chunk = (int)((tiles + p.splits - 1) / p.splits);
