@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <cstddef>
 #include <type_traits>
 
 #include "../../include/zipserv.h"
@@ -551,8 +552,8 @@ constexpr int kPickChunk = 65536;  // pages of a bit map
 __device__ __forceinline__ float wave_max(float x) { return wave_max16(row_max16(x)); }
 
 template <int NT>
-struct PickLds {
-  union {
+struct alignas(16) PickLds {
+  union {  // (first: its digits are read and cleared 16 bytes at a time)
     int hist[kPickBins];
     uint64_t map[kPickChunk / 64];
     int list[kPickList];
@@ -683,6 +684,7 @@ template <int D, int NT, int kKeys>
 __global__ __launch_bounds__(NT) void pick_kernel(SelectParams p) {
   constexpr int kWaves = NT / 64;
   __shared__ PickLds<NT> L;
+  static_assert(alignof(PickLds<NT>) >= 16 && offsetof(PickLds<NT>, hist) % 16 == 0, "digits in pieces of 16 bytes");
   const int row = blockIdx.x, b = row / p.heads_k, h = row % p.heads_k, tid = threadIdx.x, l = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   float2* scores = p.scores + (int64_t)row * p.width;
