@@ -5,7 +5,7 @@ import random
 import pytest
 
 import paged_testutil as ref
-from zipserv_asplos26_amd import attention
+from zipserv_asplos26_amd import attention, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -340,3 +340,87 @@ def test_infinite_values_with_small_weights_show(torch_cuda, dim):
         assert (out[..., 1] == float("inf")).all() and (out[..., 5] == -float("inf")).all(), out[..., 0, :8]
         rest = [i for i in range(dim) if i not in (1, 5)]
         assert (out[..., rest] == 1).all()
+
+
+def splits_asked(batch, heads, heads_k, dim, tiles, splits=0):
+    """The splits that a call is cut into, by the workspace that it asks for."""
+    need = paged._bytes("zs_decode_attention_sparse_workspace_bytes", batch, heads, heads_k, dim, tiles, 16, splits)
+    assert need % (batch * heads * (dim + 2) * 4) == 0
+    return need // (batch * heads * (dim + 2) * 4)
+
+
+def check_some(T, seed, batch, heads, heads_k, dim, tiles, alone, splits=0):
+    """Lists of `tiles` pages of 16 for `batch` sequences.  The first `alone` have pages of their own, ragged lengths,
+    lists in any order and NaNs and infinities in all that these leave out, and are compared with attention in 64
+    bits; the others share a few pages, and the last is compared too."""
+    rng = random.Random(seed)
+    width = tiles + 3
+    q, kc, vc, table = make(T, seed, alone + 1, heads, heads_k, dim, 16, width)
+    lens = [width * 16, 16 * tiles // 2 + 5, 16 * tiles - 1, 33, 0, 1][:alone]
+    assert len(lens) == alone
+    lens.append(16 * tiles)
+    pages = some_pages(T, rng, lens, heads_k, 16, tiles, width)
+    pages[-1] = T.arange(tiles, dtype=T.int32)
+    poison(T, kc, vc, table, pages, lens)
+    more = batch - len(lens)  # copies of the last sequence, with queries of their own
+    q = T.cat([q, T.randn(more, heads, dim, generator=T.Generator().manual_seed(seed)).to(T.bfloat16)])
+    grow = lambda x: T.cat([x, x[-1:].expand(more, *x.shape[1:])])  # noqa: E731
+    got, lse = attention.flash_attn_with_kvcache_sparse(
+        q.cuda(), kc.cuda(), vc.cuda(), grow(table).cuda(), grow(pages).cuda(),
+        T.tensor(lens + more * [lens[-1]], dtype=T.int32, device="cuda"), return_softmax_lse=True, num_splits=splits)
+    some = list(range(alone)) + [batch - 1]
+    want, want_lse, tol, lse_tol = ref.attend(q[some], kc, vc, table, pages, lens)
+    o, l = got.cpu()[some].double(), lse.cpu()[some].double()
+    empty = want_lse == -float("inf")
+    assert (o[empty] == 0).all() and (l[empty] == -float("inf")).all()
+    assert ((o - want).abs() <= tol).all(), float(((o - want).abs() / tol).max())
+    assert ((l - want_lse).abs() <= lse_tol)[~empty].all()
+    assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch,heads_k,group,tiles,splits", [
+    (20, 16, 1, 25, 3), (20, 16, 2, 100, 3), (40, 8, 4, 200, 3), (16, 20, 1, 33, 3), (60, 7, 2, 61, 2),
+    (105, 10, 1, 300, 1), (75, 14, 1, 140, 1), (300, 1, 16, 300, 3)])
+def test_workgroups_of_two_waves(torch_cuda, dim, batch, heads_k, group, tiles, splits):
+    # rows that fill the last round of the CUs badly: lists over more tiles than a wave's table of places holds
+    # (128 for two waves), and splits that are merged.  (Four waves would take all of them in one split; they do
+    # not show in what is asked for where two take one as well.)
+    T = torch_cuda
+    if T.cuda.get_device_properties(0).multi_processor_count == 256:
+        assert splits_asked(batch, heads_k * group, heads_k, dim, tiles) == (splits if splits > 1 else 0)
+    check_some(T, tiles, batch, heads_k * group, heads_k, dim, tiles, 4)
+
+
+@pytest.mark.parametrize("splits,dim", [(257, 128), (300, 64), (600, 128)])
+@pytest.mark.parametrize("most_in", ["first", "last", "middle", "none"])
+def test_merge_of_hundreds_of_splits(torch_cuda, dim, most_in, splits):
+    # more splits than the merge takes at once, the largest scores in its first chunk, its last or between
+    T = torch_cuda
+    tiles = 8 * splits
+    assert splits_asked(2, 4, 2, dim, tiles, splits) == splits
+    q, kc, vc, table = make(T, splits, 2, 4, 2, dim, 16, tiles, spread=0.3)
+    lens = [16 * tiles, 16 * tiles - 16 * 8 * 20 - 3]  # (the second one's last splits are empty)
+    for b in range(2):
+        if most_in != "none":
+            at = {"first": 3, "last": tiles - 170, "middle": 8 * 250}[most_in]
+            kc[table[b, at].long(), 7] = 1.5 * q[b].view(2, 2, dim).mean(1)
+        vc[table[b, :8 * 256].long()] += 1  # what the chunks hold differs
+        vc[table[b, 8 * 256:].long()] -= 1
+    pages = T.arange(tiles, dtype=T.int32).expand(2, 2, tiles).contiguous()
+    poison(T, kc, vc, table, pages, lens)
+    want, want_lse, tol, lse_tol = ref.attend(q, kc, vc, table, pages, lens)
+    sizes = ref.attend(q, kc, vc.abs(), table, pages, lens)[0]
+    # in place of 3 T 2^-24 for the sums, what these have: 32 tokens' 96 products by 2^-23 each (192), a rescaling and
+    # an addition for each of 4 waves (8), for each of 150 splits of a merging wave and 4 of these (308), less
+    # than 2^-15; the normaliser's 8 and 2 and 4 tokens, waves and lanes, 3 chunks, 64 lanes and 4 waves by 2^-24 or
+    # two, less than 2^-18
+    many = 3 * 2.0 ** -24 * T.tensor(lens, dtype=T.float64)
+    tol = tol + sizes * (2.0 ** -15 + 2.0 ** -18 - many)[:, None, None]
+    lse_tol = lse_tol + (2.0 ** -18 - many)[:, None]
+    got, lse = attention.flash_attn_with_kvcache_sparse(
+        q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), pages.cuda(), T.tensor(lens, dtype=T.int32, device="cuda"),
+        return_softmax_lse=True, num_splits=splits)
+    off, lse_off = (got.cpu().double() - want).abs(), (lse.cpu().double() - want_lse).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+    assert (lse_off <= lse_tol).all(), float((lse_off / lse_tol).max())
