@@ -582,3 +582,26 @@ def test_numbers_past_32_bits_are_refused(torch_cuda):
                  lambda: paged.plan_paged_step(i3, i3, wide, i3, i3[2:], 16, 4)]:
         with pytest.raises(ValueError):
             call()
+
+
+# ------------------------------------------------------------------------------------------------------------
+# Heads of 64 in tables of 2049 to 4096 pages
+# ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("width,top_k", [(2049, 2048), (2500, 60), (4096, 1500)])
+def test_select_small_heads(torch_cuda, width, top_k):
+    T = torch_cuda
+    q, bounds, table = (x.cuda() for x in make_select(T, width, 1, 8, 2, 64, 16, width))
+    for length in (width * 16, width * 16 - 900, (top_k + 1) * 16):
+        if length <= top_k * 16:  # the row keeps all of its pages
+            got = paged.select_kv_pages(q, bounds, table, length, 16, top_k)
+            want = T.arange(top_k, device="cuda")
+            assert T.equal(got.long(), want.masked_fill(want >= -(-length // 16), -1).expand(1, 2, top_k))
+            continue
+        for sink, local in ((1, 1), (0, 0)):
+            check_select_many(T, q, bounds, table, length, 16, top_k, sink, local)
+
+
+@pytest.mark.parametrize("kind", ["equal", "few values", "crowd and one far", "two crowds", "one page far below",
+                                  "large", "small queries", "nearly equal", "stranger"])
+def test_select_score_distributions_of_small_heads(torch_cuda, kind):
+    test_select_score_distributions(torch_cuda, kind, 3000, 700)
