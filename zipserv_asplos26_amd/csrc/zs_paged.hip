@@ -350,8 +350,9 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendParams p) 
 // most seen, over values of all sizes, sums that cancel and powers of two).  The
 // sum of sizes is a second product, of the same operands without their signs.
 // pick_kernel finds a narrow window that holds the top_k-th largest fp32 score,
-// 2 E wider on both sides: scores above it are taken and scores below it are not,
-// whatever their errors.  What lies in it, a few pages, is scored again in 64 bits
+// 3 E wider on both sides (one for each of two scores that are compared and one for
+// the rounding of its ends, and 0.01 of a digit for the digits'): scores above it are
+// taken and scores below it are not, whatever their errors.  What lies in it, a few pages, is scored again in 64 bits
 // and ranked, ties to the lowest page; where it holds hundreds (long rows cut in
 // their middle, equal scores) the choice runs over 64-bit keys.  Rows where the
 // bound says nothing (scores or operands so large that products or sums leave
@@ -366,7 +367,7 @@ struct SelectParams {
   const int32_t* seqlens;
   int32_t* pages;           // [B][Hkv][top_k]
   float2* scores;           // [B][Hkv][width]: the fp32 score and the sum of its terms' sizes
-  int num_blocks, width, page, batch, heads_k, group, top_k, sink, local;
+  int num_blocks, width, page, heads_k, group, top_k, sink, local;
   FastDiv over_heads;
 };
 
@@ -1082,7 +1083,6 @@ extern "C" int zs_select_kv_pages(void* stream, const uint16_t* q, int64_t q_bat
   p.num_blocks = num_blocks;
   p.width = max_blocks_per_seq;
   p.page = page_block_size;
-  p.batch = batch;
   p.heads_k = num_heads_k;
   p.group = num_heads / num_heads_k;
   p.top_k = top_k;
