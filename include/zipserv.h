@@ -495,10 +495,15 @@ int zs_decode_attention_dense_paged(void* stream, const uint16_t* q, const uint1
  *   slots, sequences, positions [max_tokens]: each new token's slot (-1 where no
  *     page was left or the table's row is full), its sequence and its place in
  *     it; all -1 behind the last token;
- *   seqlens [batch]: tokens with a slot, the context's and the step's;
+ *   seqlens [batch]: the context's tokens and the step's with a slot;
  *   cu_new [batch + 1]: each sequence's first token of the step, and the end;
  *   counts [4]: tokens asked for, pages taken, pages missing, pages left (the
  *     *num_free of the next step).
+ * A context is taken to be where context_lens says, in the first ceil(len /
+ * page_block_size) entries of its row.  Where these are not all there (an entry
+ * below 0, a context of more pages than max_blocks_per_seq) that is the caller's
+ * mistake and not reported: a new token in such a page gets slot -1 and counts in
+ * seqlens, and not in counts[2].
  * batch is at most 4096.  The outputs overlap neither each other nor the inputs. */
 int zs_paged_plan(void* stream, const int32_t* context_lens, const int32_t* new_lens, int batch,
                   int32_t* block_table, int64_t table_stride, int max_blocks_per_seq,

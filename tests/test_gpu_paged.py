@@ -605,3 +605,15 @@ def test_select_small_heads(torch_cuda, width, top_k):
                                   "large", "small queries", "nearly equal", "stranger"])
 def test_select_score_distributions_of_small_heads(torch_cuda, kind):
     test_select_score_distributions(torch_cuda, kind, 3000, 700)
+
+
+def test_plan_of_a_context_that_is_not_in_the_table(torch_cuda):
+    # what the documentation says of it: slot -1, in seqlens, not among the missing pages; the other sequences' places
+    # are what they would be
+    T = torch_cuda
+    table = [[0, 0], [4, -1], [0, 0]]
+    p = paged.plan_paged_step(ints(T, [100, 20, 0]), ints(T, [5, 3, 17]), ints(T, table), ints(T, [7, 8, 9]),
+                              ints(T, [3]), 16, 30)
+    assert p.slots.tolist() == [-1] * 8 + list(range(9 * 16, 10 * 16)) + [8 * 16] + [-1] * 5
+    assert p.seqlens.tolist() == [105, 23, 17] and p.counts.tolist() == [25, 2, 0, 1]
+    assert p.positions.tolist()[:8] == [100, 101, 102, 103, 104, 20, 21, 22]

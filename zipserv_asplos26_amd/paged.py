@@ -139,7 +139,7 @@ class PagedPlan:
     slots: object       # [max_tokens] slot of each new token, -1 without one
     sequences: object   # [max_tokens] its sequence, -1 behind the last token
     positions: object   # [max_tokens] its place in the sequence, -1 behind the last
-    seqlens: object     # [batch] cached tokens after the step
+    seqlens: object     # [batch] cached tokens after the step: the context's and the new ones with a slot
     cu_new: object      # [batch + 1] each sequence's first token of the step
     counts: object      # [4] tokens asked for, pages taken, missing, left
 
@@ -160,7 +160,10 @@ def plan_paged_step(context_lens, new_lens, block_table, free_pages, num_free, p
 
     Where pages run out (or a row of the table is full) the tokens that would
     need them get slot -1, and seqlens and counts say so: counts[0] against
-    cu_new[-1] shows tokens left out, counts[2] the pages missing."""
+    cu_new[-1] shows tokens left out, counts[2] the pages missing.  The context's
+    own pages are taken to be in the table: a context that is longer than its row,
+    or a negative entry among its pages, is not reported (new tokens there get slot
+    -1 and count in seqlens all the same)."""
     torch = _torch()
     i32 = torch.int32
     _check(context_lens, "context_lens", i32, (None,))
