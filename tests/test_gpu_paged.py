@@ -617,3 +617,41 @@ def test_plan_of_a_context_that_is_not_in_the_table(torch_cuda):
     assert p.slots.tolist() == [-1] * 8 + list(range(9 * 16, 10 * 16)) + [8 * 16] + [-1] * 5
     assert p.seqlens.tolist() == [105, 23, 17] and p.counts.tolist() == [25, 2, 0, 1]
     assert p.positions.tolist()[:8] == [100, 101, 102, 103, 104, 20, 21, 22]
+
+
+def test_pages_of_finished_sequences_go_back(torch_cuda):
+    # by torch operations that do not wait; more tokens pass through the pool than it holds, and every sequence's
+    # are there when it attends
+    T = torch_cuda
+    s = Server(T, blocks=24)
+    s.free = T.cat([s.free, s.free[:1]])  # one place more, for what is not given back
+    H, Hk, D = s.shape
+    fed, rng = [[] for _ in range(4)], random.Random(1)
+    for i in range(40):
+        done = T.tensor([len(f) > rng.randint(40, 90) for f in fed])
+        for b in range(4):
+            if done[b]:
+                fed[b] = []
+        dev = done.cuda()
+        T.cuda.set_sync_debug_mode("error")
+        held = (s.lens + s.page - 1) // s.page
+        give = (dev[:, None] & (T.arange(s.table.shape[1], device="cuda") < held[:, None])).view(-1)
+        at = give.cumsum(0)
+        place = T.where(give, s.num_free + at - 1, s.free.numel() - 1)
+        s.free.scatter_(0, place, s.table.view(-1))
+        s.num_free.copy_(s.num_free + at[-1:].to(T.int32))
+        s.lens.copy_(s.lens.masked_fill(dev, 0))
+        T.cuda.set_sync_debug_mode("default")
+        s.feed([rng.randint(0, 12) for _ in range(4)], i)
+        p = s.step()[0]
+        rows, lens = s.qkv.cpu(), p.cu_new.tolist()
+        for b in range(4):
+            fed[b] += list(rows[lens[b]:lens[b + 1]])
+        assert p.counts[2] == 0 and p.seqlens.tolist() == [len(f) for f in fed]
+        table, kc = s.table.cpu(), s.k_cache.cpu()
+        used = [int(table[b, j]) for b in range(4) for j in range(-(-len(fed[b]) // 16))]
+        left = s.free[:s.num_free.item()].tolist()
+        assert sorted(used + left) == list(range(24))
+        for b, f in enumerate(fed):
+            for t, r in enumerate(f):
+                assert T.equal(kc[table[b, t // 16], t % 16].reshape(-1), r[H * D:(H + Hk) * D])
