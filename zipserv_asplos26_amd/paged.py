@@ -239,7 +239,13 @@ def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size:
     that share the KV head (in 64 bits, so the selection is the definition's;
     scores that are no number count as +inf).  The first sink_pages and the last
     local_pages of a sequence are always taken, the others by score, ties to the
-    lowest page; sequences of at most top_k pages keep them all."""
+    lowest page; sequences of at most top_k pages keep them all.
+
+    Rows that fp32 cannot settle cost 25 to 50 times as much, as one workgroup
+    scores all of their pages in 64 bits (0.25 ms for 2000 pages, 0.8 ms for 8000):
+    those with a key that is not finite or a table entry outside the pool among
+    their pages, queries with values past 2^60 or (0 aside) below 2^-126, and more than
+    4096 pages that score the same (a query or a cache of zeros)."""
     torch = _torch()
     q = _query(q)
     here = _here(q)
