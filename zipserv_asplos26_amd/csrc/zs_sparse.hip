@@ -370,7 +370,7 @@ __global__ __launch_bounds__(kMergeWaves * 64) void sparse_merge_kernel(SparsePa
 // more than it gives (8 KV heads' 256 tokens: 6.6 us whole, over 8 in two).  More
 // splits only add partial results (128 lists of 4096 tokens, head_dim 128: 53.4 us
 // in 2, 54.9 and up in 4).  Where that leaves the last round of the CUs part empty,
-// workgroups of two waves, up to 1024 of them, spread better: 320 lists of 1024,
+// workgroups of two waves, up to four a CU, spread better: 320 lists of 1024,
 // 2048, 4096 tokens 41.2 -> 39.4, 71.6 -> 68.8, 130 -> 128 us, 800 of 1024 88.8 ->
 // 86.2, but 512 of 4096 (two full rounds) 183.8 -> 190.5.
 struct SparseCut {
@@ -387,7 +387,7 @@ static SparseCut sparse_cut(int batch, int heads_k, int64_t tiles, int num_split
   const int splits = at_most(cus / units, 4);
   const int64_t items = units * splits, rounds = (items + cus - 1) / cus;
   if (100 * items >= 85 * rounds * cus || splits < cus / units) return {4, splits};
-  return {2, at_most(1024 / units, 2)};
+  return {2, at_most(4 * cus / units, 2)};
 }
 
 static size_t sparse_ws_bytes(int batch, int heads, int head_dim, int splits) {
