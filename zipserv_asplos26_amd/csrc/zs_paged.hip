@@ -31,7 +31,7 @@ namespace zs {
 // from L2) and then places its 512 tokens by a search over the first sum.  A
 // table entry is written by the token that opens its page and read only for
 // pages that the sequence had before, so no workgroup waits for another.  What it
-// takes is latency: loads, two barriers a chunk of sequences, a search in LDS; 3.6 us
+// takes is latency: loads, two barriers a chunk of sequences, a search in LDS; 3.5 us
 // for one sequence, 4.7 for 300 with 24400 places (6.3 with a scan for each of the
 // four counts and 256 sequences a chunk).
 constexpr int kPlanThreads = 512;
@@ -198,8 +198,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanParams p) {
 // the keys through LDS: the threads of a run's first token go through the run's
 // other rows there.  Where the last run goes on behind the workgroup's tokens, all
 // its threads read the rest of it (from L2, as another workgroup copies it) and
-// meet in LDS.  8000 tokens of 8 heads of 128 in pages of 16: 16.8 us, 80% of the
-// rate of a copy; 3001 of 16 heads of 64 in pages of 128: 11.8 us, 6.2 without
+// meet in LDS.  8000 tokens of 8 heads of 128 in pages of 16: 16.9 us, 78% of the
+// rate of a copy; 3001 of 16 heads of 64 in pages of 128: 11.9 us, 6.2 without
 // bounds, the rest being the chain of a run's rows.  (One thread group reading a
 // whole run, row after row: 30 and 102 us.)
 constexpr int kAppendThreads = 256;
@@ -415,9 +415,10 @@ __device__ __forceinline__ float row_max16x4(f32x4 v, int l) {
 // A workgroup of one wave scores 16 pages for one KV head.  The heads of the same
 // pages run next to one another, so a page's bounds are read from memory as one
 // piece (32 sequences to 64000 tokens, 64 / 8 heads, 271 MB: selection 81.5 -> 71.3
-// us; with 16 pages a wave in place of 64 69.5).  Workgroups of four waves take 11.1
-// and 64.8 us where these take 10.4 and 65.4 (one sequence of 32000 tokens, the 32 to
-// 64000), 69.5 and 68.3 us with the attention of 16 to 40000.
+// us; with 16 pages a wave in place of 64 69.5).  Workgroups of four waves took 11.1
+// and 64.8 us where these took 10.4 and 65.4 (one sequence of 32000 tokens, the 32 to
+// 64000; 9.3 and 64.5 since the choice's last change), 69.5 and 68.3 us with the
+// attention of 16 to 40000.
 template <int D>
 __global__ __launch_bounds__(64) void score_kernel(SelectParams p) {
   constexpr int kC = D / 32;
@@ -542,7 +543,7 @@ __device__ __forceinline__ uint64_t exact_key(const SelectParams& p, const PageB
 // ended by a barrier: so scores are loaded before the row's length is known and stay
 // in registers (kKeys a thread; the rest of longer rows is read again), sums
 // and maxima run over DPP and ballots, and one pass does all that goes by the window.
-// 8 rows of 2000 pages 7 us, of 8188 10 us, 256 rows of 125..4000 11.5 us.  For the
+// 8 rows of 2000 pages 7 us, of 8188 11 us, 256 rows of 125..4000 11 us.  For the
 // first, eight scores a thread took 8 us and sixteen 9.7, the same steps in rolled
 // loops over scores in LDS 9.6.
 constexpr int kPickBins = 2048;

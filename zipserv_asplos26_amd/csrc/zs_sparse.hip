@@ -23,11 +23,11 @@
 // stands above one step less than the number, which leaves a rest, and 2^-133 (the
 // smallest bf16, of a weight of 2^-126 or more) where that is less.
 //
-// HBM bounds it where there is enough to read: 64 sequences' 4096 tokens at 5.8 TB/s,
-// and a plain reader of random pages gets 5.65.  One pair of tiles in flight a wave
-// is enough for that; loading the next pair ahead, more waves a workgroup and more
-// splits were slower.  One sequence's 2048 tokens of 8 heads take 6 us and 2.5 for
-// the merge.
+// HBM bounds it where there is enough to read: 64 sequences' 4096 tokens at 5.75
+// to 6.0 TB/s, and a plain reader of as many random pages gets 6.0.  One pair of tiles
+// in flight a wave is enough for that; loading the next pair ahead, more waves a
+// workgroup and more splits were slower.  One sequence's 2048 tokens of 8 heads take 6
+// us and 2.6 for the merge.
 //
 // Tokens at or past the sequence's length, pages that are not in the sequence
 // and table entries outside the pool count for nothing: their scores are masked
