@@ -564,6 +564,84 @@ int zs_decode_attention_sparse_paged(void* stream, const uint16_t* q, int64_t q_
                                      uint16_t* out, float* softmax_lse, void* workspace,
                                      size_t workspace_bytes, int num_splits);
 
+/* ---------------------------------------------------------------------- */
+/* Rotary positions and a paged cache held in 4 or 8 bits (no counterpart in */
+/* the reference).  Calls of 2^32 threads and more are refused with          */
+/* ZS_E_OVERFLOW before any launch.                                          */
+/* ---------------------------------------------------------------------- */
+#define ZS_TYPE_BF16 0
+#define ZS_TYPE_FP16 1
+#define ZS_TYPE_FP32 2
+
+/* Rotary positions: pair i < num_pairs of every head of q and k turns by
+ * positions[token] * frequencies[i] (device, 64 bits; radians a position), with
+ *   y_a = factor (x_a cos - x_b sin),  y_b = factor (x_b cos + x_a sin);
+ * (a, b) = (i, i + num_pairs), or (2i, 2i + 1) where interleaved is not 0.  The
+ * other channels, and tokens whose position is negative, are copied.  q and k:
+ * [num_tokens][num_heads or num_heads_k][head_dim] of `type`, strides in elements;
+ * either may be absent (0 heads).  An output is its input (same pointer and
+ * strides: turned in place) or apart from all inputs.  num_pairs is at most 512. */
+int zs_rotary(void* stream, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+              int64_t q_out_token_stride, int64_t q_out_head_stride, int num_heads, const void* k,
+              int64_t k_token_stride, int64_t k_head_stride, void* k_out,
+              int64_t k_out_token_stride, int64_t k_out_head_stride, int num_heads_k, int type,
+              const int32_t* positions, int num_tokens, int head_dim, const double* frequencies,
+              int num_pairs, double factor, int interleaved);
+
+/* A quantised pool is bytes [num_blocks][num_heads_k][record], 16-byte aligned,
+ * with the slots and block tables of a bf16 pool.  A record holds a page of one
+ * KV head: page_block_size times 8 bytes, a token's (scale, low) of the key and
+ * (scale, low) of the value in bf16; then the tokens' rows of key codes; then
+ * those of value codes, head_dim * bits / 8 bytes each.  bits is 4 or 8.  In 4
+ * bits dword j of a row holds channel 8j + 2i in bits 4i and up and channel 8j +
+ * 2i + 1 in bits 16 + 4i and up, i < 4; in 8 bits channel d is byte d.  A value
+ * is low + code * scale.
+ * zs_quant_record_bytes: page_block_size * (8 + head_dim * bits / 4), -1 for
+ * numbers that no pool has. */
+int64_t zs_quant_record_bytes(int page_block_size, int head_dim, int bits);
+
+/* zs_paged_append into a quantised pool.  Of a row x of head_dim bf16: low = min x,
+ * scale = the least bf16 with (2^bits - 1) scale >= max x - low, code = (x - low)
+ * / scale to the nearest, the even one of two (0 where scale is 0); both
+ * differences rounded to fp32.  A row with a value that is not finite, or whose max
+ * x - low is not, gets NaN for low and scale and codes 0.  No slot may occur
+ * twice; tokens may come in any order. */
+int zs_paged_append_quant(void* stream, const uint16_t* k, const uint16_t* v, int64_t k_token_stride,
+                          int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                          const int32_t* slots, int num_tokens, uint8_t* cache, int num_blocks,
+                          int page_block_size, int num_heads_k, int head_dim, int bits);
+
+/* The values of slots: k_out and v_out [num_tokens][num_heads_k][head_dim] bf16
+ * (16-byte aligned), low + code * scale in fp32, rounded to bf16; zeros for a slot
+ * outside the pool.  A slot may occur any number of times. */
+int zs_paged_read_quant(void* stream, const uint8_t* cache, int num_blocks, int page_block_size,
+                        int num_heads_k, int head_dim, int bits, const int32_t* slots,
+                        int num_tokens, uint16_t* k_out, uint16_t* v_out);
+
+/* Attention of each sequence's last new_tokens tokens over a quantised pool: new
+ * token i of sequence b attends to the tokens below cache_seqlens[b] - new_tokens
+ * + 1 + i (its own the last of them).  q: [batch][new_tokens][num_heads]
+ * [head_dim] bf16, strides in elements, multiples of 8; out: the same shape,
+ * contiguous; softmax_lse (optional): [batch][num_heads][new_tokens].  q and out
+ * are 16-byte aligned.  A row that sees no token gives zeros and softmax_lse -inf.
+ * Tokens past the table's width and in pages outside the pool count for nothing.  num_splits = 0 picks
+ * the splits of long sequences; the workspace (16-byte aligned) is what the query
+ * says for the same arguments.  batch, and num_heads_k times the 16-column pieces
+ * of num_heads / num_heads_k * new_tokens, are at most 65535. */
+size_t zs_decode_attention_quant_workspace_bytes(int batch, int new_tokens, int num_heads,
+                                                 int num_heads_k, int head_dim,
+                                                 int max_blocks_per_seq, int page_block_size,
+                                                 int num_splits);
+int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, int64_t q_batch_stride,
+                                    int64_t q_token_stride, int64_t q_head_stride,
+                                    const uint8_t* cache, int num_blocks, int page_block_size,
+                                    int bits, const int32_t* block_table, int64_t table_stride,
+                                    int max_blocks_per_seq, const int32_t* cache_seqlens,
+                                    int batch, int new_tokens, int num_heads, int num_heads_k,
+                                    int head_dim, float softmax_scale, uint16_t* out,
+                                    float* softmax_lse, void* workspace, size_t workspace_bytes,
+                                    int num_splits);
+
 /* Stage profiler of the re-tiled record pipeline
  * (kernel_benchmark/zipserv_tile_stage_bench_ext.cu measure_zipserv_tile_stages):
  * one wave consumes records record0 + i*stride (mod num_records), waiting

@@ -26,6 +26,9 @@ ZS_WINDOW_WEIGHTS = 1
 ZS_RETILED_AUTO_WORK_BYTES = 65600
 ZS_LAYOUT_HEAD_MAJOR = 0
 ZS_LAYOUT_TOKEN_MAJOR = 1
+ZS_TYPE_BF16 = 0
+ZS_TYPE_FP16 = 1
+ZS_TYPE_FP32 = 2
 
 _lib = None
 
@@ -119,6 +122,18 @@ SIGNATURES = {
     "zs_decode_attention_sparse_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
     "zs_decode_attention_sparse_paged": (
         C.c_int, [_p, _p, _i64, _i64, _p, _p, C.c_int, C.c_int, _p, _i64, C.c_int, _p, C.c_int, _p, C.c_int,
+                  C.c_int, C.c_int, C.c_int, C.c_float, _p, _p, _p, C.c_size_t, C.c_int]),
+    "zs_rotary": (
+        C.c_int, [_p] + [_p, _i64, _i64, _p, _i64, _i64, C.c_int] * 2 + [C.c_int, _p, C.c_int, C.c_int, _p, C.c_int,
+                                                                        C.c_double, C.c_int]),
+    "zs_quant_record_bytes": (_i64, [C.c_int, C.c_int, C.c_int]),
+    "zs_paged_append_quant": (
+        C.c_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, C.c_int, _p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "zs_paged_read_quant": (
+        C.c_int, [_p, _p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _p, C.c_int, _p, _p]),
+    "zs_decode_attention_quant_workspace_bytes": (C.c_size_t, [C.c_int] * 8),
+    "zs_decode_attention_quant_paged": (
+        C.c_int, [_p, _p, _i64, _i64, _i64, _p, C.c_int, C.c_int, C.c_int, _p, _i64, C.c_int, _p, C.c_int, C.c_int,
                   C.c_int, C.c_int, C.c_int, C.c_float, _p, _p, _p, C.c_size_t, C.c_int]),
     "zs_measure_record_stages": (
         C.c_int, [_p, _p, _p, _p, C.c_uint8, C.c_int, C.c_int, _i64, _i64, C.c_int, C.c_int,

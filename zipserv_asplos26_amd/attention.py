@@ -401,6 +401,55 @@ def flash_attn_with_kvcache_sparse(q, k_cache, v_cache, block_table, pages, cach
     return (out, lse) if return_softmax_lse else out
 
 
+def flash_attn_with_kvcache_quantized(q, cache, block_table, cache_seqlens, softmax_scale: Optional[float] = None,
+                                      num_splits: int = 0, return_softmax_lse: bool = False):
+    """Attention over a paged cache held in 4 or 8 bits (`paged.QuantizedKVCache`).
+    q: (B, H, D) or (B, new, H, D) bf16, each sequence's last `new` tokens, possibly a slice
+    of a fused projection's output; new token i attends to the tokens below
+    cache_seqlens - new + 1 + i, its own the last of them (cache_seqlens: int32 [B]
+    or an int, the new tokens counted).  block_table: (B, max_blocks) int32.
+    Scores, softmax and sums are fp32 over the cache's values low + code * scale,
+    which are not rounded first.  Returns out shaped like q (and softmax_lse [B,
+    H], or [B, H, new] for a q of four dimensions, when asked); a row that sees no
+    token gives zeros and lse -inf.  num_splits cuts each sequence's tokens alike, 0 by
+    the size of the call."""
+    torch = _torch()
+    shape = q.shape if isinstance(q, torch.Tensor) else ()
+    paged._check(q, "q", torch.bfloat16, (None,) * (4 if len(shape) == 4 else 3), contiguous=False)
+    here = paged._here(q)
+    if here is None:
+        with torch.cuda.device(q.device):
+            return flash_attn_with_kvcache_quantized(q, cache, block_table, cache_seqlens, softmax_scale, num_splits,
+                                                     return_softmax_lse)
+    device, stream = here
+    data, nblocks, page, Hkv, D, bits = paged._quantized(cache)
+    if cache.data.get_device() != device:
+        raise ValueError(f"cache must be on cuda:{device}")
+    q4 = q if len(shape) == 4 else q[:, None]
+    B, new, H, dim = q4.shape
+    if dim != D:
+        raise ValueError(f"q has heads of {dim}, the cache of {D}")
+    table, row, width = paged._table(block_table, B, device)
+    lens = paged._lengths(cache_seqlens, B, device)
+    if Hkv == 0 or H % Hkv:
+        raise ValueError(f"{H} query heads do not share {Hkv} KV heads evenly")
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    splits = paged._whole(num_splits, "num_splits")
+    q0, q1, q2, q3 = q4.stride()
+    if q3 != 1 or (q0 | q1 | q2) % 8 or q4.data_ptr() % 16:
+        q4 = q4.clone(memory_format=torch.contiguous_format)
+        q0, q1, q2, _ = q4.stride()
+    out = paged._new_like(q, shape)
+    lse = torch.empty((B, H, new) if len(shape) == 4 else (B, H), dtype=torch.float32, device=q.device) \
+        if return_softmax_lse else None
+    wsb = paged._bytes("zs_decode_attention_quant_workspace_bytes", B, new, H, Hkv, D, width, page, splits)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
+    check("zs_decode_attention_quant_paged", lib().zs_decode_attention_quant_paged(
+        stream, q4.data_ptr(), q0, q1, q2, data, nblocks, page, bits, table.data_ptr(), row, width, lens.data_ptr(),
+        B, new, H, Hkv, D, scale, out.data_ptr(), _dptr(lse), _dptr(ws), wsb, splits))
+    return (out, lse) if return_softmax_lse else out
+
+
 def fwd_kvcache_zipserv(q, k_sign_mantissa, k_compressed_full, k_bitmap1, k_bitmap2, k_bitmap3,
                         k_tile_offsets_median, k_tile_offsets_global, k_rows: int, k_cols: int,
                         k_max_high_freq_count: int, k_max_full_count: int, k_start_exp: int,

@@ -41,6 +41,7 @@
 
 #include "../../include/zipserv.h"
 #include "zs_device.hpp"
+#include "zs_splits.hpp"
 
 namespace zs {
 
@@ -288,83 +289,6 @@ __global__ __launch_bounds__(W * 64) void sparse_attn_kernel(SparseParams p) {
   }
 }
 
-// The splits of one (sequence, head) merged by four waves: their weights by a
-// lane each, then a wave takes every fourth split, eight loads in flight.
-constexpr int kMergeWaves = 4, kMergeChunk = 256;
-
-template <int D>
-__global__ __launch_bounds__(kMergeWaves * 64) void sparse_merge_kernel(SparseParams p) {
-  constexpr int kV = D / 64;  // values a lane
-  __shared__ float weight[kMergeChunk];
-  __shared__ float red[kMergeWaves];
-  __shared__ float part[kMergeWaves][D];
-  const int64_t head = blockIdx.x;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id();
-  const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + head * p.splits;
-  const float* o = p.ws_o + head * p.splits * D + kV * l;
-  float m_run = -INFINITY, sum = 0.f, acc[kV] = {};
-  for (int c0 = 0; c0 < p.splits; c0 += kMergeChunk) {
-    const int n = min(p.splits - c0, kMergeChunk);
-    const float2 own = tid < n ? ml[c0 + tid] : float2{-INFINITY, 0.f};
-    float x[8][kV];
-    auto load = [&](int s0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int s = s0 + kMergeWaves * j;
-#pragma unroll
-        for (int i = 0; i < kV; ++i) x[j][i] = s < n ? o[(int64_t)(c0 + s) * D + i] : 0.f;
-      }
-    };
-    load(w);
-    float m = own.x;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-    __syncthreads();  // the last chunk's weights are read
-    if (l == 0) red[w] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kMergeWaves; ++i) m = fmaxf(m, red[i]);
-    m = fmaxf(m, m_run);
-    const float m_use = m == -INFINITY ? 0.f : m;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-    const float f = __builtin_amdgcn_exp2f(own.x - m_use);
-    weight[tid] = f;
-    sum = sum * alpha + own.y * f;  // this thread's splits
-#pragma unroll
-    for (int i = 0; i < kV; ++i) acc[i] *= alpha;
-    m_run = m;
-    __syncthreads();
-    for (int s0 = w; s0 < n; s0 += 8 * kMergeWaves) {
-      if (s0 > w) load(s0);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float g = s0 + kMergeWaves * j < n ? weight[s0 + kMergeWaves * j] : 0.f;
-#pragma unroll
-        for (int i = 0; i < kV; ++i) acc[i] += x[j][i] * g;
-      }
-    }
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-  __syncthreads();
-  if (l == 0) red[w] = sum;
-#pragma unroll
-  for (int i = 0; i < kV; ++i) part[w][kV * l + i] = acc[i];
-  __syncthreads();
-  if (tid >= D / 2) return;
-  sum = 0.f;
-  float2 x = {0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < kMergeWaves; ++i) {
-    sum += red[i];
-    x.x += part[i][2 * tid];
-    x.y += part[i][2 * tid + 1];
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint32_t*>(p.out + head * D + 2 * tid) = pack_bf16x2(x.x * inv, x.y * inv);
-  if (p.lse && tid == 0) p.lse[head] = sum == 0.f ? -INFINITY : (m_run + __log2f(sum)) * 0.6931471805599453f;
-}
-
 // How a call is cut: workgroups of four waves, one a CU (256), each list in as
 // many splits as that takes; lists of up to 384 tokens whole, whose merge costs
 // more than it gives (8 KV heads' 256 tokens: 6.6 us whole, over 8 in two).  More
@@ -473,9 +397,7 @@ extern "C" int zs_decode_attention_sparse_paged(void* stream, const uint16_t* q,
       hipLaunchKernelGGL((sparse_attn_kernel<D, 2>), grid, dim3(2 * 64), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    const dim3 rows((unsigned)((int64_t)batch * num_heads));
-    hipLaunchKernelGGL(sparse_merge_kernel<D>, rows, dim3(kMergeWaves * 64), 0, st, p);
-    return hipGetLastError();
+    return merge_splits(st, SplitMerge::of(p.ws_o, p.ws_ml, p.out, p.lse, p.splits, batch * num_heads, num_heads, 1), D);
   };
   const hipError_t e = head_dim == 128 ? launch(std::integral_constant<int, 128>{})
                                        : launch(std::integral_constant<int, 64>{});

@@ -133,6 +133,19 @@ def _bytes(query, *sizes):
     return int(getattr(lib(), query)(*sizes))
 
 
+@dataclass(frozen=True)
+class QuantizedKVCache:
+    """A pool of pages held in 4 or 8 bits, as `quantized_kv_cache` makes it: for
+    every (page, KV head) page_block_size times 8 bytes with a token's (scale,
+    low) of the key and of the value in bf16, then the tokens' rows of key codes,
+    then those of value codes; a value is low + code * scale.  (include/zipserv.h
+    has the order of the codes.)"""
+    data: object         # uint8 (num_blocks, Hkv, page_block_size * (8 + head_dim * bits / 4))
+    page_block_size: int
+    head_dim: int
+    bits: int
+
+
 @dataclass
 class PagedPlan:
     """One step's tables (all int32 on the GPU)."""
@@ -275,3 +288,80 @@ def select_kv_pages(q, page_bounds, block_table, cache_seqlens, page_block_size:
         row, width, lens.data_ptr(), batch, heads, heads_k, dim, top_k, sink, local, pages.data_ptr(),
         ws.data_ptr(), need))
     return pages
+
+
+def quantized_kv_cache(num_blocks: int, page_block_size: int, num_heads_k: int, head_dim: int, bits: int = 4,
+                       device="cuda") -> QuantizedKVCache:
+    """An empty pool of num_blocks pages held in `bits` (4 or 8) bits; head_dim 64
+    or 128, pages a multiple of 16 tokens.  With head_dim 128 a token's key and
+    value of one KV head take 136 (264) bytes where bf16 takes 512."""
+    torch = _torch()
+    if bits not in (4, 8) or head_dim not in (64, 128):
+        raise ValueError(f"a cache of {bits} bits and head_dim {head_dim}: bits must be 4 or 8, head_dim 64 or 128")
+    if page_block_size <= 0 or page_block_size % 16:
+        raise ValueError(f"page_block_size must be a positive multiple of 16, got {page_block_size}")
+    record = page_block_size * (8 + head_dim * bits // 4)
+    data = torch.empty(num_blocks, num_heads_k, record, dtype=torch.uint8, device=device)
+    return QuantizedKVCache(data, page_block_size, head_dim, bits)
+
+
+def _quantized(cache, name="cache"):
+    """A QuantizedKVCache's numbers as the library takes them: address, num_blocks,
+    page, Hkv, head_dim, bits."""
+    if not isinstance(cache, QuantizedKVCache):
+        raise ValueError(f"{name} must be a QuantizedKVCache")
+    page, dim, bits = cache.page_block_size, cache.head_dim, cache.bits
+    if not (isinstance(page, int) and 0 < page <= _MOST and isinstance(dim, int) and 0 < dim <= _MOST
+            and bits in (4, 8)):
+        raise ValueError(f"{name}: page_block_size, head_dim or bits is wrong")
+    _check(cache.data, f"{name}.data", _torch().uint8, (None, None, page * (8 + dim * bits // 4)))
+    blocks, heads_k, _ = cache.data.shape
+    return cache.data.data_ptr(), blocks, page, heads_k, dim, bits
+
+
+def append_paged_kv_quantized(k, v, cache: QuantizedKVCache, slots) -> None:
+    """New keys and values (tokens, Hkv, D) bf16 quantised into their slots of a
+    cache held in 4 or 8 bits (slots: int32 [tokens], `PagedPlan.slots`; those
+    outside the pool are skipped, none occurs twice).  k and v may be slices of a
+    fused projection's output.
+
+    Of a token's row x of one KV head: low = min x, scale = the least bf16 with (2^bits
+    - 1) scale >= max x - low, code = (x - low) / scale to the nearest, the even
+    one of two; both differences rounded to fp32.  So a value comes back half a
+    scale off at most.  A row with a value that is not finite is stored as NaNs."""
+    torch = _torch()
+    data, blocks, page, heads_k, dim, bits = _quantized(cache)
+    here = _here(cache.data)
+    if here is None:
+        with torch.cuda.device(cache.data.device):
+            return append_paged_kv_quantized(k, v, cache, slots)
+    device, stream = here
+    _check(slots, "slots", torch.int32, (None,), device)
+    n = slots.shape[0]
+    _check(k, "k", torch.bfloat16, (n, heads_k, dim), device, contiguous=False)
+    _check(v, "v", torch.bfloat16, (n, heads_k, dim), device, contiguous=False)
+    k, k0, k1 = _rows(k)
+    v, v0, v1 = _rows(v)
+    check("zs_paged_append_quant", lib().zs_paged_append_quant(
+        stream, k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, data, blocks, page, heads_k, dim,
+        bits))
+
+
+def read_paged_kv_quantized(cache: QuantizedKVCache, slots):
+    """The keys and values in slots (int32 [tokens], in any order, any number of
+    times) of a cache held in 4 or 8 bits: (k, v), (tokens, Hkv, D) bf16 each,
+    low + code * scale in fp32, rounded to bf16; zeros for slots outside the pool
+    (-1)."""
+    torch = _torch()
+    data, blocks, page, heads_k, dim, bits = _quantized(cache)
+    here = _here(cache.data)
+    if here is None:
+        with torch.cuda.device(cache.data.device):
+            return read_paged_kv_quantized(cache, slots)
+    device, stream = here
+    _check(slots, "slots", torch.int32, (None,), device)
+    n = slots.shape[0]
+    k, v = torch.empty((2, n, heads_k, dim), dtype=torch.bfloat16, device=slots.device).unbind(0)
+    check("zs_paged_read_quant", lib().zs_paged_read_quant(
+        stream, data, blocks, page, heads_k, dim, bits, slots.data_ptr(), n, k.data_ptr(), v.data_ptr()))
+    return k, v

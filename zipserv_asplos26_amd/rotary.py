@@ -1,0 +1,150 @@
+"""Rotary positions: what turns the queries and keys of a step before they are
+appended and attended to.
+
+    frequencies, factor = rotary_frequencies(head_dim, base=500000.0, scaling="bands", stretch=8.0, trained=8192)
+    q, k = apply_rotary(q, k, plan.positions, frequencies, factor=factor)
+
+Pair i of a head's rotated channels turns by position * frequencies[i]; the
+angles are made in 64 bits, so positions of millions lose nothing and no table of
+positions is kept.
+"""
+from __future__ import annotations
+
+import math
+
+from ._lib import ZS_TYPE_BF16, ZS_TYPE_FP16, ZS_TYPE_FP32, check, lib
+from .codec import _torch
+from .paged import _check, _here, _MOST
+
+
+def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: str = "none", stretch: float = 1.0,
+                       trained: int = 0, low_turns: float = 1.0, high_turns: float = 0.0, device="cuda"):
+    """(frequencies, factor) of `apply_rotary` for the first `rotated` channels of a
+    head (even): radians a position, float64 [rotated / 2], and what cosines and
+    sines are multiplied by.
+
+    w_i = base^(-2 i / rotated), and for contexts `stretch` times the `trained` positions, by
+    `scaling`,
+      "linear": all w_i / stretch (positions interpolated);
+      "base":   base * stretch^(rotated / (rotated - 2)) for base, which divides the
+                slowest pair by stretch and leaves the fastest;
+      "bands":  a pair that turns high_turns times or more over the trained positions
+                keeps w_i, one that turns low_turns times or less gets w_i / stretch,
+                between them a share of each, linear in the turns (high_turns 0: 4);
+      "ramp":   the same with a share linear in the pair's number, from the pair that
+                turns high_turns times (0: 32), rounded down, to the one that turns
+                low_turns times, rounded up, and the factor 0.1 ln(stretch) + 1."""
+    torch = _torch()
+    if rotated <= 0 or rotated % 2:
+        raise ValueError(f"rotated must be a positive even number, got {rotated}")
+    if not (base > 0 and stretch > 0):
+        raise ValueError("base and stretch must be positive")
+    if scaling not in ("none", "linear", "base", "bands", "ramp"):
+        raise ValueError(f"scaling {scaling!r} is none of none, linear, base, bands, ramp")
+    factor, pair = 1.0, torch.arange(rotated // 2, dtype=torch.float64)
+    if scaling == "base":
+        if rotated == 2:
+            raise ValueError("a single pair has no base to scale")
+        base = base * stretch ** (rotated / (rotated - 2))
+    w = base ** (-2 * pair / rotated)
+    if scaling == "linear":
+        w = w / stretch
+    elif scaling in ("bands", "ramp"):
+        high = high_turns or (4.0 if scaling == "bands" else 32.0)
+        if trained <= 0 or not 0 < low_turns < high:
+            raise ValueError("trained must be positive and low_turns below high_turns")
+        if scaling == "bands":
+            keep = ((trained * w / (2 * math.pi) - low_turns) / (high - low_turns)).clamp(0, 1)
+        else:
+            if base == 1:
+                raise ValueError("base must not be 1")
+
+            def number(turns):  # of the pair that turns so often over the trained positions
+                return rotated * math.log(trained / (2 * math.pi * turns)) / (2 * math.log(base))
+
+            first = max(math.floor(number(high)), 0)
+            last = min(math.ceil(number(low_turns)), rotated - 1)
+            keep = 1 - ((pair - first) / max(last - first, 1e-3)).clamp(0, 1)
+            factor = 0.1 * math.log(stretch) + 1.0 if stretch > 1 else 1.0
+        w = w * keep + w / stretch * (1 - keep)
+    return w.to(device), factor
+
+
+def _strides(t):
+    """Token and head stride of (tokens, heads, dim) in elements, None where a head's
+    channels do not stand next to one another."""
+    s0, s1, s2 = t.stride()
+    return (s0, s1) if s2 == 1 or t.shape[2] == 1 else None
+
+
+def _apart(t):
+    """Whether no two entries of (tokens, heads, dim) share a place."""
+    reach = 0
+    for step, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if step <= reach:
+            return False
+        reach += step * (size - 1)
+    return True
+
+
+def apply_rotary(q, k, positions, frequencies, factor: float = 1.0, interleaved: bool = False,
+                 inplace: bool = False):
+    """q and k with their heads' first 2 * len(frequencies) channels turned by their
+    tokens' positions: (q, k).  q: (tokens, H, D) or (B, new, H, D), k the same with its own
+    heads, or None; bf16, fp16 or fp32, possibly slices of a fused projection's
+    output.  positions: int32, one a token (`PagedPlan.positions`); a token with a
+    negative one is copied as it is.  frequencies: float64 [pairs] on the GPU, radians
+    a position; cosines and sines are multiplied by factor.
+
+    Pair i is channels (i, i + pairs), with `interleaved` (2i, 2i + 1).  With `inplace` q
+    and k are turned where they are (and returned), else into new contiguous
+    tensors.  frequencies negated turn back what factor 1 has turned."""
+    torch = _torch()
+    types = {torch.bfloat16: ZS_TYPE_BF16, torch.float16: ZS_TYPE_FP16, torch.float32: ZS_TYPE_FP32}
+    if not (isinstance(q, torch.Tensor) and q.dtype in types):
+        raise ValueError("q must be a bfloat16, float16 or float32 CUDA tensor")
+    form = (None,) * (4 if q.dim() == 4 else 3)
+    _check(q, "q", q.dtype, form, contiguous=False)
+    here = _here(q)
+    if here is None:
+        with torch.cuda.device(q.device):
+            return apply_rotary(q, k, positions, frequencies, factor, interleaved, inplace)
+    device, stream = here
+    dim, lead = q.shape[-1], q.shape[:-2]
+    if k is not None:
+        _check(k, "k", q.dtype, (*lead, None, dim), device, contiguous=False)
+    _check(positions, "positions", torch.int32, (*lead,), device)
+    _check(frequencies, "frequencies", torch.float64, (None,), device)
+    pairs = frequencies.shape[0]
+    if pairs == 0 or 2 * pairs > dim:
+        raise ValueError(f"{pairs} frequencies do not fit heads of {dim} channels")
+    tokens = positions.numel()
+    if tokens > _MOST:
+        raise ValueError("there must be less than 2^31 tokens")
+
+    sides, out = [], []
+    for name, x in (("q", q), ("k", k)):
+        if x is None:
+            sides += [0, 0, 0, 0, 0, 0, 0]
+            out.append(None)
+            continue
+        if inplace:
+            try:
+                x3 = x.view(tokens, x.shape[-2], dim)
+            except RuntimeError:
+                x3 = None
+            if x3 is None or _strides(x3) is None or not _apart(x3):
+                raise ValueError(f"{name} is turned in place: its tokens must follow one stride, its heads be contiguous "
+                                 "and apart")
+            y, y3 = x, x3
+        else:
+            x3 = x.reshape(tokens, x.shape[-2], dim)
+            if _strides(x3) is None:
+                x3 = x3.contiguous()
+            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            y3 = y.view(x3.shape)
+        sides += [x3.data_ptr(), *_strides(x3), y3.data_ptr(), *_strides(y3), x3.shape[1]]
+        out.append((y, x3))  # (x3 is held until the launch is queued)
+    check("zs_rotary", lib().zs_rotary(stream, *sides, types[q.dtype], positions.data_ptr(), tokens, dim,
+                                       frequencies.data_ptr(), pairs, float(factor), int(bool(interleaved))))
+    return tuple(None if o is None else o[0] for o in out)
