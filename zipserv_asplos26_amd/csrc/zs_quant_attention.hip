@@ -5,25 +5,38 @@
 // 0..15 or 0..255,
 //   q.k       = s_k (q.c) + low_k sum(q),
 //   sum p v   = sum (p s_v) c + sum p low_v,
-// so the codes themselves are the matrix operands, exact in bf16, and a token costs two
+// so the codes themselves are the matrix operands, exactly, and a token costs two
 // products more a row, not a value each channel.
 //
 // A column is a (new token, query head) of one KV head's group; a workgroup of
-// kWaves waves takes 16 columns of a sequence and a split of its tokens, a wave 32
-// tokens (two tiles of 16) at a time, all in registers:
-//   S^T = C_k q^T with v_mfma_f32_16x16x32_bf16: lane l holds D / 4 codes of token
+// kQaWaves waves takes up to 16 columns and a part of the tokens, a wave 32 tokens (two
+// tiles of 16) at a time, all in registers, with the next pair's loads on the way:
+//   S^T = C_k q^T with v_mfma_f32_16x16x32_f16: lane l holds D / 4 codes of token
 //   l%16 (channels D/4 * (l/16) and up, one piece of its row), 8 of them the A operand of a
-//   step; q^T (lane l: column l%16, the same channels) is the B operand.
+//   step; q^T (lane l: column l%16, the same channels) is the B operand.  A code's bits
+//   are an fp16 subnormal, code 2^-24, which costs an "and" for two codes and a shift for four.
 //   Online softmax in the log2 domain, fp32.
-//   O^T += C_v^T W^T over K = 32 tokens: S^T leaves lane l the weights of column l%16
-//   for tokens 4*(l/16)..+3 of both tiles, the B operand if k index 8*(l/16) + j
-//   stands for token 4*(l/16) + j%4 of tile j/4; lane l reads the l%16-th part of those
-//   eight rows, D / 16 channels of 8 tokens, which are D / 16 A operands.
-// In 4 bits a shift and a mask put two codes into the mantissas of two bf16 of
-// exponent 4, that is 16 + c: the 16s are taken off through the sums of q and of the weights.
+//   O^T += C_v^T W^T over K = 32 tokens with v_mfma_f32_16x16x32_bf16: S^T leaves lane l
+//   the weights of column l%16 for tokens 4*(l/16)..+3 of both tiles, the B operand if
+//   k index 8*(l/16) + j stands for token 4*(l/16) + j%4 of tile j/4; lane l reads the
+//   l%16-th part of those eight rows, D / 16 channels of 8 tokens, which are D / 16 A
+//   operands.  A weight times s_v goes in as three bf16, all of its 24 bits (two, 18 bits: 4.3
+//   us less of 67 where 40 columns share a KV head, nothing in the other cases).  In 4 bits a
+//   shift and an and-or put two codes into the mantissas of two bf16 of exponent 4, 16 +
+//   c: the 16s are taken off through the sum of p (low_v - 16 s_v).
+// With 8 columns or fewer the tile's other columns repeat them, and a lane does the softmax
+// of only a half of its tokens (4 or fewer: a quarter) and gets the other weights from
+// the lanes that did them: 231 vector instructions a pair for 8 columns, 290 for 16.
+//
+// What bounds it: 64 sequences' 8000 tokens (64 / 8 heads of 128 in 4 bits, 557 MB) take 106
+// us, 5.3 TB/s, where a kernel that only reads them takes 98; with 16 columns and more
+// the vector instructions do (three tiles of columns over 113 MB: 67 us, reading
+// alone 37); one sequence's 32000 tokens 13.5 us and 4 for the merge, start, loads and
+// merge being a chain of latencies.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -48,16 +61,21 @@ struct QuantAttnParams {
   const int32_t* seqlens;
   uint16_t* out;  // [B][new][H][D]
   float* lse;     // [B][H][new] or null
-  float* ws_o;    // [row][splits][D], rows in the order of lse (splits > 1)
-  float* ws_ml;   // [row][splits][2]
-  int num_blocks, width, page, heads, heads_k, group, new_tokens, columns, splits;
+  float* ws_o;    // [slot][Hkv][columns of a KV head][D] (where sequences may be cut)
+  float* ws_ml;   // [slot][Hkv][columns][2]: maximum (log2 domain) and sum
+  int2* ws_plan;  // [B]: a sequence's first slot and its splits (where they go by the lengths)
+  int num_blocks, width, page, heads, heads_k, group, new_tokens, columns, batch;
+  int splits;           // of every sequence, or 0: by the lengths
+  int parts;            // of all sequences together, where they are cut by the lengths
   FastDiv tiles;        // 16-token tiles of a page
   FastDiv over_group;   // a column's new token
-  FastDiv over_heads_k;
-  float scale_log2;
+  FastDiv over_heads_k, over_column_tiles, over_splits;
+  float scale_log2, flip;  // of the softmax scale: its size, and its sign as 1 or -1
 };
 
 constexpr int kQaWaves = 4;
+constexpr int kParts = 3;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 template <int D, int kBits>
 struct QaShape {
@@ -77,11 +95,16 @@ __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* w) {
   for (int i = 0; i < N; ++i) w[i] = x[i];
 }
 
-// Nibble i of both halves of w as two bf16 of 16 + code.
+// Nibble i of both halves of w as two bf16 of 16 + code.  (The constants come out
+// of registers: with literals the and-or is two instructions.)
+struct NibbleBits {
+  uint32_t mask = 0x00780078u, sixteen = 0x41804180u;
+  __device__ __forceinline__ NibbleBits() { asm("" : "+s"(mask), "+v"(sixteen)); }
+};
 template <int i>
-__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w) {
+__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w, const NibbleBits& c) {
   const uint32_t x = 4 * i < 3 ? w << (3 - 4 * i) : w >> (4 * i - 3);
-  return (x & 0x00780078u) | 0x41804180u;
+  return (x & c.mask) | c.sixteen;
 }
 
 // Bytes i of a and b as two bf16.
@@ -91,17 +114,37 @@ __device__ __forceinline__ uint32_t bytes_bf16(uint32_t a, uint32_t b) {
   return __builtin_amdgcn_perm(y, x, 0x07060302);
 }
 
-// Step c's operand from a lane's piece of a key row.
+// Step c's operand from a lane's piece of a key row: codes as fp16 subnormals, which
+// the matrix cores take as they are, code * 2^-24.  In 4 bits the second nibble of
+// each byte stays where it is, 16 times as large, and q is 1/16 there.
 template <int kBits>
-__device__ __forceinline__ bf16x8 key_operand(const uint32_t* w, int c) {
+__device__ __forceinline__ f16x8 key_operand(const uint32_t* w, int c) {
   u32x4 x;
   if constexpr (kBits == 4) {
-    x = u32x4{nibbles_bf16<0>(w[c]), nibbles_bf16<1>(w[c]), nibbles_bf16<2>(w[c]), nibbles_bf16<3>(w[c])};
+    const uint32_t y = w[c] >> 8;
+    x = u32x4{w[c] & 0x000F000Fu, w[c] & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u};
   } else {
-    const uint32_t a = w[2 * c], b = w[2 * c + 1];
-    x = u32x4{bytes_bf16<0>(a, a >> 8), bytes_bf16<2>(a, a >> 8), bytes_bf16<0>(b, b >> 8), bytes_bf16<2>(b, b >> 8)};
+    const uint32_t u = w[2 * c], v = w[2 * c + 1];
+    x = u32x4{u & 0x00FF00FFu, u >> 8 & 0x00FF00FFu, v & 0x00FF00FFu, v >> 8 & 0x00FF00FFu};
   }
-  return as_bf16x8(x);
+  return __builtin_bit_cast(f16x8, x);
+}
+
+// The same channels of q, 8 bf16 times `factor` (a power of two), in the order and
+// with the factors of a key operand.
+template <int kBits>
+__device__ __forceinline__ f16x8 query_operand(u32x4 in, float factor) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(in[i] << 16) * factor;
+    x[2 * i + 1] = __uint_as_float(in[i] & 0xFFFF0000u) * factor;
+  }
+  f16x8 y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    y[i] = (_Float16)(kBits == 4 ? x[i] * (i & 2 ? 0.0625f : 1.f) : x[(i & 4) + (i & 1) * 2 + (i >> 1 & 1)]);
+  return y;
 }
 
 // A lane's parts of eight value rows, and the operand of output tile n from them:
@@ -112,15 +155,15 @@ struct ValuePart;
 template <>
 struct ValuePart<128, 4> {
   uint32_t w[8];
-  __device__ __forceinline__ void load(int j, const uint8_t* row, int g) {
-    w[j] = *reinterpret_cast<const uint32_t*>(row + 4 * g);
+  __device__ __forceinline__ void load(int j, const uint8_t* part) {
+    w[j] = *reinterpret_cast<const uint32_t*>(part);
   }
   template <int n>
-  __device__ __forceinline__ bf16x8 operand() const {
+  __device__ __forceinline__ bf16x8 operand(const NibbleBits& nb) const {
     u32x4 x;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      x[i] = nibbles_bf16<n / 2>(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], n % 2 ? 0x07060302 : 0x05040100));
+      x[i] = nibbles_bf16<n / 2>(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], n % 2 ? 0x07060302 : 0x05040100), nb);
     return as_bf16x8(x);
   }
 };
@@ -128,14 +171,14 @@ struct ValuePart<128, 4> {
 template <>
 struct ValuePart<64, 4> {
   uint16_t w[8];
-  __device__ __forceinline__ void load(int j, const uint8_t* row, int g) {
-    w[j] = *reinterpret_cast<const uint16_t*>(row + 2 * g);
+  __device__ __forceinline__ void load(int j, const uint8_t* part) {
+    w[j] = *reinterpret_cast<const uint16_t*>(part);
   }
   template <int n>
-  __device__ __forceinline__ bf16x8 operand() const {
+  __device__ __forceinline__ bf16x8 operand(const NibbleBits& nb) const {
     u32x4 x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = nibbles_bf16<n>((uint32_t)w[2 * i] | (uint32_t)w[2 * i + 1] << 16);
+    for (int i = 0; i < 4; ++i) x[i] = nibbles_bf16<n>((uint32_t)w[2 * i] | (uint32_t)w[2 * i + 1] << 16, nb);
     return as_bf16x8(x);
   }
 };
@@ -144,9 +187,9 @@ template <int D>
 struct ValuePart<D, 8> {
   static constexpr int kW = D / 64;
   uint32_t w[8][kW];
-  __device__ __forceinline__ void load(int j, const uint8_t* row, int g) { load_words<kW>(row + 4 * kW * g, w[j]); }
+  __device__ __forceinline__ void load(int j, const uint8_t* part) { load_words<kW>(part, w[j]); }
   template <int n>
-  __device__ __forceinline__ bf16x8 operand() const {
+  __device__ __forceinline__ bf16x8 operand(const NibbleBits& nb) const {
     u32x4 x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = bytes_bf16<n % 4>(w[2 * i][n / 4], w[2 * i + 1][n / 4]);
@@ -170,221 +213,453 @@ __device__ __forceinline__ void unrolled(F&& f) {
   }
 }
 
-template <int D, int kBits>
-__global__ __launch_bounds__(kQaWaves * 64) void quant_attn_kernel(QuantAttnParams p) {
+// How the tokens of a batch are cut.  Either every sequence into the same number of
+// splits, or, where that is left open, the tiles of all sequences, one behind another, into
+// p.parts equal parts, so that every workgroup has as much to do however the lengths differ:
+// a workgroup takes what its part has of each sequence, one after the other.  Part i
+// starts at tile floor(i T / P) of the T.  What it has of a sequence that it does not
+// have whole goes into slot 2 i, or 2 i + 1 where the sequence starts inside the part (a
+// part has one at most that ends, and one that starts, outside it).
+constexpr int kLeastChunk = 32;  // tiles of a part at least
+
+__device__ __forceinline__ int qa_tiles_of(const QuantAttnParams& p, int len) {
+  return (int)min(((int64_t)max(len, 0) + 15) / 16, (int64_t)p.width * p.tiles.d);
+}
+
+// (Products below 2^53 are exact, and so is the floor of a quotient of them.)
+__device__ __forceinline__ int qa_part_start(int i, int parts, int total) {
+  return (int)floor((double)i * total / parts);
+}
+// The part that tile t is in: the last i with floor(i T / P) <= t.
+__device__ __forceinline__ int qa_part_of(int t, int parts, int total) {
+  return (int)floor(((double)(t + 1) * parts - 1) / total);
+}
+
+// The lane, and what is made of it, anew: kept over a loop that it is used in at both ends
+// it takes registers.
+__device__ __forceinline__ int qa_lane() {
+  int l = lane_id();
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
+// The waves' states of a tile of columns merged and written, two output tiles a wave: the
+// result, or what goes into a slot (slot >= 0).
+template <int D, int kBits, int kColumns>
+__device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem, const f32x4* O, float m_own, float l_own,
+                                          float z, int ct, int h, int b, int slot) {
   typedef QaShape<D, kBits> Shape;
-  typedef QuantRow<D, kBits> Row;
-  constexpr int kC = Shape::kC, kO = Shape::kO, W = kQaWaves;
-  __shared__ float smem[W * Shape::kState];
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
-  const int g = l & 15, lg = l >> 4;
-  const int ct = (int)p.over_heads_k.div(blockIdx.y), h = blockIdx.y - ct * p.heads_k, b = blockIdx.z;
-  const int len = max(p.seqlens[b], 0);
-
-  // the split's tiles: an equal part of those that the sequence has
-  const int all = (int)min(((int64_t)len + 15) / 16, (int64_t)p.width * p.tiles.d);
-  const int t0 = (int)((int64_t)all * blockIdx.x / p.splits), t1 = (int)((int64_t)all * (blockIdx.x + 1) / p.splits);
-
-  // this lane's column: new token `fresh` of head h * group + hh; it sees `limit` tokens
-  const int column = min(16 * ct + g, p.columns - 1);
-  const int fresh = (int)p.over_group.div((uint32_t)column), hh = column - fresh * p.group;
-  const int first = len - p.new_tokens + 1, limit = first + fresh;
-  bf16x8 Q[kC];
-  {
-    const uint16_t* row = p.q + b * p.q_batch + fresh * p.q_token + (int64_t)(h * p.group + hh) * p.q_head + D / 4 * lg;
-#pragma unroll
-    for (int c = 0; c < kC; ++c) Q[c] = *reinterpret_cast<const bf16x8*>(row + 8 * c);
-  }
-  // the sum of the column's q, and what the 16s of 4-bit codes add to a score
-  f32x4 sum_q = {0.f, 0.f, 0.f, 0.f};
-  {
-    const bf16x8 ones = as_bf16x8(u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
-#pragma unroll
-    for (int c = 0; c < kC; ++c) sum_q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, Q[c], sum_q, 0, 0, 0);
-  }
-  const float qs = sum_q[0] * p.scale_log2;
-  const f32x4 start = sum_q * (kBits == 4 ? -16.f : 0.f);
-
-  f32x4 O[kO];
-#pragma unroll
-  for (int i = 0; i < kO; ++i) O[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -INFINITY, l_run = 0.f, z = 0.f;  // z: sum p low_v, and the 16s
-
-  const int page = p.page;
-  const int k_at = 8 * page + g * Row::kBytes + 4 * Shape::kKey * lg;
-  const int v_at = (8 + Row::kBytes) * page + 4 * lg * Row::kBytes;
-
-  // Lane i holds the place of tile i%2 of the wave's (32 c0 + i/2)-th pair: its page
-  // (-1: none of the pool, or no tile of the split) and its tile there.
-  for (int c0 = 0; t0 + 2 * (w + W * 32 * c0) < t1; ++c0) {
-    int block = -1, sub = 0;
-    {
-      const int tile = t0 + 2 * (w + W * (32 * c0 + (l >> 1))) + (l & 1);
-      if (tile < t1) {
-        const int lp = (int)p.tiles.div((uint32_t)tile);
-        sub = tile - lp * (int)p.tiles.d;
-        block = p.table[b * p.table_stride + lp];
-        if (block >= p.num_blocks) block = -1;
-      }
-    }
-    for (int i = 0; i < 32; ++i) {
-      const int tile = t0 + 2 * (w + W * (32 * c0 + i));
-      if (tile >= t1) break;
-      int b0 = __builtin_amdgcn_readlane(block, 2 * i), s0 = __builtin_amdgcn_readlane(sub, 2 * i);
-      int b1 = __builtin_amdgcn_readlane(block, 2 * i + 1), s1 = __builtin_amdgcn_readlane(sub, 2 * i + 1);
-      if (b0 < 0 && b1 < 0) continue;
-      const bool none0 = b0 < 0, none1 = b1 < 0;  // a tile without a page reads the other's
-      if (none0) b0 = b1, s0 = s1;
-      if (none1) b1 = b0, s1 = s0;
-      const uint8_t* r0 = p.cache + ((int64_t)b0 * p.heads_k + h) * p.record;
-      const uint8_t* r1 = p.cache + ((int64_t)b1 * p.heads_k + h) * p.record;
-      uint32_t K0[Shape::kKey], K1[Shape::kKey], side[2][8];
-      ValuePart<D, kBits> V;
-      load_words<Shape::kKey>(r0 + k_at + 16 * s0 * Row::kBytes, K0);
-      load_words<Shape::kKey>(r1 + k_at + 16 * s1 * Row::kBytes, K1);
-      load_words<8>(r0 + 8 * (16 * s0 + 4 * lg), side[0]);
-      load_words<8>(r1 + 8 * (16 * s1 + 4 * lg), side[1]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        V.load(j, r0 + v_at + (16 * s0 + j) * Row::kBytes, g);
-        V.load(4 + j, r1 + v_at + (16 * s1 + j) * Row::kBytes, g);
-      }
-      f32x4 S0 = start, S1 = start;
-#pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        S0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key_operand<kBits>(K0, c), Q[c], S0, 0, 0, 0);
-        S1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key_operand<kBits>(K1, c), Q[c], S1, 0, 0, 0);
-      }
-      float s[8], vs[8], vl[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t kp = side[j / 4][2 * (j % 4)], vp = side[j / 4][2 * (j % 4) + 1];
-        const float ks = __uint_as_float(kp << 16), kl = __uint_as_float(kp & 0xFFFF0000u);
-        s[j] = fmaf(ks * p.scale_log2, j < 4 ? S0[j % 4] : S1[j % 4], kl * qs);
-        vs[j] = __uint_as_float(vp << 16);
-        vl[j] = __uint_as_float(vp & 0xFFFF0000u);
-      }
-      // Behind a column's limit and where there is no page nothing counts, whatever it holds.
-      if (none0 || none1 || first - 16 * tile < 32) {  // (uniform)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool seen = 16 * (j / 4) + 4 * lg + j % 4 < limit - 16 * tile && !(j < 4 ? none0 : none1);
-          s[j] = seen ? s[j] : -INFINITY;
-          vs[j] = seen ? vs[j] : 0.f;
-          vl[j] = seen ? vl[j] : 0.f;
-        }
-      }
-      float mx = s[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[j]);
-      const float m_new = fmaxf(m_run, wave_max16(mx));
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-      m_run = m_new;
-      l_run *= alpha;
-      z *= alpha;
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
-#pragma unroll
-        for (int k = 0; k < kO; ++k) O[k] *= alpha;
-      }
-      // weights times scales as sums of three bf16, all of their 24 bits
-      u32x4 hi, mid, lo;
-#pragma unroll
-      for (int i2 = 0; i2 < 4; ++i2) {
-        uint32_t a[2], c[2], d[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = 2 * i2 + e;
-          const float x = __builtin_amdgcn_exp2f(s[j] - m_use);
-          l_run += x;
-          const float y = x * vs[j];
-          z = fmaf(x, vl[j], z);
-          if constexpr (kBits == 4) z = fmaf(y, -16.f, z);
-          a[e] = __float_as_uint(y) & 0xFFFF0000u;
-          const float r = y - __uint_as_float(a[e]);
-          c[e] = __float_as_uint(r) & 0xFFFF0000u;
-          d[e] = __float_as_uint(r - __uint_as_float(c[e]));
-        }
-        hi[i2] = __builtin_amdgcn_perm(a[1], a[0], 0x07060302);
-        mid[i2] = __builtin_amdgcn_perm(c[1], c[0], 0x07060302);
-        lo[i2] = __builtin_amdgcn_perm(d[1], d[0], 0x07060302);
-      }
-      unrolled<0, kO>([&](auto n) {
-        constexpr int k = decltype(n)::value;
-        const bf16x8 A = V.template operand<k>();
-        O[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, as_bf16x8(hi), O[k], 0, 0, 0);
-        O[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, as_bf16x8(mid), O[k], 0, 0, 0);
-        O[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, as_bf16x8(lo), O[k], 0, 0, 0);
-      });
-    }
-  }
-
-  // The waves' states merged by the first one.
-  l_run = wave_sum16(l_run);
-  z = wave_sum16(z);
+  constexpr int kO = Shape::kO, W = kQaWaves;
+  static_assert(W >= kO / 2, "");
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = qa_lane(), lg = l >> 4;
   float* cb = smem + w * Shape::kState + l;
 #pragma unroll
   for (int i = 0; i < kO; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) cb[(4 * i + r) * 64] = O[i][r] + z;
-  cb[4 * kO * 64] = m_run;
-  cb[(4 * kO + 1) * 64] = l_run;
+  cb[4 * kO * 64] = m_own;
+  cb[(4 * kO + 1) * 64] = l_own;
   __syncthreads();
-  if (w != 0) return;
+  if (w >= kO / 2) return;
   const float* src = smem + l;
-  float m = -INFINITY;
+  float m = -FLT_MAX, sum = 0.f, o[2][4] = {};
 #pragma unroll
   for (int i = 0; i < W; ++i) m = fmaxf(m, src[i * Shape::kState + 4 * kO * 64]);
-  const float m_use = m == -INFINITY ? 0.f : m;
-  float sum = 0.f, o[4 * kO];
-#pragma unroll
-  for (int i = 0; i < 4 * kO; ++i) o[i] = 0.f;
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    const float f = __builtin_amdgcn_exp2f(src[i * Shape::kState + 4 * kO * 64] - m_use);
+    const float f = __builtin_amdgcn_exp2f(src[i * Shape::kState + 4 * kO * 64] - m);
     sum += src[i * Shape::kState + (4 * kO + 1) * 64] * f;
 #pragma unroll
-    for (int k = 0; k < kO; ++k)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[qa_channel<D, kBits>(r, k)] += src[i * Shape::kState + (4 * k + r) * 64] * f;
+      for (int r = 0; r < 4; ++r) o[n][r] += src[i * Shape::kState + (4 * (2 * w + n) + r) * 64] * f;
   }
-  if (16 * ct + g >= p.columns) return;
-  const int head = h * p.group + hh;
-  const int64_t row = ((int64_t)b * p.heads + head) * p.new_tokens + fresh;
-  if (p.splits == 1) {
+  const int column = kColumns * ct + (l & 15);
+  if ((l & 15) >= kColumns || column >= p.columns) return;
+  // neighbouring channels: (r, 0), (r, 1), or with two codes of a byte apart (2i, 0),
+  // (2i + 1, 0), (2i, 1), (2i + 1, 1)
+  constexpr bool kFour = D == 64 && kBits == 4;
+  static_assert(qa_channel<D, kBits>(1, 0) == (kFour ? 1 : D / 16), "");
+  const int at = D / 4 * lg + (kFour ? 4 : 2) * w;
+  const int fresh = (int)p.over_group.div((uint32_t)column), head = h * p.group + column - fresh * p.group;
+  if (slot < 0) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint16_t* out = p.out + (((int64_t)b * p.new_tokens + fresh) * p.heads + head) * D + D / 4 * lg;
+    uint16_t* out = p.out + (((int64_t)b * p.new_tokens + fresh) * p.heads + head) * D + at;
+    if constexpr (kFour) {
 #pragma unroll
-    for (int i = 0; i < kO / 2; ++i) {
-      u32x4 x;
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<uint2*>(out + 8 * i) = uint2{pack_bf16x2(o[0][2 * i] * inv, o[0][2 * i + 1] * inv),
+                                                       pack_bf16x2(o[1][2 * i] * inv, o[1][2 * i + 1] * inv)};
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = pack_bf16x2(o[8 * i + 2 * j] * inv, o[8 * i + 2 * j + 1] * inv);
-      *reinterpret_cast<u32x4*>(out + 8 * i) = x;
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<uint32_t*>(out + D / 16 * r) = pack_bf16x2(o[0][r] * inv, o[1][r] * inv);
     }
-    if (p.lse && lg == 0) p.lse[row] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * 0.6931471805599453f;
+    if (p.lse && lg == 0 && w == 0)
+      p.lse[((int64_t)b * p.heads + head) * p.new_tokens + fresh] =
+          sum == 0.f ? -INFINITY : (m + __log2f(sum)) * 0.6931471805599453f;
   } else {
-    const int64_t slot = row * p.splits + blockIdx.x;
-    float* out = p.ws_o + slot * D + D / 4 * lg;
+    const int64_t row = ((int64_t)slot * p.heads_k + h) * p.columns + column;
+    float* out = p.ws_o + row * D + at;
+    if constexpr (kFour) {
 #pragma unroll
-    for (int i = 0; i < kO; ++i)
-      *reinterpret_cast<f32x4*>(out + 4 * i) = f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
-    if (lg == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * slot) = float2{m, sum};
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<f32x4*>(out + 8 * i) = f32x4{o[0][2 * i], o[0][2 * i + 1], o[1][2 * i], o[1][2 * i + 1]};
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) *reinterpret_cast<float2*>(out + D / 16 * r) = float2{o[0][r], o[1][r]};
+    }
+    if (lg == 0 && w == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * row) = float2{m, sum};
   }
 }
 
-// How many splits: one workgroup a CU, each wave with a pair of tiles at least.
-static int qa_splits(int batch, int units, int64_t tiles, int num_splits) {
-  const int64_t most = std::max<int64_t>(1, (tiles + 2 * kQaWaves - 1) / (2 * kQaWaves));
-  const int64_t want = num_splits > 0 ? num_splits : std::max<int64_t>(1, device_cu_count() / ((int64_t)batch * units));
-  return (int)std::min(want, most);
+// What a wave has of a pair of tiles: codes, and (scale, low) of the keys and values of
+// the lane's kTokens tokens.
+template <int D, int kBits, int kTokens>
+struct QaPair {
+  uint32_t k[2][QaShape<D, kBits>::kKey], side[2 * kTokens];
+  ValuePart<D, kBits> v;
+  int tile;        // the first one's number in the sequence
+  bool none[2];    // no page of the pool
+};
+
+// What no kernel writes while this one runs, for scalar loads.
+typedef const int32_t __attribute__((address_space(4))) * ConstantInts;
+__device__ __forceinline__ ConstantInts as_constant(const int32_t* p) { return (ConstantInts)(uintptr_t)p; }
+
+// Lane l's x from lane l%16 + kBy (of the 16, going round) of its row.
+template <int kBy>
+__device__ __forceinline__ uint32_t row_from(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, 0x120 + 16 - kBy, 0xF, 0xF, false);  // row_ror
+}
+__device__ __forceinline__ float row_from8(float x) { return __uint_as_float(row_from<8>(__float_as_uint(x))); }
+__device__ __forceinline__ float row_from4(float x) { return __uint_as_float(row_from<4>(__float_as_uint(x))); }
+
+template <int D, int kBits, int kFold>
+__global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 ? 2 : 3) void quant_attn_kernel(QuantAttnParams p) {
+  typedef QaShape<D, kBits> Shape;
+  typedef QuantRow<D, kBits> Row;
+  constexpr int kC = Shape::kC, kO = Shape::kO, W = kQaWaves;
+  constexpr int kColumns = 16 / kFold, kTokens = 8 / kFold;  // of a tile of columns; a lane's tokens of a pair
+  typedef QaPair<D, kBits, kTokens> Pair;
+  __shared__ float smem[W * Shape::kState];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+  // Column tiles of the same tokens go to one XCD (workgroups are dealt out to the
+  // eight in turn), one soon after another.
+  const int item = (int)p.over_column_tiles.div(blockIdx.x >> 3), ct = (int)(blockIdx.x >> 3) - item * (int)p.over_column_tiles.d;
+  const int at = 8 * item + (blockIdx.x & 7);
+  const int part = (int)p.over_heads_k.div((uint32_t)at), h = at - part * p.heads_k;
+
+  // The range of tiles, and the first sequence that has any of it (one without tiles
+  // belongs to the part that its place is in), with its length and first tile.
+  int from, to, b, len, start = 0, parts = 0, total = 0;
+  const ConstantInts lens = as_constant(p.seqlens);
+  if (p.splits) {  // (uniform)
+    b = (int)p.over_splits.div((uint32_t)part);
+    if (b >= p.batch) return;
+    len = lens[b];
+    const int tiles = qa_tiles_of(p, len), i = part - b * p.splits;
+    from = (int)((int64_t)tiles * i / p.splits);
+    to = (int)((int64_t)tiles * (i + 1) / p.splits);
+  } else {
+    // lane i: sequence s0 + i; one sequence alone by scalars, 1 us sooner
+    int s0 = 0, mine = 0, tiles = 0, end = 0;
+    auto look = [&](int before) {
+      mine = s0 + l < p.batch ? p.seqlens[s0 + l] : 0;
+      tiles = qa_tiles_of(p, mine);
+      end = before + wave_inclusive_scan(tiles);
+      return __builtin_amdgcn_readlane(end, 63);
+    };
+    if (p.batch == 1)
+      total = qa_tiles_of(p, lens[0]);
+    else
+      for (; s0 < p.batch; s0 += 64) total = look(total);
+    parts = min(p.parts, max(1, total / kLeastChunk));
+    if (part >= parts) return;
+    from = qa_part_start(part, parts, total);
+    to = qa_part_start(part + 1, parts, total);
+    if (p.batch == 1) {
+      b = 0;
+      len = lens[0];
+    } else {
+      s0 = 0;
+      if (p.batch > 64)
+        for (int before = look(0); before <= from && s0 + 64 < p.batch;) s0 += 64, before = look(before);
+      const bool has = s0 + l < p.batch && (tiles ? end > from : end >= from);
+      const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(has) | 1ull << 63);
+      b = s0 + i;
+      len = __builtin_amdgcn_readlane(mine, i);
+      start = __builtin_amdgcn_readlane(end, i) - __builtin_amdgcn_readlane(tiles, i);
+    }
+  }
+
+  auto segment = [&](int len, int t0, int t1, int slot) {
+  const int l = qa_lane();
+  const int g = l & 15, lg = l >> 4;
+  const int fold = g / kColumns;
+  // the lane's tokens of a pair: kTokens from `token` of tile `mine` (all of both: 4 each)
+  const int mine = fold * 2 / kFold, token = 4 * lg + (kFold == 4 ? 2 * (fold & 1) : 0);
+  // Where the two tiles of the wave's n-th pair are: the table's entry and the tile in the
+  // page.  Scalar loads, which the many vector loads on the way do not have to be waited
+  // out for, and looked at only when the pair is fetched.
+  struct Place {
+    int block[2], sub[2];
+  };
+  const volatile auto* row = as_constant(p.table + b * p.table_stride);  // (volatile: or the loads move to their use)
+  auto places = [&](int n) {
+    Place x;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int tile = t0 + 2 * (w + W * n) + t;
+      const int lp = (int)p.tiles.div((uint32_t)min(tile, t1 - 1));
+      x.sub[t] = tile - lp * (int)p.tiles.d;
+      x.block[t] = row[lp];
+    }
+    return x;
+  };
+  const uint32_t k_at = g * Row::kBytes + 4 * Shape::kKey * lg, v_at = 4 * lg * Row::kBytes + Row::kBytes / 16 * g;
+  // The wave's n-th pair, on its way.  A tile without a page reads page 0.
+  auto fetch = [&](Pair& x, const Place& at, int n) {
+    x.tile = t0 + 2 * (w + W * n);
+    const uint8_t* kr[2];
+    const uint8_t* vr[2];
+    const uint8_t* sr[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x.none[t] = (uint32_t)at.block[t] >= (uint32_t)p.num_blocks || x.tile + t >= t1;
+      const int bl = x.none[t] ? 0 : at.block[t], su = x.none[t] ? 0 : at.sub[t];
+      // (scalar addresses, and a lane's own part in 32 bits)
+      const uint8_t* record = p.cache + ((int64_t)bl * p.heads_k + h) * p.record;
+      kr[t] = record + 8 * p.page + 16 * su * Row::kBytes;
+      vr[t] = kr[t] + p.page * Row::kBytes;
+      load_words<Shape::kKey>(kr[t] + k_at, x.k[t]);
+      sr[t] = record + 128 * su;
+    }
+    if constexpr (kFold == 1) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) load_words<8>(sr[t] + 32u * lg, x.side + 8 * t);
+    } else {
+      load_words<2 * kTokens>((mine ? sr[1] : sr[0]) + 8u * token, x.side);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.v.load(j, vr[j / 4] + v_at + j % 4 * Row::kBytes);
+  };
+  const int pairs = t1 - t0 - 2 * w > 0 ? (t1 - t0 - 2 * w + 2 * W - 1) / (2 * W) : 0;  // of this wave
+  Pair pair[2];
+  Place ahead[2];
+  if (pairs > 0) {
+    ahead[0] = places(0);
+    ahead[1] = places(1);
+    fetch(pair[0], ahead[0], 0);
+  }
+
+  // This lane's column: new token `fresh` of head h * group + hh; it sees `limit` tokens.
+  // q goes in as fp16, times a power of two that takes the largest of a column's to
+  // 2^14..2^15: of the others nothing above 2^-39 of that is lost.  Scores are kept
+  // without `unit`, which is left to do.
+  const int first = len - p.new_tokens + 1;
+  f16x8 Q[kC];
+  float qs, unit;
+  int limit;
+  {
+    const int column = min(kColumns * ct + g % kColumns, p.columns - 1);
+    const int fresh = (int)p.over_group.div((uint32_t)column), hh = column - fresh * p.group;
+    limit = first + fresh;
+    const uint16_t* row = p.q + b * p.q_batch + fresh * p.q_token + (int64_t)(h * p.group + hh) * p.q_head + D / 4 * lg;
+    u32x4 x[kC];
+    float sum = 0.f, most = 0.f;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      x[c] = *reinterpret_cast<const u32x4*>(row + 8 * c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float u = __uint_as_float(x[c][j] << 16), v = __uint_as_float(x[c][j] & 0xFFFF0000u);
+        sum += u + v;
+        most = fmaxf(most, fmaxf(fabsf(u), fabsf(v)));
+      }
+    }
+    most = wave_max16(most);
+    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
+    const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) Q[c] = query_operand<kBits>(x[c], p.flip * up);
+    qs = wave_sum16(sum) * (p.flip * up * 0x1p-24f);
+    unit = fmaxf(p.scale_log2 * __uint_as_float((uint32_t)(127 + 10 + e) << 23), FLT_MIN);  // (0 times -inf is none)
+  }
+
+  f32x4 O[kO];
+#pragma unroll
+  for (int k = 0; k < kO; ++k) O[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -FLT_MAX, l_run = 0.f, z = 0.f;  // z: sum p low_v, the 16s taken off
+  const NibbleBits nb;
+
+  auto consume = [&](const Pair& x) {
+    f32x4 S[2] = {};
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const f16x8 K0 = key_operand<kBits>(x.k[0], c), K1 = key_operand<kBits>(x.k[1], c);
+      S[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K0, Q[c], S[0], 0, 0, 0);
+      S[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K1, Q[c], S[1], 0, 0, 0);
+    }
+    float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens];
+#pragma unroll
+    for (int j = 0; j < kTokens; ++j) {
+      const uint32_t kp = x.side[2 * j], vp = x.side[2 * j + 1];
+      ks[j] = __uint_as_float(kp << 16);
+      kl[j] = __uint_as_float(kp & 0xFFFF0000u);
+      vs[j] = __uint_as_float(vp << 16);
+      vl[j] = __uint_as_float(vp & 0xFFFF0000u);
+      if constexpr (kBits == 4) vl[j] = fmaf(vs[j], -16.f, vl[j]);
+    }
+    // Behind a column's limit and where there is no page nothing counts, whatever it holds.
+    const bool cut = x.none[0] || x.none[1] || first - 16 * x.tile < 32;  // (uniform)
+    constexpr int kWords = kTokens / 2;                                   // packed pairs of a lane's weights
+    u32x4 weights[kParts];
+    {
+      float s[kTokens], vs_i[kTokens], vl_i[kTokens];
+#pragma unroll
+      for (int j = 0; j < kTokens; ++j) {
+        float c;
+        if constexpr (kFold == 1)
+          c = S[j / 4][j % 4];
+        else if constexpr (kFold == 2)
+          c = fold ? S[1][j] : S[0][j];
+        else
+          c = fold & 2 ? (fold & 1 ? S[1][2 + j] : S[1][j]) : (fold & 1 ? S[0][2 + j] : S[0][j]);
+        s[j] = fmaf(ks[j], c, kl[j] * qs);
+        vs_i[j] = vs[j];
+        vl_i[j] = vl[j];
+      }
+      if (cut) {
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+          const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
+          const bool seen = at < limit - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
+          s[j] = seen ? s[j] : -INFINITY;
+          vs_i[j] = seen ? vs[j] : 0.f;
+          vl_i[j] = seen ? vl[j] : 0.f;
+        }
+      }
+      // The maximum is moved only where a score is 8 above it, that is a weight 2^8 where
+      // 1 was the most: sums lose nothing by that.
+      float mx = s[0];
+#pragma unroll
+      for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, s[j]);
+      if (__builtin_amdgcn_ballot_w64(mx * unit > m_run + 8.f)) {
+        if constexpr (kFold >= 2) mx = fmaxf(mx, row_from8(mx));
+        if constexpr (kFold == 4) mx = fmaxf(mx, row_from4(mx));
+        const float m_new = fmaxf(m_run, wave_max16(mx) * unit);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
+        z *= alpha;
+#pragma unroll
+        for (int k = 0; k < kO; ++k) O[k] *= alpha;
+      }
+      // weights times scales as sums of three bf16, all of their 24 bits
+      uint32_t own[kParts][kWords];
+#pragma unroll
+      for (int j = 0; j < kTokens; j += 2) {
+        float r[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float weight = __builtin_amdgcn_exp2f(fmaf(s[j + e], unit, -m_run));
+          l_run += weight;
+          z = fmaf(weight, vl_i[j + e], z);
+          r[e] = weight * vs_i[j + e];
+        }
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+          const uint32_t a = pack_bf16x2(r[0], r[1]);
+          own[k][j / 2] = a;
+          r[0] -= __uint_as_float(a << 16);
+          r[1] -= __uint_as_float(a & 0xFFFF0000u);
+        }
+      }
+      // the other folds' tokens of the column
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) {
+        if constexpr (kFold == 1)
+          weights[k] = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
+        else if constexpr (kFold == 2)
+          weights[k] = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
+        else
+          weights[k] = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
+      }
+    }
+    unrolled<0, kO>([&](auto n) {
+      constexpr int o = decltype(n)::value;
+      const bf16x8 A = x.v.template operand<o>(nb);
+#pragma unroll
+      for (int k = 0; k < kParts; ++k)
+        O[o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, as_bf16x8(weights[k]), O[o], 0, 0, 0);
+    });
+  };
+
+  // A pair's loads go out while the one before is worked on, and its places are read one
+  // pair earlier still.  (Past the last pair page 0 is read, so that the number of loads
+  // on the way is known.)
+  for (int n = 0; n < pairs; n += 2) {
+    fetch(pair[1], ahead[1], n + 1);
+    ahead[0] = places(n + 2);
+    consume(pair[0]);
+    fetch(pair[0], ahead[0], n + 2);
+    ahead[1] = places(n + 3);
+    if (n + 1 < pairs) consume(pair[1]);
+  }
+
+  l_run = wave_sum16(l_run);
+  z = wave_sum16(z);
+  if constexpr (kFold >= 2) l_run += row_from8(l_run), z += row_from8(z);
+  if constexpr (kFold == 4) l_run += row_from4(l_run), z += row_from4(z);
+  qa_finish<D, kBits, kColumns>(p, smem, O, m_run, l_run, z, ct, h, b, slot);
+  };
+
+  for (;;) {
+    const int tiles = qa_tiles_of(p, len);
+    const int t0 = max(from - start, 0), t1 = min(to - start, tiles);
+    int slot = p.splits == 1 ? -1 : part;
+    if (p.splits == 0) {
+      const bool whole = t0 == 0 && t1 == tiles;
+      slot = 2 * part + (start > from);
+      if (t0 == 0 && h == 0 && ct == 0 && threadIdx.x == 0)
+        p.ws_plan[b] = int2{slot, whole ? 1 : qa_part_of(start + tiles - 1, parts, total) + 1 - part};
+      slot = whole ? -1 : slot;
+    }
+    segment(max(len, 0), t0, t1, slot);
+    start += tiles;
+    if (++b >= p.batch || p.splits || (start >= to && part != parts - 1)) return;
+    len = lens[b];
+    __syncthreads();  // the states are read
+  }
 }
 
-static int qa_column_tiles(int heads, int heads_k, int new_tokens) {
-  return (int)(((int64_t)(heads / heads_k) * new_tokens + 15) / 16);
-}
+// How a call is cut.  Tiles of columns: 4 or 8 columns where there are no more, else 16.
+struct QaCut {
+  int64_t columns, column_tiles, groups, slots;  // groups: workgroups of a KV head and a tile of columns
+  int splits, parts;                             // as in the parameters
 
-static size_t qa_ws_bytes(int64_t rows, int head_dim, int splits) {
-  return splits <= 1 ? 0 : (size_t)rows * splits * (head_dim + 2) * sizeof(float);
+  bool whole() const { return splits == 1; }
+  size_t ws_bytes(int batch, int heads_k, int head_dim) const {
+    return whole() ? 0 : (size_t)slots * heads_k * columns * (head_dim + 2) * sizeof(float) + batch * sizeof(int2);
+  }
+};
+
+static QaCut qa_cut(int batch, int new_tokens, int heads, int heads_k, int head_dim, int64_t tiles, int num_splits) {
+  QaCut c{};
+  c.columns = (int64_t)(heads / heads_k) * new_tokens;
+  c.column_tiles = (c.columns + 15) / 16;
+  const int64_t units = c.column_tiles * heads_k, target = (int64_t)(head_dim == 64 ? 4 : 3) * device_cu_count();
+  if (num_splits > 0)
+    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(num_splits, (tiles + 2 * kQaWaves - 1) / (2 * kQaWaves)));
+  else if (tiles <= kLeastChunk || batch * units >= 2 * target || batch * tiles > INT_MAX)
+    c.splits = 1;
+  else
+    c.parts = (int)std::max<int64_t>(1, target / units);
+  if (c.parts > batch) c.parts -= c.parts % batch;  // sequences of one length are cut alike
+  c.groups = c.splits ? (int64_t)batch * c.splits : c.parts;
+  c.slots = c.splits ? c.groups : 2 * c.groups;
+  return c;
 }
 
 }  // namespace zs
@@ -398,9 +673,8 @@ extern "C" size_t zs_decode_attention_quant_workspace_bytes(int batch, int new_t
       head_dim <= 0 || max_blocks_per_seq <= 0 || page_block_size < 16 || num_splits < 0)
     return 0;
   const int64_t rows = (int64_t)batch * num_heads * new_tokens, tiles = (int64_t)max_blocks_per_seq * (page_block_size / 16);
-  const int64_t units = (int64_t)num_heads_k * qa_column_tiles(num_heads, num_heads_k, new_tokens);
-  if (rows > INT_MAX || tiles > INT_MAX || units > 65535) return 0;  // (such a call is refused)
-  return qa_ws_bytes(rows, head_dim, qa_splits(batch, (int)units, tiles, num_splits));
+  if (rows > INT_MAX || tiles > INT_MAX) return 0;  // (such a call is refused)
+  return qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, tiles, num_splits).ws_bytes(batch, num_heads_k, head_dim);
 }
 
 extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, int64_t q_batch_stride,
@@ -423,14 +697,14 @@ extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, 
       ((q_batch_stride | q_token_stride | q_head_stride) & 7))
     return ZS_E_INVAL;
   const int64_t rows = (int64_t)batch * num_heads * new_tokens, tiles = (int64_t)max_blocks_per_seq * (page_block_size / 16);
-  const int64_t columns = (int64_t)(num_heads / num_heads_k) * new_tokens, units = num_heads_k * ((columns + 15) / 16);
-  if (batch > 65535 || units > 65535) return ZS_E_UNSUPPORTED;
   if (rows > INT_MAX || tiles > INT_MAX) return ZS_E_OVERFLOW;
-  QuantAttnParams p{};
-  p.splits = qa_splits(batch, (int)units, tiles, num_splits);
-  if (!grid_fits(p.splits, kQaWaves * 64) || (p.splits > 1 && !grid_fits(rows, kMergeWaves * 64)))
+  const QaCut cut = qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, tiles, num_splits);
+  const int64_t groups = (cut.groups * num_heads_k + 7) / 8 * 8 * cut.column_tiles;
+  if (cut.groups > INT_MAX / num_heads_k || !grid_fits(groups, kQaWaves * 64) ||
+      (!cut.whole() && !grid_fits(merge_parts_groups(batch, num_heads_k, cut.columns), kPartMergeThreads)))
     return ZS_E_OVERFLOW;
-  if (workspace_bytes < qa_ws_bytes(rows, head_dim, p.splits) || (p.splits > 1 && !workspace)) return ZS_E_INVAL;
+  if (workspace_bytes < cut.ws_bytes(batch, num_heads_k, head_dim) || (!cut.whole() && !workspace)) return ZS_E_INVAL;
+  QuantAttnParams p{};
   p.q = q;
   p.q_batch = q_batch_stride;
   p.q_token = q_token_stride;
@@ -442,8 +716,15 @@ extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, 
   p.seqlens = cache_seqlens;
   p.out = out;
   p.lse = softmax_lse;
-  p.ws_o = static_cast<float*>(workspace);
-  p.ws_ml = p.ws_o + (size_t)rows * p.splits * head_dim;
+  if (!cut.whole()) {
+    const size_t ws_rows = (size_t)cut.slots * num_heads_k * cut.columns;
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_ml = p.ws_o + ws_rows * head_dim;
+    p.ws_plan = reinterpret_cast<int2*>(p.ws_ml + 2 * ws_rows);
+  }
+  p.batch = batch;
+  p.splits = cut.splits;
+  p.parts = cut.parts;
   p.num_blocks = num_blocks;
   p.width = max_blocks_per_seq;
   p.page = page_block_size;
@@ -451,15 +732,24 @@ extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, 
   p.heads_k = num_heads_k;
   p.group = num_heads / num_heads_k;
   p.new_tokens = new_tokens;
-  p.columns = (int)columns;
+  p.columns = (int)cut.columns;
   p.tiles = FastDiv::of(page_block_size / 16);
   p.over_group = FastDiv::of(p.group);
   p.over_heads_k = FastDiv::of(num_heads_k);
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.over_column_tiles = FastDiv::of((uint32_t)cut.column_tiles);
+  p.over_splits = FastDiv::of(std::max(1, cut.splits));
+  p.scale_log2 = fabsf(softmax_scale) * 1.4426950408889634f;
+  p.flip = softmax_scale < 0.f ? -1.f : 1.f;
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(p.splits, (unsigned)units, batch), block(kQaWaves * 64);
-  auto launch = [&](auto d, auto n) {
-    hipLaunchKernelGGL((quant_attn_kernel<decltype(d)::value, decltype(n)::value>), grid, block, 0, st, p);
+  const dim3 grid((unsigned)groups), block(kQaWaves * 64);
+  auto launch = [&](auto dim, auto width) {
+    constexpr int D = decltype(dim)::value, kBits = decltype(width)::value;
+    if (cut.columns <= 4)
+      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 4>), grid, block, 0, st, p);
+    else if (cut.columns <= 8)
+      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 2>), grid, block, 0, st, p);
+    else
+      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 1>), grid, block, 0, st, p);
   };
   typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 8> Eight;
@@ -470,8 +760,10 @@ extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, 
   else
     bits == 4 ? launch(Small{}, Four{}) : launch(Small{}, Eight{});
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && p.splits > 1)
-    e = merge_splits(st, SplitMerge::of(p.ws_o, p.ws_ml, out, softmax_lse, p.splits, (int)rows, num_heads, new_tokens),
-                     head_dim);
+  if (e == hipSuccess && !cut.whole()) {
+    PartMerge m{p.ws_o, p.ws_ml, p.splits ? nullptr : p.ws_plan, out, softmax_lse, p.splits, p.columns, new_tokens,
+                p.over_group};
+    e = merge_parts(st, m, batch, num_heads_k, head_dim);
+  }
   return e == hipSuccess ? ZS_OK : (int)e;
 }

@@ -397,7 +397,7 @@ extern "C" int zs_decode_attention_sparse_paged(void* stream, const uint16_t* q,
       hipLaunchKernelGGL((sparse_attn_kernel<D, 2>), grid, dim3(2 * 64), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    return merge_splits(st, SplitMerge::of(p.ws_o, p.ws_ml, p.out, p.lse, p.splits, batch * num_heads, num_heads, 1), D);
+    return merge_splits(st, SplitMerge{p.ws_o, p.ws_ml, p.out, p.lse, p.splits, batch * num_heads}, D);
   };
   const hipError_t e = head_dim == 128 ? launch(std::integral_constant<int, 128>{})
                                        : launch(std::integral_constant<int, 64>{});

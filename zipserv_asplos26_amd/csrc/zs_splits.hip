@@ -1,14 +1,10 @@
 // zs_splits.hip -- the merge of an attention's splits (gfx950).
 #include "zs_splits.hpp"
 
-namespace zs {
+#include <cfloat>
+#include <type_traits>
 
-__device__ __forceinline__ int64_t out_row(const SplitMerge& p, int64_t row) {
-  if (p.new_tokens.d == 1) return row;
-  const uint32_t bh = p.new_tokens.div((uint32_t)row), i = (uint32_t)row - bh * p.new_tokens.d;
-  const uint32_t b = p.over_heads.div(bh), h = bh - b * p.over_heads.d;
-  return ((int64_t)b * p.new_tokens.d + i) * p.heads + h;
-}
+namespace zs {
 
 // The splits of one row merged by four waves: their weights by a
 // lane each, then a wave takes every fourth split, eight loads in flight.
@@ -20,10 +16,10 @@ __global__ __launch_bounds__(kMergeWaves * 64) void merge_kernel(SplitMerge p) {
   __shared__ float weight[kMergeChunk];
   __shared__ float red[kMergeWaves];
   __shared__ float part[kMergeWaves][D];
-  const int64_t head = blockIdx.x;
+  const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane_id();
-  const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + head * p.splits;
-  const float* o = p.ws_o + head * p.splits * D + kV * l;
+  const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + row * p.splits;
+  const float* o = p.ws_o + row * p.splits * D + kV * l;
   float m_run = -INFINITY, sum = 0.f, acc[kV] = {};
   for (int c0 = 0; c0 < p.splits; c0 += kMergeChunk) {
     const int n = min(p.splits - c0, kMergeChunk);
@@ -83,8 +79,105 @@ __global__ __launch_bounds__(kMergeWaves * 64) void merge_kernel(SplitMerge p) {
     x.y += part[i][2 * tid + 1];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint32_t*>(p.out + out_row(p, head) * D + 2 * tid) = pack_bf16x2(x.x * inv, x.y * inv);
-  if (p.lse && tid == 0) p.lse[head] = sum == 0.f ? -INFINITY : (m_run + __log2f(sum)) * 0.6931471805599453f;
+  *reinterpret_cast<uint32_t*>(p.out + row * D + 2 * tid) = pack_bf16x2(x.x * inv, x.y * inv);
+  if (p.lse && tid == 0) p.lse[row] = sum == 0.f ? -INFINITY : (m_run + __log2f(sum)) * 0.6931471805599453f;
+}
+
+// Eight columns of a (sequence, KV head) by eight waves: a wave has a column, or where there
+// are fewer several share one, every kShare-th split each.  Most workgroups of a
+// batch whose sequences are whole have nothing to do, so there are few of them.
+constexpr int kPartWaves = kPartMergeThreads / 64;
+
+template <int D, int kShare>
+__global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge p) {
+  constexpr int kV = D / 64, kColumns = kPartWaves / kShare, kAtOnce = 8;
+  __shared__ float part[kPartWaves][D + 2];
+  const uint32_t bh = p.over_pieces.div(blockIdx.x), piece = blockIdx.x - bh * p.over_pieces.d;
+  const uint32_t b = p.over_heads_k.div(bh), h = bh - b * p.over_heads_k.d;
+  int first = b * p.splits, next = first + 1, step = 1, splits = p.splits;
+  if (p.plan) {
+    const int2 mine = p.plan[b];
+    first = mine.x;
+    next = (first & ~1) + 2;
+    step = 2;
+    splits = mine.y;
+  }
+  if (splits <= 1) return;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+  const int column = piece * kColumns + w / kShare, share = w % kShare;
+  const bool live = column < p.columns;
+  const int64_t rows = (int64_t)p.over_heads_k.d * p.columns, at = (int64_t)h * p.columns + column;
+  auto slot = [&](int i) { return (i == 0 ? first : next + (i - 1) * step) * rows + at; };
+  float m_run = -FLT_MAX, sum = 0.f, acc[kV] = {};
+  for (int c0 = share; live && c0 < splits; c0 += 64 * kShare) {
+    // 64 splits of this wave's: a lane's own maximum and sum, then their outputs
+    const int n = min((splits - c0 + kShare - 1) / kShare, 64);
+    const float2 own = l < n ? *reinterpret_cast<const float2*>(p.ws_ml + 2 * slot(c0 + l * kShare)) : float2{-FLT_MAX, 0.f};
+    float x[kAtOnce][kV];
+    auto load = [&](int s0) {
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const float* o = p.ws_o + slot(c0 + min(s0 + j, n - 1) * kShare) * D + kV * l;
+#pragma unroll
+        for (int i = 0; i < kV; ++i) x[j][i] = o[i];
+      }
+    };
+    load(0);
+    float m = own.x;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    m = fmaxf(m, m_run);
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m);
+    const float f = __builtin_amdgcn_exp2f(own.x - m);
+    m_run = m;
+    sum = sum * alpha + own.y * f;  // of this lane's splits (0 past the last)
+#pragma unroll
+    for (int i = 0; i < kV; ++i) acc[i] *= alpha;
+    for (int s0 = 0; s0 < n; s0 += kAtOnce) {
+      if (s0) load(s0);
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const float g = s0 + j < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + j)) : 0.f;
+#pragma unroll
+        for (int i = 0; i < kV; ++i) acc[i] += s0 + j < n ? x[j][i] * g : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+  if constexpr (kShare > 1) {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) part[w][kV * l + i] = acc[i];
+    if (l == 0) part[w][D] = m_run, part[w][D + 1] = sum;
+    __syncthreads();
+    if (share != 0) return;
+    float m = -FLT_MAX;
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) m = fmaxf(m, part[w + i][D]);
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kV; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {
+      const float f = __builtin_amdgcn_exp2f(part[w + i][D] - m);
+      sum += part[w + i][D + 1] * f;
+#pragma unroll
+      for (int j = 0; j < kV; ++j) acc[j] += part[w + i][kV * l + j] * f;
+    }
+    m_run = m;
+  }
+  if (!live) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int fresh = (int)p.over_group.div((uint32_t)column), group = (int)p.over_group.d;
+  const int heads = group * (int)p.over_heads_k.d, head = h * group + column - fresh * group;
+  uint16_t* out = p.out + (((int64_t)b * p.new_tokens + fresh) * heads + head) * D;
+  if constexpr (kV == 2)
+    *reinterpret_cast<uint32_t*>(out + 2 * l) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  else
+    out[l] = (uint16_t)pack_bf16x2(acc[0] * inv, 0.f);
+  if (p.lse && l == 0)
+    p.lse[((int64_t)b * heads + head) * p.new_tokens + fresh] =
+        sum == 0.f ? -INFINITY : (m_run + __log2f(sum)) * 0.6931471805599453f;
 }
 
 hipError_t merge_splits(hipStream_t stream, const SplitMerge& p, int head_dim) {
@@ -94,6 +187,33 @@ hipError_t merge_splits(hipStream_t stream, const SplitMerge& p, int head_dim) {
   else
     hipLaunchKernelGGL(merge_kernel<64>, grid, block, 0, stream, p);
   return hipGetLastError();
+}
+
+// Columns of a workgroup: one, where there are so few rows that eight waves for each
+// leave CUs idle (32 rows of 64 splits: 4 us, 6 with two waves for each), else eight.
+static int columns_at_once(int batch, int heads_k, int64_t columns) {
+  return (int64_t)batch * heads_k * columns <= 512 ? 1 : 8;
+}
+
+int64_t merge_parts_groups(int batch, int heads_k, int64_t columns) {
+  const int at_once = columns_at_once(batch, heads_k, columns);
+  return (int64_t)batch * heads_k * ((columns + at_once - 1) / at_once);
+}
+
+hipError_t merge_parts(hipStream_t stream, PartMerge p, int batch, int heads_k, int head_dim) {
+  const int at_once = columns_at_once(batch, heads_k, p.columns);
+  p.over_heads_k = FastDiv::of(heads_k);
+  p.over_pieces = FastDiv::of((p.columns + at_once - 1) / at_once);
+  const dim3 grid((unsigned)merge_parts_groups(batch, heads_k, p.columns)), block(kPartMergeThreads);
+  auto launch = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    if (at_once == 1)
+      hipLaunchKernelGGL((merge_parts_kernel<D, 8>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((merge_parts_kernel<D, 1>), grid, block, 0, stream, p);
+    return hipGetLastError();
+  };
+  return head_dim == 128 ? launch(std::integral_constant<int, 128>{}) : launch(std::integral_constant<int, 64>{});
 }
 
 }  // namespace zs

@@ -11,22 +11,33 @@ namespace zs {
 
 constexpr int kMergeWaves = 4;  // of a row's workgroup
 
-// Row r is new token r % new_tokens of (sequence, head) r / new_tokens: that is also
-// the order of lse; out is [sequence][new token][head][D].
+// Row r is (sequence, head) r, its splits are in the slots r * splits and up.
 struct SplitMerge {
-  const float* ws_o;   // [row][split][D], not divided by the split's sum
-  const float* ws_ml;  // [row][split][2]: maximum (log2 domain) and sum
-  uint16_t* out;
-  float* lse;          // or null
-  int splits, rows, heads;
-  FastDiv new_tokens, over_heads;
-
-  static SplitMerge of(const float* ws_o, const float* ws_ml, uint16_t* out, float* lse, int splits, int rows,
-                       int heads, int new_tokens) {
-    return SplitMerge{ws_o, ws_ml, out, lse, splits, rows, heads, FastDiv::of(new_tokens), FastDiv::of(heads)};
-  }
+  const float* ws_o;   // [slot][D], not divided by the split's sum
+  const float* ws_ml;  // [slot][2]: maximum (log2 domain) and sum
+  uint16_t* out;       // [row][D]
+  float* lse;          // [row], or null
+  int splits, rows;
 };
 
 hipError_t merge_splits(hipStream_t stream, const SplitMerge& p, int head_dim);
+
+// Slots of [heads_k][columns] rows, a column being new token * group + head of the
+// group; out is [sequence][new token][head][D], lse [sequence][head][new token].  A
+// sequence's slots are b * splits and up, or with a plan, (first, number) a sequence,
+// the first and then first / 2 * 2 + 2, + 4, ...; a sequence of one is written already.
+struct PartMerge {
+  const float* ws_o;
+  const float* ws_ml;
+  const int2* plan;  // or null
+  uint16_t* out;
+  float* lse;
+  int splits, columns, new_tokens;
+  FastDiv over_group, over_heads_k, over_pieces;  // (the last two are set by the call)
+};
+
+constexpr int kPartMergeThreads = 512;  // of each of merge_parts_groups() workgroups
+int64_t merge_parts_groups(int batch, int heads_k, int64_t columns);
+hipError_t merge_parts(hipStream_t stream, PartMerge p, int batch, int heads_k, int head_dim);
 
 }  // namespace zs
