@@ -10,8 +10,11 @@
 // of positions is read.  They are made once a token and shared by its heads through
 // LDS.
 //
-// A workgroup takes kTokens tokens; a thread 16 bytes of both members of its pairs
-// (of one, where they are neighbours) at a time.
+// A workgroup takes one token, or up to four while they have no more than 64 angles, one
+// wave's work; a thread 16 bytes of both members of its pairs (of one, where they are
+// neighbours) at a time, written past the caches.  HBM bounds it: 8192 tokens of 40 heads of
+// 128 in bf16 take 26.2 us, 168 MB at 6.4 TB/s, some of it from the last-level cache (28.5
+// in workgroups of 256 threads and four tokens); one token 3.4 us, launch and latency.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -25,7 +28,7 @@ namespace zs {
 
 bool grid_fits(int64_t groups, int threads);  // zs_paged.hip
 
-constexpr int kRotaryThreads = 256;
+constexpr int kRotaryThreads = 512;
 constexpr int kRotaryPairs = 512;  // angles a workgroup holds
 
 struct RotaryTensor {
@@ -76,6 +79,7 @@ template <class T, int E, bool kNeighbours, bool kWide>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryParams p) {
   typedef T Whole __attribute__((ext_vector_type(E)));
   typedef Whole Vec __attribute__((aligned(kWide ? 16 : sizeof(T))));
+  auto store = [](T* at, Whole x) { __builtin_nontemporal_store(x, reinterpret_cast<Vec*>(at)); };
   __shared__ float2 turn[kRotaryPairs];
   const int t0 = blockIdx.x * p.group, n = min(p.group, p.tokens - t0);
   for (int i = threadIdx.x; i < n * p.pairs; i += kRotaryThreads) {
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryParams p) 
     if (c >= p.rotated_items) {  // behind the rotated channels
       const int at = 2 * p.pairs + (c - p.rotated_items) * (kWide ? E : 1);
       if constexpr (kWide)
-        *reinterpret_cast<Vec*>(out + at) = *reinterpret_cast<const Vec*>(in + at);
+        store(out + at, *reinterpret_cast<const Vec*>(in + at));
       else
         out[at] = in[at];
     } else if constexpr (kNeighbours) {
@@ -110,7 +114,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryParams p) 
         y[j] = (T)(u * r.x - v * r.y);
         y[j + 1] = (T)(v * r.x + u * r.y);
       }
-      *reinterpret_cast<Vec*>(out + c * E) = placed ? y : a;
+      store(out + c * E, placed ? y : a);
     } else {
       const Vec a = *reinterpret_cast<const Vec*>(in + c * E);
       const Vec b = *reinterpret_cast<const Vec*>(in + p.pairs + c * E);
@@ -122,8 +126,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryParams p) 
         y[j] = (T)(u * r.x - v * r.y);
         z[j] = (T)(v * r.x + u * r.y);
       }
-      *reinterpret_cast<Vec*>(out + c * E) = placed ? y : a;
-      *reinterpret_cast<Vec*>(out + p.pairs + c * E) = placed ? z : b;
+      store(out + c * E, placed ? y : a);
+      store(out + p.pairs + c * E, placed ? z : b);
     }
   }
 }
@@ -180,7 +184,7 @@ extern "C" int zs_rotary(void* stream, const void* q, int64_t q_token_stride, in
   const int64_t per_token = (int64_t)p.items * (num_heads + (int64_t)num_heads_k);
   if (per_token > INT_MAX / 8) return ZS_E_OVERFLOW;
   p.per_token = (int)per_token;
-  p.group = std::max(1, std::min(4, kRotaryPairs / num_pairs));
+  p.group = std::max(1, std::min(4, 64 / num_pairs));
   p.over_items = FastDiv::of(p.items);
   p.over_token = FastDiv::of(p.per_token);
   p.over_pairs = FastDiv::of(num_pairs);
