@@ -133,7 +133,7 @@ def _bytes(query, *sizes):
     return int(getattr(lib(), query)(*sizes))
 
 
-@dataclass(frozen=True)
+@dataclass(slots=True)
 class QuantizedKVCache:
     """A pool of pages held in 4 or 8 bits, as `quantized_kv_cache` makes it: for
     every (page, KV head) page_block_size times 8 bytes with a token's (scale,
@@ -305,18 +305,24 @@ def quantized_kv_cache(num_blocks: int, page_block_size: int, num_heads_k: int, 
     return QuantizedKVCache(data, page_block_size, head_dim, bits)
 
 
-def _quantized(cache, name="cache"):
+def _quantized(cache):
     """A QuantizedKVCache's numbers as the library takes them: address, num_blocks,
     page, Hkv, head_dim, bits."""
-    if not isinstance(cache, QuantizedKVCache):
-        raise ValueError(f"{name} must be a QuantizedKVCache")
-    page, dim, bits = cache.page_block_size, cache.head_dim, cache.bits
-    if not (isinstance(page, int) and 0 < page <= _MOST and isinstance(dim, int) and 0 < dim <= _MOST
-            and bits in (4, 8)):
-        raise ValueError(f"{name}: page_block_size, head_dim or bits is wrong")
-    _check(cache.data, f"{name}.data", _torch().uint8, (None, None, page * (8 + dim * bits // 4)))
-    blocks, heads_k, _ = cache.data.shape
-    return cache.data.data_ptr(), blocks, page, heads_k, dim, bits
+    if type(cache) is not QuantizedKVCache:
+        raise ValueError("cache must be a QuantizedKVCache")
+    data, page, dim, bits = cache.data, cache.page_block_size, cache.head_dim, cache.bits
+    try:  # (a right one takes 1 us)
+        blocks, heads_k, record = data.shape
+        if data.is_cuda and data.is_contiguous() and data.dtype is _torch().uint8 and \
+                record == page * (8 + dim * bits // 4) and 0 < record <= _MOST and blocks <= _MOST and \
+                heads_k <= _MOST and (bits == 4 or bits == 8):
+            return data.data_ptr(), blocks, page, heads_k, dim, bits
+    except (AttributeError, TypeError, ValueError):
+        pass
+    if not (isinstance(page, int) and isinstance(dim, int) and page > 0 and dim > 0 and bits in (4, 8)):
+        raise ValueError("cache: page_block_size, head_dim or bits is wrong")
+    _check(data, "cache.data", _torch().uint8, (None, None, page * (8 + dim * bits // 4)))
+    raise ValueError(f"cache: pages of {page} tokens of {dim} channels are too large")
 
 
 def append_paged_kv_quantized(k, v, cache: QuantizedKVCache, slots) -> None:
@@ -361,7 +367,8 @@ def read_paged_kv_quantized(cache: QuantizedKVCache, slots):
     device, stream = here
     _check(slots, "slots", torch.int32, (None,), device)
     n = slots.shape[0]
-    k, v = torch.empty((2, n, heads_k, dim), dtype=torch.bfloat16, device=slots.device).unbind(0)
+    k = torch.empty((n, heads_k, dim), dtype=torch.bfloat16, device=slots.device)
+    v = torch.empty_like(k)
     check("zs_paged_read_quant", lib().zs_paged_read_quant(
         stream, data, blocks, page, heads_k, dim, bits, slots.data_ptr(), n, k.data_ptr(), v.data_ptr()))
     return k, v

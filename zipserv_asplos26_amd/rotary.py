@@ -70,21 +70,42 @@ def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: str = "none
     return w.to(device), factor
 
 
-def _strides(t):
-    """Token and head stride of (tokens, heads, dim) in elements, None where a head's
-    channels do not stand next to one another."""
-    s0, s1, s2 = t.stride()
-    return (s0, s1) if s2 == 1 or t.shape[2] == 1 else None
-
-
 def _apart(t):
-    """Whether no two entries of (tokens, heads, dim) share a place."""
+    """Whether no two entries of t share a place."""
     reach = 0
     for step, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if step <= reach:
             return False
         reach += step * (size - 1)
     return True
+
+
+_ONE, _THREE, _FOUR = (None,), (None, None, None), (None, None, None, None)
+_ABSENT = (0, 0, 0, 0, 0, 0, 0)
+
+
+def _side(name, x, tokens, dim, inplace, torch):
+    """The output of x, what is read for it, and both as the library takes them:
+    address, token and head stride of each, heads."""
+    shape, step = x.shape, x.stride()
+    heads = shape[-2]
+    rows = x
+    if len(shape) == 4:
+        if shape[0] > 1 and shape[1] > 1 and step[0] != shape[1] * step[1]:
+            rows = None  # tokens that do not follow one stride
+        else:
+            step = step[1 if shape[1] > 1 else 0:][:1] + step[2:]
+    if rows is None or (step[2] != 1 and dim > 1):
+        if inplace:
+            raise ValueError(f"{name} is turned in place: its tokens must follow one stride, its heads be contiguous")
+        rows, step = x.contiguous(), (heads * dim, dim, 1)
+    at = rows.data_ptr()
+    if inplace:
+        if not _apart(x):
+            raise ValueError(f"{name} is turned in place: its heads must be apart")
+        return x, rows, (at, step[0], step[1], at, step[0], step[1], heads)
+    out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    return out, rows, (at, step[0], step[1], out.data_ptr(), heads * dim, dim, heads)
 
 
 def apply_rotary(q, k, positions, frequencies, factor: float = 1.0, interleaved: bool = False,
@@ -100,51 +121,37 @@ def apply_rotary(q, k, positions, frequencies, factor: float = 1.0, interleaved:
     and k are turned where they are (and returned), else into new contiguous
     tensors.  frequencies negated turn back what factor 1 has turned."""
     torch = _torch()
-    types = {torch.bfloat16: ZS_TYPE_BF16, torch.float16: ZS_TYPE_FP16, torch.float32: ZS_TYPE_FP32}
-    if not (isinstance(q, torch.Tensor) and q.dtype in types):
+    if not isinstance(q, torch.Tensor):
         raise ValueError("q must be a bfloat16, float16 or float32 CUDA tensor")
-    form = (None,) * (4 if q.dim() == 4 else 3)
-    _check(q, "q", q.dtype, form, contiguous=False)
+    dtype = q.dtype
+    type_ = ZS_TYPE_BF16 if dtype is torch.bfloat16 else ZS_TYPE_FP16 if dtype is torch.float16 else \
+        ZS_TYPE_FP32 if dtype is torch.float32 else -1
+    shape = q.shape
+    four = len(shape) == 4
+    if type_ < 0:
+        raise ValueError("q must be a bfloat16, float16 or float32 CUDA tensor")
+    _check(q, "q", dtype, _FOUR if four else _THREE, None, False)
     here = _here(q)
     if here is None:
         with torch.cuda.device(q.device):
             return apply_rotary(q, k, positions, frequencies, factor, interleaved, inplace)
     device, stream = here
-    dim, lead = q.shape[-1], q.shape[:-2]
+    if four:
+        lead, dim, tokens = (shape[0], shape[1]), shape[3], shape[0] * shape[1]
+    else:
+        lead, dim, tokens = (shape[0],), shape[2], shape[0]
     if k is not None:
-        _check(k, "k", q.dtype, (*lead, None, dim), device, contiguous=False)
-    _check(positions, "positions", torch.int32, (*lead,), device)
-    _check(frequencies, "frequencies", torch.float64, (None,), device)
+        _check(k, "k", dtype, (*lead, None, dim), device, False)
+    _check(positions, "positions", torch.int32, lead, device)
+    _check(frequencies, "frequencies", torch.float64, _ONE, device)
     pairs = frequencies.shape[0]
     if pairs == 0 or 2 * pairs > dim:
         raise ValueError(f"{pairs} frequencies do not fit heads of {dim} channels")
-    tokens = positions.numel()
     if tokens > _MOST:
         raise ValueError("there must be less than 2^31 tokens")
-
-    sides, out = [], []
-    for name, x in (("q", q), ("k", k)):
-        if x is None:
-            sides += [0, 0, 0, 0, 0, 0, 0]
-            out.append(None)
-            continue
-        if inplace:
-            try:
-                x3 = x.view(tokens, x.shape[-2], dim)
-            except RuntimeError:
-                x3 = None
-            if x3 is None or _strides(x3) is None or not _apart(x3):
-                raise ValueError(f"{name} is turned in place: its tokens must follow one stride, its heads be contiguous "
-                                 "and apart")
-            y, y3 = x, x3
-        else:
-            x3 = x.reshape(tokens, x.shape[-2], dim)
-            if _strides(x3) is None:
-                x3 = x3.contiguous()
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            y3 = y.view(x3.shape)
-        sides += [x3.data_ptr(), *_strides(x3), y3.data_ptr(), *_strides(y3), x3.shape[1]]
-        out.append((y, x3))  # (x3 is held until the launch is queued)
-    check("zs_rotary", lib().zs_rotary(stream, *sides, types[q.dtype], positions.data_ptr(), tokens, dim,
-                                       frequencies.data_ptr(), pairs, float(factor), int(bool(interleaved))))
-    return tuple(None if o is None else o[0] for o in out)
+    q_out, q_in, q_args = _side("q", q, tokens, dim, inplace, torch)
+    k_out, k_in, k_args = (None, None, _ABSENT) if k is None else _side("k", k, tokens, dim, inplace, torch)
+    # (q_in and k_in are held until the launch is queued)
+    check("zs_rotary", lib().zs_rotary(stream, *q_args, *k_args, type_, positions.data_ptr(), tokens, dim,
+                                       frequencies.data_ptr(), pairs, factor, bool(interleaved)))
+    return q_out, k_out
