@@ -130,7 +130,10 @@ def attend(q, data, table, lens, page, bits, scale=None):
     |q| (s_k (32 + c) + |low_k|) at most, which move a weight by twice that relatively at
     most, the normaliser included; sums of T weights and of T products of s_v (32 + c) +
     |low_v| in fp32 with their rescalings, the weights' scaling, a merge of the splits and
-    the exponentials (3 T 2^-24 in all, T counted from 64)."""
+    the exponentials (3 T 2^-24 in all, T counted from 64).  A weight times s_v enters its
+    product as two fp16: off by 2^-22 of it, which these cover, or by 2^-25 where the
+    largest of them, s_v counting as 2^-30 at least, is 2^11 or more: T 2^bits 2^-36 2^-30
+    besides what these cover."""
     B, new, H, D = q.shape
     blocks, heads_k = data.shape[:2]
     group = H // heads_k
@@ -163,7 +166,7 @@ def attend(q, data, table, lens, page, bits, scale=None):
                 ds = (x.abs() @ k_size.t()).amax(1, keepdim=True) * abs(scale) * (D + 8) * 2.0 ** -24
                 many = 3 * max(len(block), 64) * 2.0 ** -24
                 out[b, i, rows], lse[b, rows, i] = o, torch.logsumexp(s, 1)
-                tol[b, i, rows] = 2.0 ** -8 * o.abs() + (w @ v_size) * (2 * ds + many) + 1e-30
+                tol[b, i, rows] = 2.0 ** -8 * o.abs() + (w @ v_size) * (2 * ds + many) + len(block) * 2.0 ** (bits - 66)
                 lse_tol[b, rows, i] = ds[:, 0] + many + 2.0 ** -22 * lse[b, rows, i].abs()
     return out, lse, tol, lse_tol
 

@@ -213,6 +213,31 @@ def test_scores_far_apart(torch_cuda, bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("which", ["apart", "small", "large", "flat", "zero", "mixed"])
+def test_values_of_all_sizes(torch_cuda, which, bits):
+    # value rows whose scales are far apart, all small, all large, or 0 (rows of one value)
+    T = torch_cuda
+    lens, page, width = [700, 333, 64], 16, 44
+    q, data, table = make(T, 17, 3, 1, 8, 2, 64, page, width, bits)
+    side = data[..., :8 * page].view(np.uint16).reshape(len(data), 2, page, 4)
+    g = T.Generator().manual_seed(18)
+    power = T.randint(-20, 20, side.shape[:3], generator=g).float() if which == "apart" else \
+        T.full(side.shape[:3], {"small": -29.0, "large": 100.0}.get(which, 0.0))
+    if which == "mixed":  # nearly nothing, then a few that are 2^150 times as large
+        power = T.full(side.shape[:3], -60.0)
+        power[int(table[0, 30])] = power[int(table[1, 2])] = 90.0
+    scale = T.randn(side.shape[:3], generator=g).exp() * 2.0 ** power
+    low = -scale * 2 ** (bits - 1)
+    if which in ("flat", "zero"):
+        flat = T.rand(side.shape[:3], generator=g) < (0.5 if which == "flat" else 2.0)
+        scale[flat] = 0.0
+    side[..., 2], side[..., 3] = ref.bf16_bits(scale.to(T.bfloat16)), ref.bf16_bits(low.to(T.bfloat16))
+    want = ref.attend(q, data, table, lens, page, bits)
+    for splits in (1, 0, 5):
+        check(T, q, data, table, lens, page, bits, want=want, num_splits=splits)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 def test_pages_that_are_not_in_the_pool(torch_cuda, bits):
     T = torch_cuda
     lens, page, width = [150, 96, 40, 70], 16, 10

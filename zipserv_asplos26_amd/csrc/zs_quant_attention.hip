@@ -13,25 +13,27 @@
 // tiles of 16) at a time, all in registers, with the next pair's loads on the way:
 //   S^T = C_k q^T with v_mfma_f32_16x16x32_f16: lane l holds D / 4 codes of token
 //   l%16 (channels D/4 * (l/16) and up, one piece of its row), 8 of them the A operand of a
-//   step; q^T (lane l: column l%16, the same channels) is the B operand.  A code's bits
-//   are an fp16 subnormal, code 2^-24, which costs an "and" for two codes and a shift for four.
+//   step; q^T (lane l: column l%16, the same channels) is the B operand.
 //   Online softmax in the log2 domain, fp32.
-//   O^T += C_v^T W^T over K = 32 tokens with v_mfma_f32_16x16x32_bf16: S^T leaves lane l
-//   the weights of column l%16 for tokens 4*(l/16)..+3 of both tiles, the B operand if
-//   k index 8*(l/16) + j stands for token 4*(l/16) + j%4 of tile j/4; lane l reads the
+//   O^T += C_v^T W^T over K = 32 tokens with the same instruction: S^T leaves lane l the
+//   weights of column l%16 for tokens 4*(l/16)..+3 of both tiles, the B operand if k
+//   index 8*(l/16) + j stands for token 4*(l/16) + j%4 of tile j/4; lane l reads the
 //   l%16-th part of those eight rows, D / 16 channels of 8 tokens, which are D / 16 A
-//   operands.  A weight times s_v goes in as three bf16, all of its 24 bits (two, 18 bits: 4.3
-//   us less of 67 where 40 columns share a KV head, nothing in the other cases).  In 4 bits a
-//   shift and an and-or put two codes into the mantissas of two bf16 of exponent 4, 16 +
-//   c: the 16s are taken off through the sum of p (low_v - 16 s_v).
+//   operands.
+// A code's bits are an fp16 subnormal, code 2^-24, which the matrix cores take as it is: an
+// "and" for two codes and a shift for four (8 bits of values: a byte permute for two).
+// What meets them has to be fp16 as well: q, times a power of two a column, and the weights
+// times s_v as two fp16 each, 22 bits, relative to the largest of them so far.  As
+// bf16, 16 + code by a shift and an and-or, with weights of three parts, values took
+// 231 and 290 vector instructions a pair where it is 199 and 251 (8 and 16 columns).
 // With 8 columns or fewer the tile's other columns repeat them, and a lane does the softmax
 // of only a half of its tokens (4 or fewer: a quarter) and gets the other weights from
-// the lanes that did them: 231 vector instructions a pair for 8 columns, 290 for 16.
+// the lanes that did them.
 //
 // What bounds it: 64 sequences' 8000 tokens (64 / 8 heads of 128 in 4 bits, 557 MB) take 106
 // us, 5.3 TB/s, where a kernel that only reads them takes 98; with 16 columns and more
-// the vector instructions do (three tiles of columns over 113 MB: 67 us, reading
-// alone 37); one sequence's 32000 tokens 13.5 us and 4 for the merge, start, loads and
+// the vector instructions do (three tiles of columns over 113 MB: 64 us, reading
+// alone 37); one sequence's 32000 tokens 13 us and 4 for the merge, start, loads and
 // merge being a chain of latencies.
 #include <hip/hip_runtime.h>
 
@@ -74,8 +76,10 @@ struct QuantAttnParams {
 };
 
 constexpr int kQaWaves = 4;
-constexpr int kParts = 3;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// 2^-30: scales below count as this in what weights are relative to, or their sums could leave fp32.
+constexpr uint32_t kLeastScale = (127 - 30) << 23;
 
 template <int D, int kBits>
 struct QaShape {
@@ -93,25 +97,6 @@ __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* w) {
   const Vec x = *reinterpret_cast<const Vec*>(at);
 #pragma unroll
   for (int i = 0; i < N; ++i) w[i] = x[i];
-}
-
-// Nibble i of both halves of w as two bf16 of 16 + code.  (The constants come out
-// of registers: with literals the and-or is two instructions.)
-struct NibbleBits {
-  uint32_t mask = 0x00780078u, sixteen = 0x41804180u;
-  __device__ __forceinline__ NibbleBits() { asm("" : "+s"(mask), "+v"(sixteen)); }
-};
-template <int i>
-__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w, const NibbleBits& c) {
-  const uint32_t x = 4 * i < 3 ? w << (3 - 4 * i) : w >> (4 * i - 3);
-  return (x & c.mask) | c.sixteen;
-}
-
-// Bytes i of a and b as two bf16.
-template <int i>
-__device__ __forceinline__ uint32_t bytes_bf16(uint32_t a, uint32_t b) {
-  const uint32_t x = __float_as_uint((float)(a >> 8 * i & 255u)), y = __float_as_uint((float)(b >> 8 * i & 255u));
-  return __builtin_amdgcn_perm(y, x, 0x07060302);
 }
 
 // Step c's operand from a lane's piece of a key row: codes as fp16 subnormals, which
@@ -147,10 +132,17 @@ __device__ __forceinline__ f16x8 query_operand(u32x4 in, float factor) {
   return y;
 }
 
-// A lane's parts of eight value rows, and the operand of output tile n from them:
-// its channel n (the map from (part, n) to a channel is qa_channel).
+// A lane's parts of eight value rows, and the operand of output tile n from them, its
+// channel n of the eight tokens (the map from (part, n) to a channel is qa_channel), as
+// fp16 subnormals again, 16 times as large where sixteenfold(n).
 template <int D, int kBits>
 struct ValuePart;
+
+template <int i>
+__device__ __forceinline__ uint32_t nibbles_f16(uint32_t w) {
+  const uint32_t x = i >= 2 ? w >> 8 : w;
+  return x & (i % 2 ? 0x00F000F0u : 0x000F000Fu);
+}
 
 template <>
 struct ValuePart<128, 4> {
@@ -158,13 +150,14 @@ struct ValuePart<128, 4> {
   __device__ __forceinline__ void load(int j, const uint8_t* part) {
     w[j] = *reinterpret_cast<const uint32_t*>(part);
   }
+  static constexpr bool sixteenfold(int n) { return n / 2 % 2; }
   template <int n>
-  __device__ __forceinline__ bf16x8 operand(const NibbleBits& nb) const {
+  __device__ __forceinline__ f16x8 operand() const {
     u32x4 x;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      x[i] = nibbles_bf16<n / 2>(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], n % 2 ? 0x07060302 : 0x05040100), nb);
-    return as_bf16x8(x);
+      x[i] = nibbles_f16<n / 2>(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], n % 2 ? 0x07060302 : 0x05040100));
+    return __builtin_bit_cast(f16x8, x);
   }
 };
 
@@ -174,12 +167,13 @@ struct ValuePart<64, 4> {
   __device__ __forceinline__ void load(int j, const uint8_t* part) {
     w[j] = *reinterpret_cast<const uint16_t*>(part);
   }
+  static constexpr bool sixteenfold(int n) { return n % 2; }
   template <int n>
-  __device__ __forceinline__ bf16x8 operand(const NibbleBits& nb) const {
+  __device__ __forceinline__ f16x8 operand() const {
     u32x4 x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = nibbles_bf16<n>((uint32_t)w[2 * i] | (uint32_t)w[2 * i + 1] << 16, nb);
-    return as_bf16x8(x);
+    for (int i = 0; i < 4; ++i) x[i] = nibbles_f16<n>((uint32_t)w[2 * i] | (uint32_t)w[2 * i + 1] << 16);
+    return __builtin_bit_cast(f16x8, x);
   }
 };
 
@@ -188,12 +182,14 @@ struct ValuePart<D, 8> {
   static constexpr int kW = D / 64;
   uint32_t w[8][kW];
   __device__ __forceinline__ void load(int j, const uint8_t* part) { load_words<kW>(part, w[j]); }
+  static constexpr bool sixteenfold(int) { return false; }
   template <int n>
-  __device__ __forceinline__ bf16x8 operand(const NibbleBits& nb) const {
-    u32x4 x;
+  __device__ __forceinline__ f16x8 operand() const {
+    u32x4 x;  // byte n % 4 of both tokens, zeros above
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = bytes_bf16<n % 4>(w[2 * i][n / 4], w[2 * i + 1][n / 4]);
-    return as_bf16x8(x);
+    for (int i = 0; i < 4; ++i)
+      x[i] = __builtin_amdgcn_perm(w[2 * i + 1][n / 4], w[2 * i][n / 4], 0x0C040C00u + 0x00010001u * (n % 4));
+    return __builtin_bit_cast(f16x8, x);
   }
 };
 
@@ -256,7 +252,8 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
 #pragma unroll
   for (int i = 0; i < kO; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) cb[(4 * i + r) * 64] = O[i][r] + z;
+    for (int r = 0; r < 4; ++r)
+      cb[(4 * i + r) * 64] = fmaf(O[i][r], ValuePart<D, kBits>::sixteenfold(i) ? 0x1p20f : 0x1p24f, z);
   cb[4 * kO * 64] = m_own;
   cb[(4 * kO + 1) * 64] = l_own;
   __syncthreads();
@@ -267,12 +264,12 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
   for (int i = 0; i < W; ++i) m = fmaxf(m, src[i * Shape::kState + 4 * kO * 64]);
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    const float f = __builtin_amdgcn_exp2f(src[i * Shape::kState + 4 * kO * 64] - m);
-    sum += src[i * Shape::kState + (4 * kO + 1) * 64] * f;
+    const float f = __builtin_amdgcn_exp2f(0.5f * (src[i * Shape::kState + 4 * kO * 64] - m));  // (in two steps, as there)
+    sum += src[i * Shape::kState + (4 * kO + 1) * 64] * f * f;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[n][r] += src[i * Shape::kState + (4 * (2 * w + n) + r) * 64] * f;
+      for (int r = 0; r < 4; ++r) o[n][r] += src[i * Shape::kState + (4 * (2 * w + n) + r) * 64] * f * f;
   }
   const int column = kColumns * ct + (l & 15);
   if ((l & 15) >= kColumns || column >= p.columns) return;
@@ -484,15 +481,13 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
 #pragma unroll
     for (int c = 0; c < kC; ++c) Q[c] = query_operand<kBits>(x[c], p.flip * up);
     qs = wave_sum16(sum) * (p.flip * up * 0x1p-24f);
-    unit = fmaxf(p.scale_log2 * __uint_as_float((uint32_t)(127 + 10 + e) << 23), FLT_MIN);  // (0 times -inf is none)
+    unit = p.scale_log2 * __uint_as_float((uint32_t)(127 + 10 + e) << 23);
   }
 
   f32x4 O[kO];
 #pragma unroll
   for (int k = 0; k < kO; ++k) O[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -FLT_MAX, l_run = 0.f, z = 0.f;  // z: sum p low_v, the 16s taken off
-  const NibbleBits nb;
-
+  float m_run = -FLT_MAX, l_run = 0.f, z = 0.f;  // z: sum p low_v
   auto consume = [&](const Pair& x) {
     f32x4 S[2] = {};
 #pragma unroll
@@ -501,7 +496,7 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
       S[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K0, Q[c], S[0], 0, 0, 0);
       S[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K1, Q[c], S[1], 0, 0, 0);
     }
-    float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens];
+    float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kTokens];
 #pragma unroll
     for (int j = 0; j < kTokens; ++j) {
       const uint32_t kp = x.side[2 * j], vp = x.side[2 * j + 1];
@@ -509,90 +504,86 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
       kl[j] = __uint_as_float(kp & 0xFFFF0000u);
       vs[j] = __uint_as_float(vp << 16);
       vl[j] = __uint_as_float(vp & 0xFFFF0000u);
-      if constexpr (kBits == 4) vl[j] = fmaf(vs[j], -16.f, vl[j]);
+      vs_log[j] = (float)max(vp << 16, kLeastScale);  // * 2^-23: log2 of the scale + 127, up to 0.09 less
     }
     // Behind a column's limit and where there is no page nothing counts, whatever it holds.
     const bool cut = x.none[0] || x.none[1] || first - 16 * x.tile < 32;  // (uniform)
     constexpr int kWords = kTokens / 2;                                   // packed pairs of a lane's weights
-    u32x4 weights[kParts];
-    {
-      float s[kTokens], vs_i[kTokens], vl_i[kTokens];
+    float s[kTokens];
+#pragma unroll
+    for (int j = 0; j < kTokens; ++j) {
+      float c;
+      if constexpr (kFold == 1)
+        c = S[j / 4][j % 4];
+      else if constexpr (kFold == 2)
+        c = fold ? S[1][j] : S[0][j];
+      else
+        c = fold & 2 ? (fold & 1 ? S[1][2 + j] : S[1][j]) : (fold & 1 ? S[0][2 + j] : S[0][j]);
+      s[j] = fmaf(ks[j], c, kl[j] * qs) * unit;
+    }
+    if (cut) {
 #pragma unroll
       for (int j = 0; j < kTokens; ++j) {
-        float c;
-        if constexpr (kFold == 1)
-          c = S[j / 4][j % 4];
-        else if constexpr (kFold == 2)
-          c = fold ? S[1][j] : S[0][j];
-        else
-          c = fold & 2 ? (fold & 1 ? S[1][2 + j] : S[1][j]) : (fold & 1 ? S[0][2 + j] : S[0][j]);
-        s[j] = fmaf(ks[j], c, kl[j] * qs);
-        vs_i[j] = vs[j];
-        vl_i[j] = vl[j];
+        const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
+        const bool seen = at < limit - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
+        s[j] = seen ? s[j] : -INFINITY;
+        vs[j] = seen ? vs[j] : 0.f;
+        vl[j] = seen ? vl[j] : 0.f;
       }
-      if (cut) {
+    }
+    // What a weight is relative to: so that the largest product of a weight and a value's
+    // scale is 2^11..2^15.  Moved only where a product would be larger.
+    float mx = fmaf(vs_log[0], 0x1p-23f, s[0]);
 #pragma unroll
-        for (int j = 0; j < kTokens; ++j) {
-          const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
-          const bool seen = at < limit - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
-          s[j] = seen ? s[j] : -INFINITY;
-          vs_i[j] = seen ? vs[j] : 0.f;
-          vl_i[j] = seen ? vl[j] : 0.f;
-        }
+    for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, fmaf(vs_log[j], 0x1p-23f, s[j]));
+    mx -= 127.f + 11.f;
+    if (__builtin_amdgcn_ballot_w64(mx > m_run + 4.f)) {
+      if constexpr (kFold >= 2) mx = fmaxf(mx, row_from8(mx));
+      if constexpr (kFold == 4) mx = fmaxf(mx, row_from4(mx));
+      const float m_new = fmaxf(m_run, wave_max16(mx));
+      // (in two steps: scales can be 2^160 apart, and sums of small ones' weights as large)
+      const float alpha = __builtin_amdgcn_exp2f(0.5f * (m_run - m_new));
+      m_run = m_new;
+      l_run = l_run * alpha * alpha;
+      z = z * alpha * alpha;
+#pragma unroll
+      for (int k = 0; k < kO; ++k) O[k] = O[k] * alpha * alpha;
+    }
+    // weights times scales as sums of two fp16: 22 bits, or 2^-25 where that is more
+    uint32_t own[2][kWords];
+#pragma unroll
+    for (int j = 0; j < kTokens; j += 2) {
+      float y[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float weight = __builtin_amdgcn_exp2f(s[j + e] - m_run);
+        l_run += weight;
+        z = fmaf(weight, vl[j + e], z);
+        y[e] = weight * vs[j + e];
       }
-      // The maximum is moved only where a score is 8 above it, that is a weight 2^8 where
-      // 1 was the most: sums lose nothing by that.
-      float mx = s[0];
+      const f16x2 a = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
+      const f16x2 c = __builtin_convertvector((f32x2{fmaf((float)a[0], -1.f, y[0]), fmaf((float)a[1], -1.f, y[1])}), f16x2);
+      own[0][j / 2] = __builtin_bit_cast(uint32_t, a);
+      own[1][j / 2] = __builtin_bit_cast(uint32_t, c);
+    }
+    // the other folds' tokens of the column
+    f16x8 weights[2];
 #pragma unroll
-      for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, s[j]);
-      if (__builtin_amdgcn_ballot_w64(mx * unit > m_run + 8.f)) {
-        if constexpr (kFold >= 2) mx = fmaxf(mx, row_from8(mx));
-        if constexpr (kFold == 4) mx = fmaxf(mx, row_from4(mx));
-        const float m_new = fmaxf(m_run, wave_max16(mx) * unit);
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-        m_run = m_new;
-        l_run *= alpha;
-        z *= alpha;
-#pragma unroll
-        for (int k = 0; k < kO; ++k) O[k] *= alpha;
-      }
-      // weights times scales as sums of three bf16, all of their 24 bits
-      uint32_t own[kParts][kWords];
-#pragma unroll
-      for (int j = 0; j < kTokens; j += 2) {
-        float r[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float weight = __builtin_amdgcn_exp2f(fmaf(s[j + e], unit, -m_run));
-          l_run += weight;
-          z = fmaf(weight, vl_i[j + e], z);
-          r[e] = weight * vs_i[j + e];
-        }
-#pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-          const uint32_t a = pack_bf16x2(r[0], r[1]);
-          own[k][j / 2] = a;
-          r[0] -= __uint_as_float(a << 16);
-          r[1] -= __uint_as_float(a & 0xFFFF0000u);
-        }
-      }
-      // the other folds' tokens of the column
-#pragma unroll
-      for (int k = 0; k < kParts; ++k) {
-        if constexpr (kFold == 1)
-          weights[k] = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
-        else if constexpr (kFold == 2)
-          weights[k] = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
-        else
-          weights[k] = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
-      }
+    for (int k = 0; k < 2; ++k) {
+      u32x4 y;
+      if constexpr (kFold == 1)
+        y = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
+      else if constexpr (kFold == 2)
+        y = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
+      else
+        y = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
+      weights[k] = __builtin_bit_cast(f16x8, y);
     }
     unrolled<0, kO>([&](auto n) {
       constexpr int o = decltype(n)::value;
-      const bf16x8 A = x.v.template operand<o>(nb);
+      const f16x8 A = x.v.template operand<o>();
 #pragma unroll
-      for (int k = 0; k < kParts; ++k)
-        O[o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, as_bf16x8(weights[k]), O[o], 0, 0, 0);
+      for (int k = 0; k < 2; ++k) O[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, weights[k], O[o], 0, 0, 0);
     });
   };
 

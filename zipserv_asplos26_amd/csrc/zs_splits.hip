@@ -127,19 +127,20 @@ __global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge 
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
     m = fmaxf(m, m_run);
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m);
-    const float f = __builtin_amdgcn_exp2f(own.x - m);
+    // (weights in two steps: they can be as far apart as 2^-160, of sums as large)
+    const float alpha = __builtin_amdgcn_exp2f(0.5f * (m_run - m));
+    const float f = __builtin_amdgcn_exp2f(0.5f * (own.x - m));
     m_run = m;
-    sum = sum * alpha + own.y * f;  // of this lane's splits (0 past the last)
+    sum = sum * alpha * alpha + own.y * f * f;  // of this lane's splits (0 past the last)
 #pragma unroll
-    for (int i = 0; i < kV; ++i) acc[i] *= alpha;
+    for (int i = 0; i < kV; ++i) acc[i] = acc[i] * alpha * alpha;
     for (int s0 = 0; s0 < n; s0 += kAtOnce) {
       if (s0) load(s0);
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j) {
         const float g = s0 + j < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + j)) : 0.f;
 #pragma unroll
-        for (int i = 0; i < kV; ++i) acc[i] += s0 + j < n ? x[j][i] * g : 0.f;
+        for (int i = 0; i < kV; ++i) acc[i] += s0 + j < n ? x[j][i] * g * g : 0.f;
       }
     }
   }
@@ -159,10 +160,10 @@ __global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge 
     for (int i = 0; i < kV; ++i) acc[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {
-      const float f = __builtin_amdgcn_exp2f(part[w + i][D] - m);
-      sum += part[w + i][D + 1] * f;
+      const float f = __builtin_amdgcn_exp2f(0.5f * (part[w + i][D] - m));
+      sum += part[w + i][D + 1] * f * f;
 #pragma unroll
-      for (int j = 0; j < kV; ++j) acc[j] += part[w + i][kV * l + j] * f;
+      for (int j = 0; j < kV; ++j) acc[j] += part[w + i][kV * l + j] * f * f;
     }
     m_run = m;
   }
