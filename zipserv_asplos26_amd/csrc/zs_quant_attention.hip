@@ -20,12 +20,12 @@
 //   index 8*(l/16) + j stands for token 4*(l/16) + j%4 of tile j/4; lane l reads the
 //   l%16-th part of those eight rows, D / 16 channels of 8 tokens, which are D / 16 A
 //   operands.
-// A code's bits are an fp16 subnormal, code 2^-24, which the matrix cores take as it is: an
-// "and" for two codes and a shift for four (8 bits of values: a byte permute for two).
+// A code's bits are an fp16 subnormal, which the matrix cores take as it is: an "and"
+// for two codes and a shift for four (8 bits of values: a byte permute for two).
 // What meets them has to be fp16 as well: q, times a power of two a column, and the weights
 // times s_v as two fp16 each, 22 bits, relative to the largest of them so far.  As
-// bf16, 16 + code by a shift and an and-or, with weights of three parts, values took
-// 231 and 290 vector instructions a pair where it is 199 and 251 (8 and 16 columns).
+// bf16, 16 + code by a shift and an and-or, with weights of three parts, a pair took
+// 231 and 290 vector instructions where it takes 207 and 260 (8 and 16 columns).
 // With 8 columns or fewer the tile's other columns repeat them, and a lane does the softmax
 // of only a half of its tokens (4 or fewer: a quarter) and gets the other weights from
 // the lanes that did them.
@@ -99,15 +99,27 @@ __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* w) {
   for (int i = 0; i < N; ++i) w[i] = x[i];
 }
 
-// Step c's operand from a lane's piece of a key row: codes as fp16 subnormals, which
-// the matrix cores take as they are, code * 2^-24.  In 4 bits the second nibble of
-// each byte stays where it is, 16 times as large, and q is 1/16 there.
+// Codes as fp16 subnormals, whose bits are a multiple of 2^-24.  In 4 bits nibbles 0 and
+// 2 of a dword's halves come to bits 2..5 and nibbles 1 and 3 to bits 6..9, 4 and 64 times
+// the code; two shifts for four of them.  (The matrix cores line sums up by the
+// exponent that an operand could have, and a small subnormal's leading zeros are digits
+// lost: at bits 0..3 and 4..7, with one shift, scores are 2^-22 off, at these 2^-24.)
+template <int kBits>
+constexpr float kCodeUnit = kBits == 4 ? 0x1p-22f : 0x1p-24f;
+
+template <int i>
+__device__ __forceinline__ uint32_t nibbles_f16(uint32_t w) {
+  const uint32_t x = i >= 2 ? w >> 6 : w << 2;
+  return x & (i % 2 ? 0x03C003C0u : 0x003C003Cu);
+}
+
+// Step c's operand from a lane's piece of a key row.  Nibbles 1 and 3 are 16 times as
+// large, and q is 1/16 there.
 template <int kBits>
 __device__ __forceinline__ f16x8 key_operand(const uint32_t* w, int c) {
   u32x4 x;
   if constexpr (kBits == 4) {
-    const uint32_t y = w[c] >> 8;
-    x = u32x4{w[c] & 0x000F000Fu, w[c] & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u};
+    x = u32x4{nibbles_f16<0>(w[c]), nibbles_f16<1>(w[c]), nibbles_f16<2>(w[c]), nibbles_f16<3>(w[c])};
   } else {
     const uint32_t u = w[2 * c], v = w[2 * c + 1];
     x = u32x4{u & 0x00FF00FFu, u >> 8 & 0x00FF00FFu, v & 0x00FF00FFu, v >> 8 & 0x00FF00FFu};
@@ -137,12 +149,6 @@ __device__ __forceinline__ f16x8 query_operand(u32x4 in, float factor) {
 // fp16 subnormals again, 16 times as large where sixteenfold(n).
 template <int D, int kBits>
 struct ValuePart;
-
-template <int i>
-__device__ __forceinline__ uint32_t nibbles_f16(uint32_t w) {
-  const uint32_t x = i >= 2 ? w >> 8 : w;
-  return x & (i % 2 ? 0x00F000F0u : 0x000F000Fu);
-}
 
 template <>
 struct ValuePart<128, 4> {
@@ -253,7 +259,7 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
   for (int i = 0; i < kO; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      cb[(4 * i + r) * 64] = fmaf(O[i][r], ValuePart<D, kBits>::sixteenfold(i) ? 0x1p20f : 0x1p24f, z);
+      cb[(4 * i + r) * 64] = fmaf(O[i][r], (ValuePart<D, kBits>::sixteenfold(i) ? 0.0625f : 1.f) / kCodeUnit<kBits>, z);
   cb[4 * kO * 64] = m_own;
   cb[(4 * kO + 1) * 64] = l_own;
   __syncthreads();
@@ -293,8 +299,7 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
         *reinterpret_cast<uint32_t*>(out + D / 16 * r) = pack_bf16x2(o[0][r] * inv, o[1][r] * inv);
     }
     if (p.lse && lg == 0 && w == 0)
-      p.lse[((int64_t)b * p.heads + head) * p.new_tokens + fresh] =
-          sum == 0.f ? -INFINITY : (m + __log2f(sum)) * 0.6931471805599453f;
+      p.lse[((int64_t)b * p.heads + head) * p.new_tokens + fresh] = natural_log_sum(m, sum);
   } else {
     const int64_t row = ((int64_t)slot * p.heads_k + h) * p.columns + column;
     float* out = p.ws_o + row * D + at;
@@ -480,8 +485,8 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
     const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
 #pragma unroll
     for (int c = 0; c < kC; ++c) Q[c] = query_operand<kBits>(x[c], p.flip * up);
-    qs = wave_sum16(sum) * (p.flip * up * 0x1p-24f);
-    unit = p.scale_log2 * __uint_as_float((uint32_t)(127 + 10 + e) << 23);
+    qs = wave_sum16(sum) * (p.flip * up * kCodeUnit<kBits>);
+    unit = p.scale_log2 * (__uint_as_float((uint32_t)(127 - 14 + e) << 23) / kCodeUnit<kBits>);
   }
 
   f32x4 O[kO];
@@ -729,7 +734,7 @@ extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, 
   p.over_heads_k = FastDiv::of(num_heads_k);
   p.over_column_tiles = FastDiv::of((uint32_t)cut.column_tiles);
   p.over_splits = FastDiv::of(std::max(1, cut.splits));
-  p.scale_log2 = fabsf(softmax_scale) * 1.4426950408889634f;
+  p.scale_log2 = (float)(fabs((double)softmax_scale) * 1.4426950408889634);
   p.flip = softmax_scale < 0.f ? -1.f : 1.f;
   const hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)groups), block(kQaWaves * 64);

@@ -177,8 +177,7 @@ __global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge 
   else
     out[l] = (uint16_t)pack_bf16x2(acc[0] * inv, 0.f);
   if (p.lse && l == 0)
-    p.lse[((int64_t)b * heads + head) * p.new_tokens + fresh] =
-        sum == 0.f ? -INFINITY : (m_run + __log2f(sum)) * 0.6931471805599453f;
+    p.lse[((int64_t)b * heads + head) * p.new_tokens + fresh] = natural_log_sum(m_run, sum);
 }
 
 hipError_t merge_splits(hipStream_t stream, const SplitMerge& p, int head_dim) {

@@ -22,6 +22,13 @@ struct SplitMerge {
 
 hipError_t merge_splits(hipStream_t stream, const SplitMerge& p, int head_dim);
 
+// ln(sum 2^m), -inf for no sum.  (The sum's exponent goes to m, in 64 bits, so that neither
+// the size of the sum nor that of m costs digits.)
+__device__ __forceinline__ float natural_log_sum(float m, float sum) {
+  const double log2 = ((double)m + __builtin_amdgcn_frexp_expf(sum)) + __log2f(__builtin_amdgcn_frexp_mantf(sum));
+  return sum == 0.f ? -INFINITY : (float)(log2 * 0.69314718055994530942);
+}
+
 // Slots of [heads_k][columns] rows, a column being new token * group + head of the
 // group; out is [sequence][new token][head][D], lse [sequence][head][new token].  A
 // sequence's slots are b * splits and up, or with a plan, (first, number) a sequence,
