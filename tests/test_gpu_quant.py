@@ -188,6 +188,28 @@ def test_every_length(torch_cuda, dim, bits, new):
         check(T, q, data, table, lens, page, bits, want=want, num_splits=splits)
 
 
+@pytest.mark.parametrize("kind", ["ragged", "empty", "one", "edges", "even"])
+@pytest.mark.parametrize("batch", [2, 64, 65, 200])
+def test_batches_cut_by_their_lengths(torch_cuda, batch, kind):
+    # parts that hold pieces of several sequences, sequences in several parts, and empty ones wherever they stand
+    T = torch_cuda
+    rng = random.Random(batch)
+    page, width = 16, 40
+    lens = {"ragged": [rng.choice([0, 0, 1, 5, 16, 17, 100, 333, 640]) for _ in range(batch)], "empty": [0] * batch,
+            "one": [0] * (batch - 1) + [611], "edges": [0] * batch, "even": [320] * batch}[kind]
+    if kind == "edges":  # the places around which sequences are looked through
+        for b in (0, 1, 62, 63, 64, 65, 127, 128, batch - 2):
+            lens[b % batch] = rng.choice([16, 512, 640])
+    q, data, table = make(T, batch, batch, 1, 2, 1, 64, page, width, 4)
+    poison(T, data, table, lens, page)
+    want = ref.attend(q, data, table, lens, page, 4)
+    for n in (lens, lens[::-1]):
+        if n is not lens:
+            q, table = q.flip(0).contiguous(), table.flip(0).contiguous()
+            want = tuple(w.flip(0) for w in want)
+        check(T, q, data, table, n, page, 4, want=want)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_long_context(torch_cuda, bits):
     # one sequence over many splits, next to short ones in a wide table

@@ -384,11 +384,14 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
       b = 0;
       len = lens[0];
     } else {
-      s0 = 0;
-      if (p.batch > 64)
-        for (int before = look(0); before <= from && s0 + 64 < p.batch;) s0 += 64, before = look(before);
-      const bool has = s0 + l < p.batch && (tiles ? end > from : end >= from);
-      const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(has) | 1ull << 63);
+      uint64_t have = 0;
+      for (int before = 0, s1 = 0; s1 < p.batch && !have; s1 += 64) {
+        s0 = s1;
+        if (p.batch > 64) before = look(before);
+        have = __builtin_amdgcn_ballot_w64(s0 + l < p.batch && (tiles ? end > from : end >= from));
+      }
+      if (!have) return;  // (never: `from` is below `total`, or all are empty)
+      const int i = __builtin_ctzll(have);
       b = s0 + i;
       len = __builtin_amdgcn_readlane(mine, i);
       start = __builtin_amdgcn_readlane(end, i) - __builtin_amdgcn_readlane(tiles, i);
