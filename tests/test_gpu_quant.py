@@ -194,8 +194,8 @@ def test_batches_cut_by_their_lengths(torch_cuda, batch, kind):
     # parts that hold pieces of several sequences, sequences in several parts, and empty ones wherever they stand
     T = torch_cuda
     rng = random.Random(batch)
-    page, width = 16, 40
-    lens = {"ragged": [rng.choice([0, 0, 1, 5, 16, 17, 100, 333, 640]) for _ in range(batch)], "empty": [0] * batch,
+    page, width = 16, 80
+    lens = {"ragged": [rng.choice([0, 0, 1, 5, 16, 17, 100, 333, 640, 1111]) for _ in range(batch)], "empty": [0] * batch,
             "one": [0] * (batch - 1) + [611], "edges": [0] * batch, "even": [320] * batch}[kind]
     if kind == "edges":  # the places around which sequences are looked through
         for b in (0, 1, 62, 63, 64, 65, 127, 128, batch - 2):
