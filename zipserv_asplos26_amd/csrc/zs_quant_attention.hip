@@ -222,7 +222,7 @@ __device__ __forceinline__ void unrolled(F&& f) {
 // starts at tile floor(i T / P) of the T.  What it has of a sequence that it does not
 // have whole goes into slot 2 i, or 2 i + 1 where the sequence starts inside the part (a
 // part has one at most that ends, and one that starts, outside it).
-constexpr int kLeastChunk = 16;  // tiles of a part at least (one sequence of 2000 tokens: 13.7 us with 32, 11.8 with 16)
+constexpr int kLeastChunk = 16;  // tiles of a part (one sequence of 2000 tokens: 13.7 us with 32, 11.8 with 16)
 
 __device__ __forceinline__ int qa_tiles_of(const QuantAttnParams& p, int len) {
   return (int)min(((int64_t)max(len, 0) + 15) / 16, (int64_t)p.width * p.tiles.d);
@@ -248,8 +248,8 @@ __device__ __forceinline__ int qa_lane() {
 // The waves' states of a tile of columns merged and written, two output tiles a wave: the
 // result, or what goes into a slot (slot >= 0).
 template <int D, int kBits, int kColumns>
-__device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem, const f32x4* O, float m_own, float l_own,
-                                          float z, int ct, int h, int b, int slot) {
+__device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem, const f32x4* O, float m_own,
+                                          float l_own, float z, int ct, int h, int b, int slot) {
   typedef QaShape<D, kBits> Shape;
   constexpr int kO = Shape::kO, W = kQaWaves;
   static_assert(W >= kO / 2, "");
@@ -270,7 +270,8 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
   for (int i = 0; i < W; ++i) m = fmaxf(m, src[i * Shape::kState + 4 * kO * 64]);
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    const float f = __builtin_amdgcn_exp2f(0.5f * (src[i * Shape::kState + 4 * kO * 64] - m));  // (in two steps, as there)
+    // (in two steps, as for a new maximum)
+    const float f = __builtin_amdgcn_exp2f(0.5f * (src[i * Shape::kState + 4 * kO * 64] - m));
     sum += src[i * Shape::kState + (4 * kO + 1) * 64] * f * f;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -337,8 +338,10 @@ __device__ __forceinline__ uint32_t row_from(uint32_t x) {
 __device__ __forceinline__ float row_from8(float x) { return __uint_as_float(row_from<8>(__float_as_uint(x))); }
 __device__ __forceinline__ float row_from4(float x) { return __uint_as_float(row_from<4>(__float_as_uint(x))); }
 
+// (Waves a SIMD: what the registers of a pair on its way and one in work leave room for.)
 template <int D, int kBits, int kFold>
-__global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 ? 2 : 3) void quant_attn_kernel(QuantAttnParams p) {
+__global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 ? 2 : 3) void quant_attn_kernel(
+    QuantAttnParams p) {
   typedef QaShape<D, kBits> Shape;
   typedef QuantRow<D, kBits> Row;
   constexpr int kC = Shape::kC, kO = Shape::kO, W = kQaWaves;
@@ -348,7 +351,8 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
   // Column tiles of the same tokens go to one XCD (workgroups are dealt out to the
   // eight in turn), one soon after another.
-  const int item = (int)p.over_column_tiles.div(blockIdx.x >> 3), ct = (int)(blockIdx.x >> 3) - item * (int)p.over_column_tiles.d;
+  const int item = (int)p.over_column_tiles.div(blockIdx.x >> 3);
+  const int ct = (int)(blockIdx.x >> 3) - item * (int)p.over_column_tiles.d;
   const int at = 8 * item + (blockIdx.x & 7);
   const int part = (int)p.over_heads_k.div((uint32_t)at), h = at - part * p.heads_k;
 
@@ -398,220 +402,223 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
     }
   }
 
+  // Tiles t0 .. t1 of sequence b, into its slot or as its result.
   auto segment = [&](int len, int t0, int t1, int slot) {
-  const int l = qa_lane();
-  const int g = l & 15, lg = l >> 4;
-  const int fold = g / kColumns;
-  // the lane's tokens of a pair: kTokens from `token` of tile `mine` (all of both: 4 each)
-  const int mine = fold * 2 / kFold, token = 4 * lg + (kFold == 4 ? 2 * (fold & 1) : 0);
-  // Where the two tiles of the wave's n-th pair are: the table's entry and the tile in the
-  // page.  Scalar loads, which the many vector loads on the way do not have to be waited
-  // out for, and looked at only when the pair is fetched.
-  struct Place {
-    int block[2], sub[2];
-  };
-  const volatile auto* row = as_constant(p.table + b * p.table_stride);  // (volatile: or the loads move to their use)
-  auto places = [&](int n) {
-    Place x;
+    const int l = qa_lane();
+    const int g = l & 15, lg = l >> 4;
+    const int fold = g / kColumns;
+    // the lane's tokens of a pair: kTokens from `token` of tile `mine` (all of both: 4 each)
+    const int mine = fold * 2 / kFold, token = 4 * lg + (kFold == 4 ? 2 * (fold & 1) : 0);
+    // Where the two tiles of the wave's n-th pair are: the table's entry and the tile in the
+    // page.  Scalar loads, which the many vector loads on the way do not have to be waited
+    // out for, and looked at only when the pair is fetched.
+    struct Place {
+      int block[2], sub[2];
+    };
+    const volatile auto* row = as_constant(p.table + b * p.table_stride);  // (volatile: or the loads move to their use)
+    auto places = [&](int n) {
+      Place x;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int tile = t0 + 2 * (w + W * n) + t;
-      const int lp = (int)p.tiles.div((uint32_t)min(tile, t1 - 1));
-      x.sub[t] = tile - lp * (int)p.tiles.d;
-      x.block[t] = row[lp];
-    }
-    return x;
-  };
-  const uint32_t k_at = g * Row::kBytes + 4 * Shape::kKey * lg, v_at = 4 * lg * Row::kBytes + Row::kBytes / 16 * g;
-  // The wave's n-th pair, on its way.  A tile without a page reads page 0.
-  auto fetch = [&](Pair& x, const Place& at, int n) {
-    x.tile = t0 + 2 * (w + W * n);
-    const uint8_t* kr[2];
-    const uint8_t* vr[2];
-    const uint8_t* sr[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      x.none[t] = (uint32_t)at.block[t] >= (uint32_t)p.num_blocks || x.tile + t >= t1;
-      const int bl = x.none[t] ? 0 : at.block[t], su = x.none[t] ? 0 : at.sub[t];
-      // (scalar addresses, and a lane's own part in 32 bits)
-      const uint8_t* record = p.cache + ((int64_t)bl * p.heads_k + h) * p.record;
-      kr[t] = record + 8 * p.page + 16 * su * Row::kBytes;
-      vr[t] = kr[t] + p.page * Row::kBytes;
-      load_words<Shape::kKey>(kr[t] + k_at, x.k[t]);
-      sr[t] = record + 128 * su;
-    }
-    if constexpr (kFold == 1) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) load_words<8>(sr[t] + 32u * lg, x.side + 8 * t);
-    } else {
-      load_words<2 * kTokens>((mine ? sr[1] : sr[0]) + 8u * token, x.side);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x.v.load(j, vr[j / 4] + v_at + j % 4 * Row::kBytes);
-  };
-  const int pairs = t1 - t0 - 2 * w > 0 ? (t1 - t0 - 2 * w + 2 * W - 1) / (2 * W) : 0;  // of this wave
-  Pair pair[2];
-  Place ahead[2];
-  if (pairs > 0) {
-    ahead[0] = places(0);
-    ahead[1] = places(1);
-    fetch(pair[0], ahead[0], 0);
-  }
-
-  // This lane's column: new token `fresh` of head h * group + hh; it sees `limit` tokens.
-  // q goes in as fp16, times a power of two that takes the largest of a column's to
-  // 2^14..2^15: of the others nothing above 2^-39 of that is lost.  Scores are kept
-  // without `unit`, which is left to do.
-  const int first = len - p.new_tokens + 1;
-  f16x8 Q[kC];
-  float qs, unit;
-  int limit;
-  {
-    const int column = min(kColumns * ct + g % kColumns, p.columns - 1);
-    const int fresh = (int)p.over_group.div((uint32_t)column), hh = column - fresh * p.group;
-    limit = first + fresh;
-    const uint16_t* row = p.q + b * p.q_batch + fresh * p.q_token + (int64_t)(h * p.group + hh) * p.q_head + D / 4 * lg;
-    u32x4 x[kC];
-    float sum = 0.f, most = 0.f;
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      x[c] = *reinterpret_cast<const u32x4*>(row + 8 * c);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float u = __uint_as_float(x[c][j] << 16), v = __uint_as_float(x[c][j] & 0xFFFF0000u);
-        sum += u + v;
-        most = fmaxf(most, fmaxf(fabsf(u), fabsf(v)));
+      for (int t = 0; t < 2; ++t) {
+        const int tile = t0 + 2 * (w + W * n) + t;
+        const int lp = (int)p.tiles.div((uint32_t)min(tile, t1 - 1));
+        x.sub[t] = tile - lp * (int)p.tiles.d;
+        x.block[t] = row[lp];
       }
-    }
-    most = wave_max16(most);
-    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
-    const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+      return x;
+    };
+    const uint32_t k_at = g * Row::kBytes + 4 * Shape::kKey * lg, v_at = 4 * lg * Row::kBytes + Row::kBytes / 16 * g;
+    // The wave's n-th pair, on its way.  A tile without a page reads page 0.
+    auto fetch = [&](Pair& x, const Place& at, int n) {
+      x.tile = t0 + 2 * (w + W * n);
+      const uint8_t* kr[2];
+      const uint8_t* vr[2];
+      const uint8_t* sr[2];
 #pragma unroll
-    for (int c = 0; c < kC; ++c) Q[c] = query_operand<kBits>(x[c], p.flip * up);
-    qs = wave_sum16(sum) * (p.flip * up * kCodeUnit<kBits>);
-    unit = p.scale_log2 * (__uint_as_float((uint32_t)(127 - 14 + e) << 23) / kCodeUnit<kBits>);
-  }
+      for (int t = 0; t < 2; ++t) {
+        x.none[t] = (uint32_t)at.block[t] >= (uint32_t)p.num_blocks || x.tile + t >= t1;
+        const int bl = x.none[t] ? 0 : at.block[t], su = x.none[t] ? 0 : at.sub[t];
+        // (scalar addresses, and a lane's own part in 32 bits)
+        const uint8_t* record = p.cache + ((int64_t)bl * p.heads_k + h) * p.record;
+        kr[t] = record + 8 * p.page + 16 * su * Row::kBytes;
+        vr[t] = kr[t] + p.page * Row::kBytes;
+        load_words<Shape::kKey>(kr[t] + k_at, x.k[t]);
+        sr[t] = record + 128 * su;
+      }
+      if constexpr (kFold == 1) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) load_words<8>(sr[t] + 32u * lg, x.side + 8 * t);
+      } else {
+        load_words<2 * kTokens>((mine ? sr[1] : sr[0]) + 8u * token, x.side);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x.v.load(j, vr[j / 4] + v_at + j % 4 * Row::kBytes);
+    };
+    const int pairs = t1 - t0 - 2 * w > 0 ? (t1 - t0 - 2 * w + 2 * W - 1) / (2 * W) : 0;  // of this wave
+    Pair pair[2];
+    Place ahead[2];
+    if (pairs > 0) {
+      ahead[0] = places(0);
+      ahead[1] = places(1);
+      fetch(pair[0], ahead[0], 0);
+    }
 
-  f32x4 O[kO];
+    // This lane's column: new token `fresh` of head h * group + hh; it sees `limit` tokens.
+    // q goes in as fp16, times a power of two that takes the largest of a column's to
+    // 2^14..2^15: of the others nothing above 2^-39 of that is lost.  Scores are kept
+    // without `unit`, which is left to do.
+    const int first = len - p.new_tokens + 1;
+    f16x8 Q[kC];
+    float qs, unit;
+    int limit;
+    {
+      const int column = min(kColumns * ct + g % kColumns, p.columns - 1);
+      const int fresh = (int)p.over_group.div((uint32_t)column), hh = column - fresh * p.group;
+      limit = first + fresh;
+      const int64_t head = h * p.group + hh;
+      const uint16_t* row = p.q + b * p.q_batch + fresh * p.q_token + head * p.q_head + D / 4 * lg;
+      u32x4 x[kC];
+      float sum = 0.f, most = 0.f;
 #pragma unroll
-  for (int k = 0; k < kO; ++k) O[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -FLT_MAX, l_run = 0.f, z = 0.f;  // z: sum p low_v
-  auto consume = [&](const Pair& x) {
-    f32x4 S[2] = {};
+      for (int c = 0; c < kC; ++c) {
+        x[c] = *reinterpret_cast<const u32x4*>(row + 8 * c);
 #pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      const f16x8 K0 = key_operand<kBits>(x.k[0], c), K1 = key_operand<kBits>(x.k[1], c);
-      S[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K0, Q[c], S[0], 0, 0, 0);
-      S[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K1, Q[c], S[1], 0, 0, 0);
+        for (int j = 0; j < 4; ++j) {
+          const float u = __uint_as_float(x[c][j] << 16), v = __uint_as_float(x[c][j] & 0xFFFF0000u);
+          sum += u + v;
+          most = fmaxf(most, fmaxf(fabsf(u), fabsf(v)));
+        }
+      }
+      most = wave_max16(most);
+      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
+      const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) Q[c] = query_operand<kBits>(x[c], p.flip * up);
+      qs = wave_sum16(sum) * (p.flip * up * kCodeUnit<kBits>);
+      unit = p.scale_log2 * (__uint_as_float((uint32_t)(127 - 14 + e) << 23) / kCodeUnit<kBits>);
     }
-    float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kTokens];
+
+    f32x4 O[kO];
 #pragma unroll
-    for (int j = 0; j < kTokens; ++j) {
-      const uint32_t kp = x.side[2 * j], vp = x.side[2 * j + 1];
-      ks[j] = __uint_as_float(kp << 16);
-      kl[j] = __uint_as_float(kp & 0xFFFF0000u);
-      vs[j] = __uint_as_float(vp << 16);
-      vl[j] = __uint_as_float(vp & 0xFFFF0000u);
-      vs_log[j] = (float)max(vp << 16, kLeastScale);  // * 2^-23: log2 of the scale + 127, up to 0.09 less
-    }
-    // Behind a column's limit and where there is no page nothing counts, whatever it holds.
-    const bool cut = x.none[0] || x.none[1] || first - 16 * x.tile < 32;  // (uniform)
-    constexpr int kWords = kTokens / 2;                                   // packed pairs of a lane's weights
-    float s[kTokens];
+    for (int k = 0; k < kO; ++k) O[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -FLT_MAX, l_run = 0.f, z = 0.f;  // z: sum p low_v
+    auto consume = [&](const Pair& x) {
+      f32x4 S[2] = {};
 #pragma unroll
-    for (int j = 0; j < kTokens; ++j) {
-      float c;
-      if constexpr (kFold == 1)
-        c = S[j / 4][j % 4];
-      else if constexpr (kFold == 2)
-        c = fold ? S[1][j] : S[0][j];
-      else
-        c = fold & 2 ? (fold & 1 ? S[1][2 + j] : S[1][j]) : (fold & 1 ? S[0][2 + j] : S[0][j]);
-      s[j] = fmaf(ks[j], c, kl[j] * qs) * unit;
-    }
-    if (cut) {
+      for (int c = 0; c < kC; ++c) {
+        const f16x8 K0 = key_operand<kBits>(x.k[0], c), K1 = key_operand<kBits>(x.k[1], c);
+        S[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K0, Q[c], S[0], 0, 0, 0);
+        S[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K1, Q[c], S[1], 0, 0, 0);
+      }
+      float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kTokens];
 #pragma unroll
       for (int j = 0; j < kTokens; ++j) {
-        const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
-        const bool seen = at < limit - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
-        s[j] = seen ? s[j] : -INFINITY;
-        vs[j] = seen ? vs[j] : 0.f;
-        vl[j] = seen ? vl[j] : 0.f;
+        const uint32_t kp = x.side[2 * j], vp = x.side[2 * j + 1];
+        ks[j] = __uint_as_float(kp << 16);
+        kl[j] = __uint_as_float(kp & 0xFFFF0000u);
+        vs[j] = __uint_as_float(vp << 16);
+        vl[j] = __uint_as_float(vp & 0xFFFF0000u);
+        vs_log[j] = (float)max(vp << 16, kLeastScale);  // * 2^-23: log2 of the scale + 127, up to 0.09 less
       }
-    }
-    // What a weight is relative to: so that the largest product of a weight and a value's
-    // scale is 2^11..2^15.  Moved only where a product would be larger.
-    float mx = fmaf(vs_log[0], 0x1p-23f, s[0]);
+      // Behind a column's limit and where there is no page nothing counts, whatever it holds.
+      const bool cut = x.none[0] || x.none[1] || first - 16 * x.tile < 32;  // (uniform)
+      constexpr int kWords = kTokens / 2;                                   // packed pairs of a lane's weights
+      float s[kTokens];
 #pragma unroll
-    for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, fmaf(vs_log[j], 0x1p-23f, s[j]));
-    mx -= 127.f + 11.f;
-    if (__builtin_amdgcn_ballot_w64(mx > m_run + 4.f)) {
-      if constexpr (kFold >= 2) mx = fmaxf(mx, row_from8(mx));
-      if constexpr (kFold == 4) mx = fmaxf(mx, row_from4(mx));
-      const float m_new = fmaxf(m_run, wave_max16(mx));
-      // (in two steps: scales can be 2^160 apart, and sums of small ones' weights as large)
-      const float alpha = __builtin_amdgcn_exp2f(0.5f * (m_run - m_new));
-      m_run = m_new;
-      l_run = l_run * alpha * alpha;
-      z = z * alpha * alpha;
-#pragma unroll
-      for (int k = 0; k < kO; ++k) O[k] = O[k] * alpha * alpha;
-    }
-    // weights times scales as sums of two fp16: 22 bits, or 2^-25 where that is more
-    uint32_t own[2][kWords];
-#pragma unroll
-    for (int j = 0; j < kTokens; j += 2) {
-      float y[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float weight = __builtin_amdgcn_exp2f(s[j + e] - m_run);
-        l_run += weight;
-        z = fmaf(weight, vl[j + e], z);
-        y[e] = weight * vs[j + e];
+      for (int j = 0; j < kTokens; ++j) {
+        float c;
+        if constexpr (kFold == 1)
+          c = S[j / 4][j % 4];
+        else if constexpr (kFold == 2)
+          c = fold ? S[1][j] : S[0][j];
+        else
+          c = fold & 2 ? (fold & 1 ? S[1][2 + j] : S[1][j]) : (fold & 1 ? S[0][2 + j] : S[0][j]);
+        s[j] = fmaf(ks[j], c, kl[j] * qs) * unit;
       }
-      const f16x2 a = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
-      const f16x2 c = __builtin_convertvector((f32x2{fmaf((float)a[0], -1.f, y[0]), fmaf((float)a[1], -1.f, y[1])}), f16x2);
-      own[0][j / 2] = __builtin_bit_cast(uint32_t, a);
-      own[1][j / 2] = __builtin_bit_cast(uint32_t, c);
-    }
-    // the other folds' tokens of the column
-    f16x8 weights[2];
+      if (cut) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      u32x4 y;
-      if constexpr (kFold == 1)
-        y = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
-      else if constexpr (kFold == 2)
-        y = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
-      else
-        y = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
-      weights[k] = __builtin_bit_cast(f16x8, y);
-    }
-    unrolled<0, kO>([&](auto n) {
-      constexpr int o = decltype(n)::value;
-      const f16x8 A = x.v.template operand<o>();
+        for (int j = 0; j < kTokens; ++j) {
+          const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
+          const bool seen = at < limit - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
+          s[j] = seen ? s[j] : -INFINITY;
+          vs[j] = seen ? vs[j] : 0.f;
+          vl[j] = seen ? vl[j] : 0.f;
+        }
+      }
+      // What a weight is relative to: so that the largest product of a weight and a value's
+      // scale is 2^11..2^15.  Moved only where a product would be larger.
+      float mx = fmaf(vs_log[0], 0x1p-23f, s[0]);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) O[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, weights[k], O[o], 0, 0, 0);
-    });
-  };
+      for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, fmaf(vs_log[j], 0x1p-23f, s[j]));
+      mx -= 127.f + 11.f;
+      if (__builtin_amdgcn_ballot_w64(mx > m_run + 4.f)) {
+        if constexpr (kFold >= 2) mx = fmaxf(mx, row_from8(mx));
+        if constexpr (kFold == 4) mx = fmaxf(mx, row_from4(mx));
+        const float m_new = fmaxf(m_run, wave_max16(mx));
+        // (in two steps: scales can be 2^160 apart, and sums of small ones' weights as large)
+        const float alpha = __builtin_amdgcn_exp2f(0.5f * (m_run - m_new));
+        m_run = m_new;
+        l_run = l_run * alpha * alpha;
+        z = z * alpha * alpha;
+#pragma unroll
+        for (int k = 0; k < kO; ++k) O[k] = O[k] * alpha * alpha;
+      }
+      // weights times scales as sums of two fp16: 22 bits, or 2^-25 where that is more
+      uint32_t own[2][kWords];
+#pragma unroll
+      for (int j = 0; j < kTokens; j += 2) {
+        float y[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float weight = __builtin_amdgcn_exp2f(s[j + e] - m_run);
+          l_run += weight;
+          z = fmaf(weight, vl[j + e], z);
+          y[e] = weight * vs[j + e];
+        }
+        const f16x2 a = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
+        const f32x2 rest = {fmaf((float)a[0], -1.f, y[0]), fmaf((float)a[1], -1.f, y[1])};
+        const f16x2 c = __builtin_convertvector(rest, f16x2);
+        own[0][j / 2] = __builtin_bit_cast(uint32_t, a);
+        own[1][j / 2] = __builtin_bit_cast(uint32_t, c);
+      }
+      // the other folds' tokens of the column
+      f16x8 weights[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        u32x4 y;
+        if constexpr (kFold == 1)
+          y = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
+        else if constexpr (kFold == 2)
+          y = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
+        else
+          y = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
+        weights[k] = __builtin_bit_cast(f16x8, y);
+      }
+      unrolled<0, kO>([&](auto n) {
+        constexpr int o = decltype(n)::value;
+        const f16x8 A = x.v.template operand<o>();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) O[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, weights[k], O[o], 0, 0, 0);
+      });
+    };
 
-  // A pair's loads go out while the one before is worked on, and its places are read one
-  // pair earlier still.  (Past the last pair page 0 is read, so that the number of loads
-  // on the way is known.)
-  for (int n = 0; n < pairs; n += 2) {
-    fetch(pair[1], ahead[1], n + 1);
-    ahead[0] = places(n + 2);
-    consume(pair[0]);
-    fetch(pair[0], ahead[0], n + 2);
-    ahead[1] = places(n + 3);
-    if (n + 1 < pairs) consume(pair[1]);
-  }
+    // A pair's loads go out while the one before is worked on, and its places are read one
+    // pair earlier still.  (Past the last pair page 0 is read, so that the number of loads
+    // on the way is known.)
+    for (int n = 0; n < pairs; n += 2) {
+      fetch(pair[1], ahead[1], n + 1);
+      ahead[0] = places(n + 2);
+      consume(pair[0]);
+      fetch(pair[0], ahead[0], n + 2);
+      ahead[1] = places(n + 3);
+      if (n + 1 < pairs) consume(pair[1]);
+    }
 
-  l_run = wave_sum16(l_run);
-  z = wave_sum16(z);
-  if constexpr (kFold >= 2) l_run += row_from8(l_run), z += row_from8(z);
-  if constexpr (kFold == 4) l_run += row_from4(l_run), z += row_from4(z);
-  qa_finish<D, kBits, kColumns>(p, smem, O, m_run, l_run, z, ct, h, b, slot);
+    l_run = wave_sum16(l_run);
+    z = wave_sum16(z);
+    if constexpr (kFold >= 2) l_run += row_from8(l_run), z += row_from8(z);
+    if constexpr (kFold == 4) l_run += row_from4(l_run), z += row_from4(z);
+    qa_finish<D, kBits, kColumns>(p, smem, O, m_run, l_run, z, ct, h, b, slot);
   };
 
   for (;;) {
@@ -677,9 +684,11 @@ extern "C" size_t zs_decode_attention_quant_workspace_bytes(int batch, int new_t
   if (batch <= 0 || new_tokens <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k ||
       head_dim <= 0 || max_blocks_per_seq <= 0 || page_block_size < 16 || num_splits < 0)
     return 0;
-  const int64_t rows = (int64_t)batch * num_heads * new_tokens, tiles = (int64_t)max_blocks_per_seq * (page_block_size / 16);
+  const int64_t rows = (int64_t)batch * num_heads * new_tokens;
+  const int64_t tiles = (int64_t)max_blocks_per_seq * (page_block_size / 16);
   if (rows > INT_MAX || tiles > INT_MAX) return 0;  // (such a call is refused)
-  return qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, tiles, num_splits).ws_bytes(batch, num_heads_k, head_dim);
+  return qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, tiles, num_splits)
+      .ws_bytes(batch, num_heads_k, head_dim);
 }
 
 extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, int64_t q_batch_stride,
@@ -701,7 +710,8 @@ extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, 
        15) ||
       ((q_batch_stride | q_token_stride | q_head_stride) & 7))
     return ZS_E_INVAL;
-  const int64_t rows = (int64_t)batch * num_heads * new_tokens, tiles = (int64_t)max_blocks_per_seq * (page_block_size / 16);
+  const int64_t rows = (int64_t)batch * num_heads * new_tokens;
+  const int64_t tiles = (int64_t)max_blocks_per_seq * (page_block_size / 16);
   if (rows > INT_MAX || tiles > INT_MAX) return ZS_E_OVERFLOW;
   const QaCut cut = qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, tiles, num_splits);
   const int64_t groups = (cut.groups * num_heads_k + 7) / 8 * 8 * cut.column_tiles;

@@ -112,7 +112,8 @@ __global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge 
   for (int c0 = share; live && c0 < splits; c0 += 64 * kShare) {
     // 64 splits of this wave's: a lane's own maximum and sum, then their outputs
     const int n = min((splits - c0 + kShare - 1) / kShare, 64);
-    const float2 own = l < n ? *reinterpret_cast<const float2*>(p.ws_ml + 2 * slot(c0 + l * kShare)) : float2{-FLT_MAX, 0.f};
+    const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
+    const float2 own = l < n ? ml[slot(c0 + l * kShare)] : float2{-FLT_MAX, 0.f};
     float x[kAtOnce][kV];
     auto load = [&](int s0) {
 #pragma unroll
