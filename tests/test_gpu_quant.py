@@ -176,6 +176,24 @@ def test_attention(torch_cuda, heads, heads_k, dim, page, width, new, bits):
         check(T, q, data, table, lens, page, bits, want=want, num_splits=splits)
 
 
+@pytest.mark.parametrize("dim,bits", [(128, 4), (128, 8), (64, 4), (64, 8)])
+@pytest.mark.parametrize("group,new", [(8, 4), (1, 29), (4, 12), (8, 8), (5, 13), (3, 35), (2, 60)])
+def test_columns_in_several_tiles(torch_cuda, group, new, dim, bits):
+    # two to eight tiles of 16 columns, the last one whole or not, one or two to a workgroup; the new tokens
+    # of short sequences before the first one see nothing, and scales differ enough for late maxima
+    T = torch_cuda
+    lens, page, width = [1090, 0, 1, 5, 30, 47, 333], 16, 70
+    q, data, table = make(T, group + new, len(lens), new, 2 * group, 2, dim, page, width, bits)
+    side = data[..., :8 * page].view(np.uint16).reshape(len(data), 2, page, 4)
+    power = T.randint(-12, 12, side.shape[:3], generator=T.Generator().manual_seed(new)).float()
+    side[..., 2] = ref.bf16_bits((2.0 ** power).to(T.bfloat16))
+    side[..., 3] = ref.bf16_bits((-2.0 ** (power + bits - 1)).to(T.bfloat16))
+    poison(T, data, table, lens, page)
+    want = ref.attend(q, data, table, lens, page, bits)
+    for splits in (1, 0, 3):
+        check(T, q, data, table, lens, page, bits, want=want, num_splits=splits)
+
+
 @pytest.mark.parametrize("dim,bits,new", [(128, 4, 1), (64, 4, 3), (128, 8, 2), (64, 8, 1)])
 def test_every_length(torch_cuda, dim, bits, new):
     # sequences that end at every place of a tile and of a pair of tiles

@@ -9,8 +9,8 @@
 // products more a row, not a value each channel.
 //
 // A column is a (new token, query head) of one KV head's group; a workgroup of
-// kQaWaves waves takes up to 16 columns and a part of the tokens, a wave 32 tokens (two
-// tiles of 16) at a time, all in registers, with the next pair's loads on the way:
+// kQaWaves waves takes up to 16 columns (of many: 32) and a part of the tokens, a wave 32
+// tokens (two tiles of 16) at a time, all in registers, with the next pair's loads on the way:
 //   S^T = C_k q^T with v_mfma_f32_16x16x32_f16: lane l holds D / 4 codes of token
 //   l%16 (channels D/4 * (l/16) and up, one piece of its row), 8 of them the A operand of a
 //   step; q^T (lane l: column l%16, the same channels) is the B operand.
@@ -338,16 +338,25 @@ __device__ __forceinline__ uint32_t row_from(uint32_t x) {
 __device__ __forceinline__ float row_from8(float x) { return __uint_as_float(row_from<8>(__float_as_uint(x))); }
 __device__ __forceinline__ float row_from4(float x) { return __uint_as_float(row_from<4>(__float_as_uint(x))); }
 
-// (Waves a SIMD: what the registers of a pair on its way and one in work leave room for.)
-template <int D, int kBits, int kFold>
-__global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 ? 2 : 3) void quant_attn_kernel(
+// Waves a SIMD: what the registers of a pair on its way and one in work leave room for.
+constexpr int qa_waves(int dim, int bits, int fold, int tiles) {
+  return tiles > 1 || (dim == 128 && bits == 8 && fold < 4) ? 2 : 3;
+}
+
+// kTiles tiles of columns in one workgroup: codes are loaded and widened once for all.  With
+// more than one, q is read from LDS for each pair.
+template <int D, int kBits, int kFold, int kTiles>
+__global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) void quant_attn_kernel(
     QuantAttnParams p) {
+  static_assert(kTiles == 1 || (kFold == 1 && kTiles <= kQaWaves), "");
   typedef QaShape<D, kBits> Shape;
   typedef QuantRow<D, kBits> Row;
   constexpr int kC = Shape::kC, kO = Shape::kO, W = kQaWaves;
   constexpr int kColumns = 16 / kFold, kTokens = 8 / kFold;  // of a tile of columns; a lane's tokens of a pair
   typedef QaPair<D, kBits, kTokens> Pair;
   __shared__ float smem[W * Shape::kState];
+  __shared__ __attribute__((aligned(16))) f16x8 q_lds[kTiles][kC][64];  // (one tile's stays in registers)
+  __shared__ float2 column_lds[kTiles][16];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
   // Column tiles of the same tokens go to one XCD (workgroups are dealt out to the
   // eight in turn), one soon after another.
@@ -463,18 +472,17 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
       fetch(pair[0], ahead[0], 0);
     }
 
-    // This lane's column: new token `fresh` of head h * group + hh; it sees `limit` tokens.
-    // q goes in as fp16, times a power of two that takes the largest of a column's to
-    // 2^14..2^15: of the others nothing above 2^-39 of that is lost.  Scores are kept
-    // without `unit`, which is left to do.
+    // This lane's column of a tile: new token `fresh` of head h * group + hh; it sees `limit`
+    // tokens.  q goes in as fp16, times a power of two that takes the largest of a
+    // column's to 2^14..2^15: of the others nothing above 2^-39 of that is lost.  Scores
+    // are kept without `unit`, which is left to do.
     const int first = len - p.new_tokens + 1;
-    f16x8 Q[kC];
-    float qs, unit;
-    int limit;
-    {
-      const int column = min(kColumns * ct + g % kColumns, p.columns - 1);
+    f16x8 Q[kTiles == 1 ? kC : 1];
+    float qs[kTiles], unit[kTiles];
+    int limit[kTiles];
+    auto query = [&](int i, f16x8* to, float& sum_q, float& unit_q) {
+      const int column = min(kColumns * (kTiles * ct + i) + g % kColumns, p.columns - 1);
       const int fresh = (int)p.over_group.div((uint32_t)column), hh = column - fresh * p.group;
-      limit = first + fresh;
       const int64_t head = h * p.group + hh;
       const uint16_t* row = p.q + b * p.q_batch + fresh * p.q_token + head * p.q_head + D / 4 * lg;
       u32x4 x[kC];
@@ -493,22 +501,59 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
       const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
       const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
 #pragma unroll
-      for (int c = 0; c < kC; ++c) Q[c] = query_operand<kBits>(x[c], p.flip * up);
-      qs = wave_sum16(sum) * (p.flip * up * kCodeUnit<kBits>);
-      unit = p.scale_log2 * (__uint_as_float((uint32_t)(127 - 14 + e) << 23) / kCodeUnit<kBits>);
+      for (int c = 0; c < kC; ++c) to[c] = query_operand<kBits>(x[c], p.flip * up);
+      sum_q = wave_sum16(sum) * (p.flip * up * kCodeUnit<kBits>);
+      unit_q = p.scale_log2 * (__uint_as_float((uint32_t)(127 - 14 + e) << 23) / kCodeUnit<kBits>);
+    };
+    if constexpr (kTiles == 1) {
+      query(0, Q, qs[0], unit[0]);
+    } else {
+      // wave i makes tile i's, for all of them
+      if (w < kTiles) {
+        f16x8 mine_q[kC];
+        float2 x;
+        query(w, mine_q, x.x, x.y);
+#pragma unroll
+        for (int c = 0; c < kC; ++c) q_lds[w][c][l] = mine_q[c];
+        if (lg == 0) column_lds[w][g] = x;
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const int column = min(kColumns * (kTiles * ct + i) + g % kColumns, p.columns - 1);
+      limit[i] = first + (int)p.over_group.div((uint32_t)column);
+      if constexpr (kTiles > 1) {
+        const float2 x = column_lds[i][g];
+        qs[i] = x.x;
+        unit[i] = x.y;
+      }
     }
 
-    f32x4 O[kO];
+    f32x4 O[kTiles][kO];
+    float m_run[kTiles], l_run[kTiles], z[kTiles];  // z: sum p low_v
 #pragma unroll
-    for (int k = 0; k < kO; ++k) O[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m_run = -FLT_MAX, l_run = 0.f, z = 0.f;  // z: sum p low_v
+    for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+      for (int k = 0; k < kO; ++k) O[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[i] = -FLT_MAX;
+      l_run[i] = z[i] = 0.f;
+    }
     auto consume = [&](const Pair& x) {
-      f32x4 S[2] = {};
+      f32x4 S[kTiles][2] = {};
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
         const f16x8 K0 = key_operand<kBits>(x.k[0], c), K1 = key_operand<kBits>(x.k[1], c);
-        S[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K0, Q[c], S[0], 0, 0, 0);
-        S[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K1, Q[c], S[1], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          f16x8 q;
+          if constexpr (kTiles == 1)
+            q = Q[c];
+          else
+            q = q_lds[i][c][l];
+          S[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K0, q, S[i][0], 0, 0, 0);
+          S[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K1, q, S[i][1], 0, 0, 0);
+        }
       }
       float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kTokens];
 #pragma unroll
@@ -523,82 +568,90 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
       // Behind a column's limit and where there is no page nothing counts, whatever it holds.
       const bool cut = x.none[0] || x.none[1] || first - 16 * x.tile < 32;  // (uniform)
       constexpr int kWords = kTokens / 2;                                   // packed pairs of a lane's weights
-      float s[kTokens];
+      f16x8 weights[kTiles][2];
 #pragma unroll
-      for (int j = 0; j < kTokens; ++j) {
-        float c;
-        if constexpr (kFold == 1)
-          c = S[j / 4][j % 4];
-        else if constexpr (kFold == 2)
-          c = fold ? S[1][j] : S[0][j];
-        else
-          c = fold & 2 ? (fold & 1 ? S[1][2 + j] : S[1][j]) : (fold & 1 ? S[0][2 + j] : S[0][j]);
-        s[j] = fmaf(ks[j], c, kl[j] * qs) * unit;
-      }
-      if (cut) {
+      for (int i = 0; i < kTiles; ++i) {
+        float s[kTokens], vs_i[kTokens], vl_i[kTokens];
 #pragma unroll
         for (int j = 0; j < kTokens; ++j) {
-          const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
-          const bool seen = at < limit - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
-          s[j] = seen ? s[j] : -INFINITY;
-          vs[j] = seen ? vs[j] : 0.f;
-          vl[j] = seen ? vl[j] : 0.f;
+          float c;
+          if constexpr (kFold == 1)
+            c = S[i][j / 4][j % 4];
+          else if constexpr (kFold == 2)
+            c = fold ? S[i][1][j] : S[i][0][j];
+          else
+            c = fold & 2 ? (fold & 1 ? S[i][1][2 + j] : S[i][1][j]) : (fold & 1 ? S[i][0][2 + j] : S[i][0][j]);
+          s[j] = fmaf(ks[j], c, kl[j] * qs[i]) * unit[i];
+          vs_i[j] = vs[j];
+          vl_i[j] = vl[j];
         }
-      }
-      // What a weight is relative to: so that the largest product of a weight and a value's
-      // scale is 2^11..2^15.  Moved only where a product would be larger.
-      float mx = fmaf(vs_log[0], 0x1p-23f, s[0]);
+        if (cut) {
 #pragma unroll
-      for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, fmaf(vs_log[j], 0x1p-23f, s[j]));
-      mx -= 127.f + 11.f;
-      if (__builtin_amdgcn_ballot_w64(mx > m_run + 4.f)) {
-        if constexpr (kFold >= 2) mx = fmaxf(mx, row_from8(mx));
-        if constexpr (kFold == 4) mx = fmaxf(mx, row_from4(mx));
-        const float m_new = fmaxf(m_run, wave_max16(mx));
-        // (in two steps: scales can be 2^160 apart, and sums of small ones' weights as large)
-        const float alpha = __builtin_amdgcn_exp2f(0.5f * (m_run - m_new));
-        m_run = m_new;
-        l_run = l_run * alpha * alpha;
-        z = z * alpha * alpha;
-#pragma unroll
-        for (int k = 0; k < kO; ++k) O[k] = O[k] * alpha * alpha;
-      }
-      // weights times scales as sums of two fp16: 22 bits, or 2^-25 where that is more
-      uint32_t own[2][kWords];
-#pragma unroll
-      for (int j = 0; j < kTokens; j += 2) {
-        float y[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float weight = __builtin_amdgcn_exp2f(s[j + e] - m_run);
-          l_run += weight;
-          z = fmaf(weight, vl[j + e], z);
-          y[e] = weight * vs[j + e];
+          for (int j = 0; j < kTokens; ++j) {
+            const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
+            const bool seen = at < limit[i] - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
+            s[j] = seen ? s[j] : -INFINITY;
+            vs_i[j] = seen ? vs[j] : 0.f;
+            vl_i[j] = seen ? vl[j] : 0.f;
+          }
         }
-        const f16x2 a = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
-        const f32x2 rest = {fmaf((float)a[0], -1.f, y[0]), fmaf((float)a[1], -1.f, y[1])};
-        const f16x2 c = __builtin_convertvector(rest, f16x2);
-        own[0][j / 2] = __builtin_bit_cast(uint32_t, a);
-        own[1][j / 2] = __builtin_bit_cast(uint32_t, c);
-      }
-      // the other folds' tokens of the column
-      f16x8 weights[2];
+        // What a weight is relative to: so that the largest product of a weight and a value's
+        // scale is 2^11..2^15.  Moved only where a product would be larger.
+        float mx = fmaf(vs_log[0], 0x1p-23f, s[0]);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        u32x4 y;
-        if constexpr (kFold == 1)
-          y = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
-        else if constexpr (kFold == 2)
-          y = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
-        else
-          y = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
-        weights[k] = __builtin_bit_cast(f16x8, y);
+        for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, fmaf(vs_log[j], 0x1p-23f, s[j]));
+        mx -= 127.f + 11.f;
+        if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + 4.f)) {
+          if constexpr (kFold >= 2) mx = fmaxf(mx, row_from8(mx));
+          if constexpr (kFold == 4) mx = fmaxf(mx, row_from4(mx));
+          const float m_new = fmaxf(m_run[i], wave_max16(mx));
+          // (in two steps: scales can be 2^160 apart, and sums of small ones' weights as large)
+          const float alpha = __builtin_amdgcn_exp2f(0.5f * (m_run[i] - m_new));
+          m_run[i] = m_new;
+          l_run[i] = l_run[i] * alpha * alpha;
+          z[i] = z[i] * alpha * alpha;
+#pragma unroll
+          for (int k = 0; k < kO; ++k) O[i][k] = O[i][k] * alpha * alpha;
+        }
+        // weights times scales as sums of two fp16: 22 bits, or 2^-25 where that is more
+        uint32_t own[2][kWords];
+#pragma unroll
+        for (int j = 0; j < kTokens; j += 2) {
+          float y[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float weight = __builtin_amdgcn_exp2f(s[j + e] - m_run[i]);
+            l_run[i] += weight;
+            z[i] = fmaf(weight, vl_i[j + e], z[i]);
+            y[e] = weight * vs_i[j + e];
+          }
+          const f16x2 a = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
+          const f32x2 rest = {fmaf((float)a[0], -1.f, y[0]), fmaf((float)a[1], -1.f, y[1])};
+          const f16x2 c = __builtin_convertvector(rest, f16x2);
+          own[0][j / 2] = __builtin_bit_cast(uint32_t, a);
+          own[1][j / 2] = __builtin_bit_cast(uint32_t, c);
+        }
+        // the other folds' tokens of the column
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          u32x4 y;
+          if constexpr (kFold == 1)
+            y = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
+          else if constexpr (kFold == 2)
+            y = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
+          else
+            y = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
+          weights[i][k] = __builtin_bit_cast(f16x8, y);
+        }
       }
       unrolled<0, kO>([&](auto n) {
         constexpr int o = decltype(n)::value;
         const f16x8 A = x.v.template operand<o>();
 #pragma unroll
-        for (int k = 0; k < 2; ++k) O[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, weights[k], O[o], 0, 0, 0);
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i)
+            O[i][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, weights[i][k], O[i][o], 0, 0, 0);
       });
     };
 
@@ -614,11 +667,14 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
       if (n + 1 < pairs) consume(pair[1]);
     }
 
-    l_run = wave_sum16(l_run);
-    z = wave_sum16(z);
-    if constexpr (kFold >= 2) l_run += row_from8(l_run), z += row_from8(z);
-    if constexpr (kFold == 4) l_run += row_from4(l_run), z += row_from4(z);
-    qa_finish<D, kBits, kColumns>(p, smem, O, m_run, l_run, z, ct, h, b, slot);
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      float sum = wave_sum16(l_run[i]), rest = wave_sum16(z[i]);
+      if constexpr (kFold >= 2) sum += row_from8(sum), rest += row_from8(rest);
+      if constexpr (kFold == 4) sum += row_from4(sum), rest += row_from4(rest);
+      if (i) __syncthreads();  // the last tile's states are read
+      qa_finish<D, kBits, kColumns>(p, smem, O[i], m_run[i], sum, rest, kTiles * ct + i, h, b, slot);
+    }
   };
 
   for (;;) {
@@ -647,9 +703,15 @@ __global__ __launch_bounds__(kQaWaves * 64, D == 128 && kBits == 8 && kFold < 4 
 // what registers allow at once (heads of 64: four; one less or one more costs 2 to 30%),
 // but 64 a sequence at most (32000 tokens: 17.0 us in 96, 16.3 in 64).
 constexpr int kWholeTiles = 64;
+// Tiles of columns go two to a workgroup where none or few are left over.  Sixteen
+// sequences of 8000 tokens, heads of 128, one tile against two a workgroup: two tiles 56 and
+// 54 us (8 bits 75 and 66), three 73 and 82, four 95 and 85 (8 bits 117 and 94); four
+// sequences of 4000 tokens with 32 tiles 101 and 76.
+constexpr int kOddTiles = 7;
 struct QaCut {
-  int64_t columns, column_tiles, groups, slots;  // groups: workgroups of a KV head and a tile of columns
-  int splits, parts;                             // as in the parameters
+  int64_t columns, column_tiles;  // the latter: of `tiles` times 16 columns
+  int64_t groups, slots;          // groups: workgroups of a KV head and a tile of columns
+  int tiles, splits, parts;       // (the last two as in the parameters)
 
   bool whole() const { return splits == 1; }
   size_t ws_bytes(int batch, int heads_k, int head_dim) const {
@@ -660,7 +722,9 @@ struct QaCut {
 static QaCut qa_cut(int batch, int new_tokens, int heads, int heads_k, int head_dim, int64_t tiles, int num_splits) {
   QaCut c{};
   c.columns = (int64_t)(heads / heads_k) * new_tokens;
-  c.column_tiles = (c.columns + 15) / 16;
+  const int64_t all = (c.columns + 15) / 16;
+  c.tiles = all % 2 == 0 || all >= kOddTiles ? 2 : 1;
+  c.column_tiles = (all + c.tiles - 1) / c.tiles;
   const int64_t units = c.column_tiles * heads_k, target = (int64_t)(head_dim == 64 ? 4 : 3) * device_cu_count();
   if (num_splits > 0)
     c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(num_splits, (tiles + 2 * kQaWaves - 1) / (2 * kQaWaves)));
@@ -760,11 +824,13 @@ extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, 
   auto launch = [&](auto dim, auto width) {
     constexpr int D = decltype(dim)::value, kBits = decltype(width)::value;
     if (cut.columns <= 4)
-      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 4>), grid, block, 0, st, p);
+      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 4, 1>), grid, block, 0, st, p);
     else if (cut.columns <= 8)
-      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 2>), grid, block, 0, st, p);
+      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 2, 1>), grid, block, 0, st, p);
+    else if (cut.tiles == 1)
+      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 1, 1>), grid, block, 0, st, p);
     else
-      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 1>), grid, block, 0, st, p);
+      hipLaunchKernelGGL((quant_attn_kernel<D, kBits, 1, 2>), grid, block, 0, st, p);
   };
   typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 8> Eight;
