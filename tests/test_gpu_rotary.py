@@ -132,6 +132,25 @@ def test_python_refuses(torch_cuda):
             rotary.apply_rotary(wrong, None, at, f, inplace=True)
 
 
+def test_in_place_of_one_another(torch_cuda):
+    # q and k of one buffer: rows that follow one another, heads that alternate, and places in common
+    T = torch_cuda
+    x = T.randn(10, 12, 64, device="cuda")
+    f, at = rotary.rotary_frequencies(64)[0], T.arange(10, dtype=T.int32, device="cuda")
+    for q, k in ((x[:, :8], x[:, 8:10]), (x[:, 4:], x[:, :2]), (x[:, ::3], x[:, 1::3]), (x[:, 2::3], x[:, ::3]),
+                 (x[:4], x[4:8]), (x[:1, :3], x[:1, 3:]), (x[:1, ::2], x[:1, 1::2]), (x[2:6, :1], x[2:6, 5:6])):
+        n = q.shape[0]
+        want = rotary.apply_rotary(q, k, at[:n], f)
+        got = rotary.apply_rotary(q, k, at[:n], f, inplace=True)
+        assert T.equal(got[0], want[0]) and T.equal(got[1], want[1])
+    for q, k in ((x, x), (x[:, :8], x[:, 7:]), (x[:, ::3], x[:, 3::3]), (x[:, 4:], x[:, :5]), (x[:6, :6], x[4:, :6]),
+                 (x[:1], x[:1]), (x[:1, :4], x[:1, 3:]), (x[..., :32], x[..., 16:48])):
+        before = x.clone()
+        with pytest.raises(ValueError):
+            rotary.apply_rotary(q, k, at[:q.shape[0]], f[:8], inplace=True)
+        assert T.equal(x, before)
+
+
 def test_in_a_graph_and_on_a_stream(torch_cuda):
     T = torch_cuda
     q, k, x = inputs(T, 9, 300, 8, 2, 128, T.bfloat16)

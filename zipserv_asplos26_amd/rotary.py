@@ -80,6 +80,28 @@ def _apart(t):
     return True
 
 
+def _meet(q, k, tokens, dim, size):
+    """Whether tensors of `size` bytes an element that are turned in place, as `_side`
+    gives them, may share one.  They do not where their addresses are apart, or, with the
+    same stride, their rows of heads or, interleaved, their heads."""
+    at, token, head, heads = q[0], q[1], q[2], q[6]
+    k_at, k_token, k_head, k_heads = k[0], k[1], k[2], k[6]
+    if not (tokens and heads and k_heads):
+        return False
+    off, row, k_row = (k_at - at) // size, (heads - 1) * head + dim, (k_heads - 1) * k_head + dim
+    if off >= (tokens - 1) * token + row or -off >= (tokens - 1) * k_token + k_row:
+        return False
+
+    def apart(step, one, other):  # one each in every `step` elements
+        return step > 0 and off % step >= one and off % step + other <= step
+
+    if tokens > 1 and token != k_token:
+        return True
+    if tokens > 1 and apart(token, row, k_row):
+        return False
+    return not (head == k_head and apart(head, dim, dim) and (tokens == 1 or token % head == 0))
+
+
 _ONE, _THREE, _FOUR = (None,), (None, None, None), (None, None, None, None)
 _ABSENT = (0, 0, 0, 0, 0, 0, 0)
 
@@ -118,8 +140,9 @@ def apply_rotary(q, k, positions, frequencies, factor: float = 1.0, interleaved:
     a position; cosines and sines are multiplied by factor.
 
     Pair i is channels (i, i + pairs), with `interleaved` (2i, 2i + 1).  With `inplace` q
-    and k are turned where they are (and returned), else into new contiguous
-    tensors.  frequencies negated turn back what factor 1 has turned."""
+    and k are turned where they are (and returned), else into new contiguous tensors;
+    in one buffer a token's heads of q then stand before or behind its heads of k, or the two
+    alternate.  frequencies negated turn back what factor 1 has turned."""
     torch = _torch()
     if not isinstance(q, torch.Tensor):
         raise ValueError("q must be a bfloat16, float16 or float32 CUDA tensor")
@@ -151,6 +174,8 @@ def apply_rotary(q, k, positions, frequencies, factor: float = 1.0, interleaved:
         raise ValueError("there must be less than 2^31 tokens")
     q_out, q_in, q_args = _side("q", q, tokens, dim, inplace, torch)
     k_out, k_in, k_args = (None, None, _ABSENT) if k is None else _side("k", k, tokens, dim, inplace, torch)
+    if inplace and k is not None and _meet(q_args, k_args, tokens, dim, q.element_size()):
+        raise ValueError("q and k are turned in place: they must stand apart")
     # (q_in and k_in are held until the launch is queued)
     check("zs_rotary", lib().zs_rotary(stream, *q_args, *k_args, type_, positions.data_ptr(), tokens, dim,
                                        frequencies.data_ptr(), pairs, factor, bool(interleaved)))
