@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryParams p) 
   }
   __syncthreads();
   const int all = n * p.per_token;
-  for (int i = blockIdx.y * kRotaryThreads + threadIdx.x; i < all; i += gridDim.y * kRotaryThreads) {
+  for (int i = threadIdx.x; i < all; i += kRotaryThreads) {
     const int t = (int)p.over_token.div((uint32_t)i), in_token = i - t * p.per_token;
     int h = (int)p.over_items.div((uint32_t)in_token);
     const int c = in_token - h * p.items;
