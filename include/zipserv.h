@@ -624,10 +624,11 @@ int zs_paged_read_quant(void* stream, const uint8_t* cache, int num_blocks, int 
  * [head_dim] bf16, strides in elements, multiples of 8; out: the same shape,
  * contiguous; softmax_lse (optional): [batch][num_heads][new_tokens].  q and out
  * are 16-byte aligned.  A row that sees no token gives zeros and softmax_lse -inf.
- * Tokens past the table's width and in pages outside the pool count for nothing.  num_splits = 0 picks
- * the splits of long sequences; the workspace (16-byte aligned) is what the query
- * says for the same arguments.  batch, and num_heads_k times the 16-column pieces
- * of num_heads / num_heads_k * new_tokens, are at most 65535. */
+ * Tokens past the table's width and in pages outside the pool count for nothing.
+ * num_splits = 0 cuts a batch by its lengths, n > 0 every sequence into n parts (of
+ * 128 tokens or more); the workspace (16-byte aligned) is what the query says for
+ * the same arguments.  batch * num_heads * new_tokens is below 2^31.  Scales are not
+ * negative (an append makes none), and |q| is at most 2^100. */
 size_t zs_decode_attention_quant_workspace_bytes(int batch, int new_tokens, int num_heads,
                                                  int num_heads_k, int head_dim,
                                                  int max_blocks_per_seq, int page_block_size,
