@@ -699,14 +699,16 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
 // How a call is cut.  Where num_splits leaves it open: sequences whole where the table
 // holds no more than kWholeTiles (the merge costs 4 us: 1000 tokens of one sequence take
 // 11 us whole, 11.7 in parts), or where there are six (sequence, KV head, column
-// tile) units a CU, which even out by themselves; else into parts, three workgroups a CU,
-// what registers allow at once (heads of 64: four; one less or one more costs 2 to 30%),
-// but 64 a sequence at most (32000 tokens: 17.0 us in 96, 16.3 in 64).
+// tile) units a CU, which even out by themselves; else into parts, as many as registers
+// allow at once, two to four workgroups a CU (one less or one more costs 2 to 30%: 20
+// ragged sequences of 8000 tokens with 64 heads of 128 in 8 bits take 38 us in two a CU, 43 in
+// three), but 64 a sequence at most (32000 tokens: 17.0 us in 96, 16.3 in 64).
 constexpr int kWholeTiles = 64;
-// Tiles of columns go two to a workgroup where none or few are left over.  Sixteen
-// sequences of 8000 tokens, heads of 128, one tile against two a workgroup: two tiles 56 and
-// 54 us (8 bits 75 and 66), three 73 and 82, four 95 and 85 (8 bits 117 and 94); four
-// sequences of 4000 tokens with 32 tiles 101 and 76.
+// Tiles of columns go two to a workgroup where none or few are left over, and in 8 bits
+// of 128 channels always.  Sixteen sequences of 8000 tokens, heads of 128, one tile
+// against two a workgroup: two tiles 55 and 49 us (8 bits 75 and 58), three 71 and 77 (8
+// bits 98 and 83; heads of 64 57 and 62), four 93 and 79 (8 bits 118 and 89); four
+// sequences of 4000 tokens with 32 tiles 97 and 73.
 constexpr int kOddTiles = 7;
 struct QaCut {
   int64_t columns, column_tiles;  // the latter: of `tiles` times 16 columns
@@ -719,19 +721,23 @@ struct QaCut {
   }
 };
 
-static QaCut qa_cut(int batch, int new_tokens, int heads, int heads_k, int head_dim, int64_t tiles, int num_splits) {
+static QaCut qa_cut(int batch, int new_tokens, int heads, int heads_k, int head_dim, int bits, int64_t tiles,
+                    int num_splits) {
   QaCut c{};
   c.columns = (int64_t)(heads / heads_k) * new_tokens;
   const int64_t all = (c.columns + 15) / 16;
-  c.tiles = all % 2 == 0 || all >= kOddTiles ? 2 : 1;
+  c.tiles = all > 1 && (all % 2 == 0 || all >= kOddTiles || (head_dim == 128 && bits == 8)) ? 2 : 1;
   c.column_tiles = (all + c.tiles - 1) / c.tiles;
-  const int64_t units = c.column_tiles * heads_k, target = (int64_t)(head_dim == 64 ? 4 : 3) * device_cu_count();
+  const int64_t units = c.column_tiles * heads_k, cus = device_cu_count();
+  const int fit = c.tiles == 2 || (head_dim == 128 && bits == 8 && c.columns > 4) ? 2
+                  : head_dim == 64 && c.columns <= 8                               ? 4
+                                                                                   : 3;
   if (num_splits > 0)
     c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(num_splits, (tiles + 2 * kQaWaves - 1) / (2 * kQaWaves)));
-  else if (tiles <= kWholeTiles || batch * units >= 2 * target || batch * tiles > INT_MAX)
+  else if (tiles <= kWholeTiles || batch * units >= 6 * cus || batch * tiles > INT_MAX)
     c.splits = 1;
   else
-    c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(target / units, 64 * (int64_t)batch));
+    c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(fit * cus / units, 64 * (int64_t)batch));
   if (c.parts > batch) c.parts -= c.parts % batch;  // sequences of one length are cut alike
   c.groups = c.splits ? (int64_t)batch * c.splits : c.parts;
   c.slots = c.splits ? c.groups : 2 * c.groups;
@@ -751,8 +757,11 @@ extern "C" size_t zs_decode_attention_quant_workspace_bytes(int batch, int new_t
   const int64_t rows = (int64_t)batch * num_heads * new_tokens;
   const int64_t tiles = (int64_t)max_blocks_per_seq * (page_block_size / 16);
   if (rows > INT_MAX || tiles > INT_MAX) return 0;  // (such a call is refused)
-  return qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, tiles, num_splits)
-      .ws_bytes(batch, num_heads_k, head_dim);
+  size_t most = 0;
+  for (int bits = 4; bits <= 8; bits += 4)
+    most = std::max(most, qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, bits, tiles, num_splits)
+                              .ws_bytes(batch, num_heads_k, head_dim));
+  return most;
 }
 
 extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, int64_t q_batch_stride,
@@ -777,7 +786,7 @@ extern "C" int zs_decode_attention_quant_paged(void* stream, const uint16_t* q, 
   const int64_t rows = (int64_t)batch * num_heads * new_tokens;
   const int64_t tiles = (int64_t)max_blocks_per_seq * (page_block_size / 16);
   if (rows > INT_MAX || tiles > INT_MAX) return ZS_E_OVERFLOW;
-  const QaCut cut = qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, tiles, num_splits);
+  const QaCut cut = qa_cut(batch, new_tokens, num_heads, num_heads_k, head_dim, bits, tiles, num_splits);
   const int64_t groups = (cut.groups * num_heads_k + 7) / 8 * 8 * cut.column_tiles;
   if (cut.groups > INT_MAX / num_heads_k || !grid_fits(groups, kQaWaves * 64) ||
       (!cut.whole() && !grid_fits(merge_parts_groups(batch, num_heads_k, cut.columns), kPartMergeThreads)))
