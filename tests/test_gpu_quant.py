@@ -123,6 +123,29 @@ def test_pools_past_32_bits(torch_cuda):
     assert ((out.cpu().double() - want[:, 0]).abs() <= tol[:, 0]).all()
 
 
+def test_tokens_past_32_bits(torch_cuda):
+    # more than 2^31 elements of keys: only the last tokens have slots, read back among many that have none
+    T = torch_cuda
+    n, heads_k, dim, page, bits = 2100000, 8, 128, 16, 4
+    assert n * heads_k * dim > 2 ** 31
+    cache = paged.quantized_kv_cache(2, page, heads_k, dim, bits)
+    cache.data.zero_()
+    g = T.Generator().manual_seed(4)
+    last = T.randn(page, heads_k, dim, generator=g).to(T.bfloat16)
+    k = T.zeros(n, heads_k, dim, dtype=T.bfloat16, device="cuda")
+    k[-page:] = last.cuda()
+    slots = T.full((n,), -1, dtype=T.int32, device="cuda")
+    slots[-page:] = T.arange(page, dtype=T.int32, device="cuda") + page
+    paged.append_paged_kv_quantized(k, k, cache, slots)
+    mirror = np.zeros((2, heads_k, ref.record_bytes(page, dim, bits)), dtype=np.uint8)
+    ref.append(last, last, mirror, T.arange(page) + page, page, dim, bits)
+    np.testing.assert_array_equal(cache.data.cpu().numpy(), mirror)
+    del k
+    for x, y in zip(paged.read_paged_kv_quantized(cache, slots), ref.read(mirror, T.arange(page) + page, page, dim, bits)):
+        assert T.equal(x[-page:].cpu(), y)
+        assert not x[:5].any() and not x[n // 2:n // 2 + 5].any() and not x[-page - 5:-page].any()
+
+
 # ---------------------------------------------------------------------------
 # Attention
 # ---------------------------------------------------------------------------
@@ -238,6 +261,20 @@ def test_long_context(torch_cuda, bits):
     want = ref.attend(q, data, table, lens, page, bits)
     for splits in (0, 1, 300):
         check(T, q, data, table, lens, page, bits, want=want, num_splits=splits)
+
+
+def test_queries_past_32_bits(torch_cuda):
+    # more than 2^31 elements of q: the same few sequences again and again
+    T = torch_cuda
+    few, times, new, heads, page, width, bits = 4, 1030, 64, 64, 16, 5, 4
+    lens = [80, 3, 0, 65]
+    q, data, table = make(T, 31, few, new, heads, 8, 128, page, width, bits)
+    assert q.numel() * times > 2 ** 31
+    cache, many = gpu_cache(T, data, page, 128, bits), T.tensor(lens, dtype=T.int32).repeat(times).cuda()
+    out, lse = attention.flash_attn_with_kvcache_quantized(
+        q.cuda().repeat(times, 1, 1, 1), cache, table.repeat(times, 1).cuda(), many, return_softmax_lse=True)
+    one, one_lse = check(T, q, data, table, lens, page, bits, num_splits=1)
+    assert (out.view(times, few, new, heads, 128) == one).all() and (lse.view(times, few, heads, new) == one_lse).all()
 
 
 @pytest.mark.parametrize("bits", [4, 8])

@@ -66,6 +66,21 @@ def test_far_positions(torch_cuda, interleaved):
         within(z, *ref.rotary(y, at, f, 1.0, interleaved))
 
 
+def test_tokens_past_32_bits(torch_cuda):
+    # more than 2^31 elements of q: the same few tokens again and again, into an output and in place
+    T = torch_cuda
+    q, _, _ = inputs(T, 10, 64, 32, 1, 128, T.bfloat16)
+    at, f = T.arange(100, 164, dtype=T.int32, device="cuda"), rotary.rotary_frequencies(128)[0]
+    want = rotary.apply_rotary(q.cuda(), None, at, f)[0]
+    many = q.cuda().repeat(8200, 1, 1)
+    assert many.numel() > 2 ** 31
+    got = rotary.apply_rotary(many, None, at.repeat(8200), f)[0]
+    assert (got.view(8200, 64, 32, 128) == want).all()
+    del got
+    rotary.apply_rotary(many, None, at.repeat(8200), f, inplace=True)
+    assert (many.view(8200, 64, 32, 128) == want).all()
+
+
 def test_turned_back(torch_cuda):
     # negated frequencies undo a rotation, whatever is left of it is the two roundings
     T = torch_cuda
