@@ -483,6 +483,43 @@ def test_captured_steps_replay(torch_cuda):
         T.cuda.synchronize()
 
 
+@pytest.mark.parametrize("new,bits", [(1, 4), (1, 8), (5, 8), (8, 4)])
+def test_captured_lengths_change(torch_cuda, new, bits):
+    # one captured call, replayed as sequences grow, end, come back and share each other's pages
+    T = torch_cuda
+    page, width, batch, heads, heads_k, dim = 16, 100, 70, 16, 2, 64
+    q, data, table = make(T, 40 + new, batch, new, heads, heads_k, dim, page, width, bits)
+    cache, tab, qd = gpu_cache(T, data, page, dim, bits), table.cuda(), q.cuda()
+    lens = T.full((batch,), 1600, dtype=T.int32, device="cuda")
+
+    def call():
+        return attention.flash_attn_with_kvcache_quantized(qd, cache, tab, lens, return_softmax_lse=True)
+
+    call()
+    T.cuda.synchronize()
+    graph = T.cuda.CUDAGraph()
+    with T.cuda.graph(graph):
+        out, lse = call()
+    rng = random.Random(new)
+    for turn in range(6):
+        now = [[1600] * batch, [0] * batch, [0] * (batch - 1) + [1600], [rng.choice([0, 1, 17, 333]) for _ in range(batch)],
+               [rng.randrange(1601) for _ in range(batch)], [1 + b for b in range(batch)]][turn]
+        lens.copy_(T.tensor(now, dtype=T.int32))
+        if turn == 4:
+            table[1:5] = table[0]
+            tab.copy_(table)
+        graph.replay()
+        want, want_lse = call()
+        assert T.equal(out, want) and T.equal(lse, want_lse), turn
+        if turn in (3, 4):
+            few = slice(0, 6)
+            o, l, tol, lse_tol = ref.attend(q[few], data, table[few], now[few], page, bits)
+            seen = l > -float("inf")
+            assert ((out[few].cpu().double() - o).abs() <= tol).all()
+            assert T.equal(lse[few].cpu() > -float("inf"), seen)
+            assert ((lse[few].cpu().double() - l).abs() <= lse_tol)[seen].all()
+
+
 def test_two_streams_at_once(torch_cuda):
     # calls that overlap share no workspace
     T = torch_cuda
