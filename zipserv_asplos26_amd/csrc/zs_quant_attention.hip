@@ -20,12 +20,16 @@
 //   index 8*(l/16) + j stands for token 4*(l/16) + j%4 of tile j/4; lane l reads the
 //   l%16-th part of those eight rows, D / 16 channels of 8 tokens, which are D / 16 A
 //   operands.
-// A code's bits are an fp16 subnormal, which the matrix cores take as it is: an "and"
-// for two codes and a shift for four (8 bits of values: a byte permute for two).
-// What meets them has to be fp16 as well: q, times a power of two a column, and the weights
-// times s_v as two fp16 each, 22 bits, relative to the largest of them so far.  As
-// bf16, 16 + code by a shift and an and-or, with weights of three parts, a pair took
-// 231 and 290 vector instructions where it takes 207 and 260 (8 and 16 columns).
+// A key's code is an fp16 subnormal's bits, which the matrix cores take as they are: an
+// "and" for two codes and a shift for two.  What meets them is fp16 as well: q, times a
+// power of two a column.  A value's code is a bf16's bits in the same way (below 128 a
+// subnormal's, and above they go on in the same steps): an "and" for two codes and a shift
+// for four, or a byte permute for two.  They meet weights times s_v as three bf16 each, all
+// of their 24 bits, of a range that a bf16 has as well: a weight is relative to the largest
+// score alone, and the size of a value needs no reference of its own as long as it is an
+// ordinary one (kLeastScale, kMostValue).  A part of a sequence in which it is not is done
+// a second time, with a power of two for each value and a reference for weights times these
+// beside the one for weights.
 // With 8 columns or fewer the tile's other columns repeat them, and a lane does the softmax
 // of only a half of its tokens (4 or fewer: a quarter) and gets the other weights from
 // the lanes that did them.
@@ -63,8 +67,8 @@ struct QuantAttnParams {
   const int32_t* seqlens;
   uint16_t* out;  // [B][new][H][D]
   float* lse;     // [B][H][new] or null
-  float* ws_o;    // [slot][Hkv][columns of a KV head][D] (where sequences may be cut)
-  float* ws_ml;   // [slot][Hkv][columns][2]: maximum (log2 domain) and sum
+  float* ws_o;    // [slot][Hkv][columns of a KV head][D] (where sequences may be cut): results of the slots
+  float* ws_ml;   // [slot][Hkv][columns][2]: what weights are relative to (a power of two: its log2) and their sum
   int2* ws_plan;  // [B]: a sequence's first slot and its splits (where they go by the lengths)
   int num_blocks, width, page, heads, heads_k, group, new_tokens, columns, batch;
   int splits;           // of every sequence, or 0: by the lengths
@@ -77,16 +81,23 @@ struct QuantAttnParams {
 
 constexpr int kQaWaves = 4;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-// 2^-30: scales below count as this in what weights are relative to, or their sums could leave fp32.
-constexpr uint32_t kLeastScale = (127 - 30) << 23;
+// A column's largest weight so far is 2^64, or up to 2^68 before the reference moves.  A value
+// row is ordinary if its scale is 0 or 2^-30 .. 2^16 and its low 2^16 at most: sums of
+// 2^31 weights times such values stay below 2^124, and weight * scale times a code in
+// units of 2^kValueUnit is 2^-99 or more for the largest weight, 27 bits above the least
+// normal number.
+constexpr float kWeightTop = 64.f, kWeightLag = 4.f;
+constexpr uint32_t kLeastScale = (127 - 30) << 23, kMostValue = (127 + 16) << 23;
+// Where none of a column's sums of those products reaches this, its large weights all met
+// rows of scale 0, and what the others gave may be short of digits.
+constexpr float kLeastSum = 0x1p-100f;
 
 template <int D, int kBits>
 struct QaShape {
   static constexpr int kC = D / 32;               // steps of q.c
   static constexpr int kO = D / 16;               // tiles of channels of the output
   static constexpr int kKey = D * kBits / 128;    // dwords of a key row a lane takes
-  static constexpr int kState = (4 * kO + 2) * 64;  // floats of a wave's O, maximum and sum
+  static constexpr int kState = (4 * kO + 3) * 64;  // floats of a wave's O, references and sum
 };
 
 // N dwords from a place aligned to them (to 16 bytes).
@@ -144,9 +155,18 @@ __device__ __forceinline__ f16x8 query_operand(u32x4 in, float factor) {
   return y;
 }
 
+// Value codes as a bf16's bits: code c stands for c 2^-133, in nibbles 1 and 3 for 16 times as
+// much.
+constexpr int kValueUnit = -133;
+
+template <int i>
+__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w) {
+  return (i >= 2 ? w >> 8 : w) & (i % 2 ? 0x00F000F0u : 0x000F000Fu);
+}
+
 // A lane's parts of eight value rows, and the operand of output tile n from them, its
-// channel n of the eight tokens (the map from (part, n) to a channel is qa_channel), as
-// fp16 subnormals again, 16 times as large where sixteenfold(n).
+// channel n of the eight tokens (the map from (part, n) to a channel is qa_channel),
+// 16 times as large where sixteenfold(n).
 template <int D, int kBits>
 struct ValuePart;
 
@@ -158,12 +178,12 @@ struct ValuePart<128, 4> {
   }
   static constexpr bool sixteenfold(int n) { return n / 2 % 2; }
   template <int n>
-  __device__ __forceinline__ f16x8 operand() const {
+  __device__ __forceinline__ bf16x8 operand() const {
     u32x4 x;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      x[i] = nibbles_f16<n / 2>(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], n % 2 ? 0x07060302 : 0x05040100));
-    return __builtin_bit_cast(f16x8, x);
+      x[i] = nibbles_bf16<n / 2>(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], n % 2 ? 0x07060302 : 0x05040100));
+    return __builtin_bit_cast(bf16x8, x);
   }
 };
 
@@ -175,11 +195,11 @@ struct ValuePart<64, 4> {
   }
   static constexpr bool sixteenfold(int n) { return n % 2; }
   template <int n>
-  __device__ __forceinline__ f16x8 operand() const {
+  __device__ __forceinline__ bf16x8 operand() const {
     u32x4 x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = nibbles_f16<n>((uint32_t)w[2 * i] | (uint32_t)w[2 * i + 1] << 16);
-    return __builtin_bit_cast(f16x8, x);
+    for (int i = 0; i < 4; ++i) x[i] = nibbles_bf16<n>((uint32_t)w[2 * i] | (uint32_t)w[2 * i + 1] << 16);
+    return __builtin_bit_cast(bf16x8, x);
   }
 };
 
@@ -190,12 +210,12 @@ struct ValuePart<D, 8> {
   __device__ __forceinline__ void load(int j, const uint8_t* part) { load_words<kW>(part, w[j]); }
   static constexpr bool sixteenfold(int) { return false; }
   template <int n>
-  __device__ __forceinline__ f16x8 operand() const {
+  __device__ __forceinline__ bf16x8 operand() const {
     u32x4 x;  // byte n % 4 of both tokens, zeros above
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       x[i] = __builtin_amdgcn_perm(w[2 * i + 1][n / 4], w[2 * i][n / 4], 0x0C040C00u + 0x00010001u * (n % 4));
-    return __builtin_bit_cast(f16x8, x);
+    return __builtin_bit_cast(bf16x8, x);
   }
 };
 
@@ -246,10 +266,12 @@ __device__ __forceinline__ int qa_lane() {
 }
 
 // The waves' states of a tile of columns merged and written, two output tiles a wave: the
-// result, or what goes into a slot (slot >= 0).
-template <int D, int kBits, int kColumns>
+// result, or what goes into a slot (slot >= 0; O divided by the sum as well, so that
+// slots are alike whatever their weights were relative to).  kOdd: O and z are to be
+// multiplied by 2^(off_own - 128).
+template <int D, int kBits, int kColumns, bool kOdd>
 __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem, const f32x4* O, float m_own,
-                                          float l_own, float z, int ct, int h, int b, int slot) {
+                                          float l_own, float z, float off_own, int ct, int h, int b, int slot) {
   typedef QaShape<D, kBits> Shape;
   constexpr int kO = Shape::kO, W = kQaWaves;
   static_assert(W >= kO / 2, "");
@@ -259,25 +281,41 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
   for (int i = 0; i < kO; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      cb[(4 * i + r) * 64] = fmaf(O[i][r], (ValuePart<D, kBits>::sixteenfold(i) ? 0.0625f : 1.f) / kCodeUnit<kBits>, z);
+      cb[(4 * i + r) * 64] = ldexpf(O[i][r], (ValuePart<D, kBits>::sixteenfold(i) ? -4 : 0) - kValueUnit) + z;
   cb[4 * kO * 64] = m_own;
   cb[(4 * kO + 1) * 64] = l_own;
+  if constexpr (kOdd) cb[(4 * kO + 2) * 64] = off_own;
   __syncthreads();
   if (w >= kO / 2) return;
   const float* src = smem + l;
-  float m = -FLT_MAX, sum = 0.f, o[2][4] = {};
+  float m = -FLT_MAX, off = -FLT_MAX, sum = 0.f, o[2][4] = {};
 #pragma unroll
   for (int i = 0; i < W; ++i) m = fmaxf(m, src[i * Shape::kState + 4 * kO * 64]);
+  if constexpr (kOdd) {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      off = fmaxf(off, src[i * Shape::kState + (4 * kO + 2) * 64] + (src[i * Shape::kState + 4 * kO * 64] - m));
+  }
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    // (in two steps, as for a new maximum)
-    const float f = __builtin_amdgcn_exp2f(0.5f * (src[i * Shape::kState + 4 * kO * 64] - m));
-    sum += src[i * Shape::kState + (4 * kO + 1) * 64] * f * f;
+    const float less = src[i * Shape::kState + 4 * kO * 64] - m;
+    const float f = __builtin_amdgcn_exp2f(less);
+    float fo = f;
+    if constexpr (kOdd) fo = __builtin_amdgcn_exp2f(src[i * Shape::kState + (4 * kO + 2) * 64] + less - off);
+    sum += src[i * Shape::kState + (4 * kO + 1) * 64] * f;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[n][r] += src[i * Shape::kState + (4 * (2 * w + n) + r) * 64] * f * f;
+      for (int r = 0; r < 4; ++r) o[n][r] += src[i * Shape::kState + (4 * (2 * w + n) + r) * 64] * fo;
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      o[n][r] *= inv;
+      if constexpr (kOdd) o[n][r] = ldexpf(o[n][r], (int)fmaxf(off, -1000.f) - 128);
+    }
   const int column = kColumns * ct + (l & 15);
   if ((l & 15) >= kColumns || column >= p.columns) return;
   // neighbouring channels: (r, 0), (r, 1), or with two codes of a byte apart (2i, 0),
@@ -287,17 +325,16 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
   const int at = D / 4 * lg + (kFour ? 4 : 2) * w;
   const int fresh = (int)p.over_group.div((uint32_t)column), head = h * p.group + column - fresh * p.group;
   if (slot < 0) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     uint16_t* out = p.out + (((int64_t)b * p.new_tokens + fresh) * p.heads + head) * D + at;
     if constexpr (kFour) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<uint2*>(out + 8 * i) = uint2{pack_bf16x2(o[0][2 * i] * inv, o[0][2 * i + 1] * inv),
-                                                       pack_bf16x2(o[1][2 * i] * inv, o[1][2 * i + 1] * inv)};
+        *reinterpret_cast<uint2*>(out + 8 * i) = uint2{pack_bf16x2(o[0][2 * i], o[0][2 * i + 1]),
+                                                       pack_bf16x2(o[1][2 * i], o[1][2 * i + 1])};
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<uint32_t*>(out + D / 16 * r) = pack_bf16x2(o[0][r] * inv, o[1][r] * inv);
+        *reinterpret_cast<uint32_t*>(out + D / 16 * r) = pack_bf16x2(o[0][r], o[1][r]);
     }
     if (p.lse && lg == 0 && w == 0)
       p.lse[((int64_t)b * p.heads + head) * p.new_tokens + fresh] = natural_log_sum(m, sum);
@@ -357,6 +394,7 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
   __shared__ float smem[W * Shape::kState];
   __shared__ __attribute__((aligned(16))) f16x8 q_lds[kTiles][kC][64];  // (one tile's stays in registers)
   __shared__ float2 column_lds[kTiles][16];
+  __shared__ int odd_lds[W];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
   // Column tiles of the same tokens go to one XCD (workgroups are dealt out to the
   // eight in turn), one soon after another.
@@ -411,8 +449,11 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
     }
   }
 
-  // Tiles t0 .. t1 of sequence b, into its slot or as its result.
-  auto segment = [&](int len, int t0, int t1, int slot) {
+  // Tiles t0 .. t1 of sequence b, into its slot or as its result.  odd_tag: value rows may
+  // be of any size; without, whether one was not ordinary is returned (for the whole workgroup),
+  // and then nothing is written.
+  auto segment = [&](auto odd_tag, int len, int t0, int t1, int slot) {
+    constexpr bool kOdd = decltype(odd_tag)::value;
     const int l = qa_lane();
     const int g = l & 15, lg = l >> 4;
     const int fold = g / kColumns;
@@ -464,9 +505,9 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
       for (int j = 0; j < 8; ++j) x.v.load(j, vr[j / 4] + v_at + j % 4 * Row::kBytes);
     };
     const int pairs = t1 - t0 - 2 * w > 0 ? (t1 - t0 - 2 * w + 2 * W - 1) / (2 * W) : 0;  // of this wave
-    Pair pair[2];
+    Pair pair[kOdd ? 1 : 2];
     Place ahead[2];
-    if (pairs > 0) {
+    if (!kOdd && pairs > 0) {
       ahead[0] = places(0);
       ahead[1] = places(1);
       fetch(pair[0], ahead[0], 0);
@@ -530,14 +571,18 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
       }
     }
 
+    // l_run: sum of weights, weight * 2^-m_run; z: of weights * low_v.  kOdd: O and z are of
+    // weights * 2^-off_run, and of values times a power of two each.
     f32x4 O[kTiles][kO];
-    float m_run[kTiles], l_run[kTiles], z[kTiles];  // z: sum p low_v
+    float m_run[kTiles], l_run[kTiles], z[kTiles], off_run[kTiles];
+    uint64_t odd = 0, scaled = 0;  // lanes that met a value row that is not ordinary, one with a scale
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
       for (int k = 0; k < kO; ++k) O[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
       m_run[i] = -FLT_MAX;
       l_run[i] = z[i] = 0.f;
+      off_run[i] = -1000.f;
     }
     auto consume = [&](const Pair& x) {
       f32x4 S[kTiles][2] = {};
@@ -555,7 +600,7 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
           S[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K1, q, S[i][1], 0, 0, 0);
         }
       }
-      float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kTokens];
+      float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kOdd ? kTokens : 1];
 #pragma unroll
       for (int j = 0; j < kTokens; ++j) {
         const uint32_t kp = x.side[2 * j], vp = x.side[2 * j + 1];
@@ -563,12 +608,53 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
         kl[j] = __uint_as_float(kp & 0xFFFF0000u);
         vs[j] = __uint_as_float(vp << 16);
         vl[j] = __uint_as_float(vp & 0xFFFF0000u);
-        vs_log[j] = (float)max(vp << 16, kLeastScale);  // * 2^-23: log2 of the scale + 127, up to 0.09 less
+        if constexpr (kOdd) {
+          // The exponent field f of the scale or, if more, of low 2^-kBits; times 2^(128 - f) the
+          // scale is below 4 and low below 2^(kBits + 2).
+          const int size = max(max((int)(vp << 16 & 0x7FFF0000u), (int)(vp & 0x7FFF0000u) - (kBits << 23)), 1 << 23);
+          const float by = __uint_as_float((255u << 23) - (size & 0x7F800000u));
+          vs[j] *= by;
+          vl[j] *= by;
+          vs_log[j] = (float)(size >> 23);
+        }
       }
       // Behind a column's limit and where there is no page nothing counts, whatever it holds.
       const bool cut = x.none[0] || x.none[1] || first - 16 * x.tile < 32;  // (uniform)
-      constexpr int kWords = kTokens / 2;                                   // packed pairs of a lane's weights
-      f16x8 weights[kTiles][2];
+      if constexpr (!kOdd) {
+        // each lane looks at one of its tokens, the row's lanes at all
+        uint32_t vp[kTokens];
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) vp[j] = x.side[2 * j + 1];
+#pragma unroll
+        for (int n = kTokens / 2; n > 0; n /= 2)
+#pragma unroll
+          for (int j = 0; j < n; ++j) {
+            const uint32_t upper = vp[j + n], lower = vp[j];
+            vp[j] = g & n ? upper : lower;
+          }
+        const uint32_t scale = vp[0] << 16;
+        uint64_t met = __builtin_amdgcn_ballot_w64(scale - 1 < kLeastScale - 1 ||
+                                                   max(scale, vp[0] & 0x7FFF0000u) > kMostValue);
+        if (cut) {
+          const int j = g % kTokens, t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
+          met &= __builtin_amdgcn_ballot_w64(at < len - 16 * x.tile && !(t ? x.none[1] : x.none[0]));
+        }
+        odd |= met;
+        scaled |= __builtin_amdgcn_ballot_w64(scale != 0);
+      }
+      constexpr int kWords = kTokens / 2;  // packed pairs of a lane's weights
+      bf16x8 weights[kTiles][3];
+      auto products = [&](int i0, int i1) {
+        unrolled<0, kO>([&](auto n) {
+          constexpr int o = decltype(n)::value;
+          const bf16x8 A = x.v.template operand<o>();
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int i = i0; i < i1; ++i)
+              O[i][o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, weights[i][k], O[i][o], 0, 0, 0);
+        });
+      };
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
         float s[kTokens], vs_i[kTokens], vl_i[kTokens];
@@ -595,45 +681,66 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
             vl_i[j] = seen ? vl[j] : 0.f;
           }
         }
-        // What a weight is relative to: so that the largest product of a weight and a value's
-        // scale is 2^11..2^15.  Moved only where a product would be larger.
-        float mx = fmaf(vs_log[0], 0x1p-23f, s[0]);
+        // References are whole numbers, so that moving one changes exponents only, and are moved
+        // where a weight (kOdd: or one times a value's power of two) would be larger than it may.
+        auto column_max = [](float x) {
+          if constexpr (kFold >= 2) x = fmaxf(x, row_from8(x));
+          if constexpr (kFold == 4) x = fmaxf(x, row_from4(x));
+          return wave_max16(x);
+        };
+        float mx = s[0];
 #pragma unroll
-        for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, fmaf(vs_log[j], 0x1p-23f, s[j]));
-        mx -= 127.f + 11.f;
-        if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + 4.f)) {
-          if constexpr (kFold >= 2) mx = fmaxf(mx, row_from8(mx));
-          if constexpr (kFold == 4) mx = fmaxf(mx, row_from4(mx));
-          const float m_new = fmaxf(m_run[i], wave_max16(mx));
-          // (in two steps: scales can be 2^160 apart, and sums of small ones' weights as large)
-          const float alpha = __builtin_amdgcn_exp2f(0.5f * (m_run[i] - m_new));
-          m_run[i] = m_new;
-          l_run[i] = l_run[i] * alpha * alpha;
-          z[i] = z[i] * alpha * alpha;
+        for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, s[j]);
+        bool late = mx > m_run[i] + (kWeightTop + kWeightLag);
+        if constexpr (kOdd) {
 #pragma unroll
-          for (int k = 0; k < kO; ++k) O[i][k] = O[i][k] * alpha * alpha;
+          for (int j = 0; j < kTokens; ++j)
+            late = late || s[j] - m_run[i] + (vs_log[j] - off_run[i]) > kWeightTop + kWeightLag;
         }
-        // weights times scales as sums of two fp16: 22 bits, or 2^-25 where that is more
-        uint32_t own[2][kWords];
+        if (__builtin_amdgcn_ballot_w64(late)) {
+          const float m_new = fmaxf(m_run[i], ceilf(column_max(mx)) - kWeightTop);
+          const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
+          float beta = alpha;
+          l_run[i] *= alpha;
+          if constexpr (kOdd) {
+            float most = s[0] - m_new + vs_log[0];
+#pragma unroll
+            for (int j = 1; j < kTokens; ++j) most = fmaxf(most, s[j] - m_new + vs_log[j]);
+            const float old = off_run[i] + (m_run[i] - m_new);
+            off_run[i] = fmaxf(old, ceilf(column_max(most)) - kWeightTop);
+            beta = __builtin_amdgcn_exp2f(old - off_run[i]);
+          }
+          m_run[i] = m_new;
+          z[i] *= beta;
+#pragma unroll
+          for (int k = 0; k < kO; ++k) O[i][k] *= beta;
+        }
+        // Weights times scales as sums of three bf16, which is exact: the upper 8 of 24 bits, the
+        // upper 8 of the rest, and the rest of that.
+        uint32_t own[3][kWords];
 #pragma unroll
         for (int j = 0; j < kTokens; j += 2) {
-          float y[2];
+          uint32_t y[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float weight = __builtin_amdgcn_exp2f(s[j + e] - m_run[i]);
+            const float d = s[j + e] - m_run[i];
+            float weight = __builtin_amdgcn_exp2f(d);
             l_run[i] += weight;
+            if constexpr (kOdd) weight = __builtin_amdgcn_exp2f(d + (vs_log[j + e] - off_run[i]));
             z[i] = fmaf(weight, vl_i[j + e], z[i]);
-            y[e] = weight * vs_i[j + e];
+            y[e] = __float_as_uint(weight * vs_i[j + e]);
           }
-          const f16x2 a = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
-          const f32x2 rest = {fmaf((float)a[0], -1.f, y[0]), fmaf((float)a[1], -1.f, y[1])};
-          const f16x2 c = __builtin_convertvector(rest, f16x2);
-          own[0][j / 2] = __builtin_bit_cast(uint32_t, a);
-          own[1][j / 2] = __builtin_bit_cast(uint32_t, c);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            own[k][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              y[e] = __float_as_uint(__uint_as_float(y[e]) - __uint_as_float(y[e] & 0xFFFF0000u));
+          }
         }
         // the other folds' tokens of the column
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < 3; ++k) {
           u32x4 y;
           if constexpr (kFold == 1)
             y = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
@@ -641,40 +748,66 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
             y = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
           else
             y = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
-          weights[i][k] = __builtin_bit_cast(f16x8, y);
+          weights[i][k] = __builtin_bit_cast(bf16x8, y);
         }
+        if constexpr (kOdd) products(i, i + 1);
       }
-      unrolled<0, kO>([&](auto n) {
-        constexpr int o = decltype(n)::value;
-        const f16x8 A = x.v.template operand<o>();
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i)
-            O[i][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, weights[i][k], O[i][o], 0, 0, 0);
-      });
+      if constexpr (!kOdd) products(0, kTiles);
     };
 
     // A pair's loads go out while the one before is worked on, and its places are read one
     // pair earlier still.  (Past the last pair page 0 is read, so that the number of loads
     // on the way is known.)
-    for (int n = 0; n < pairs; n += 2) {
-      fetch(pair[1], ahead[1], n + 1);
-      ahead[0] = places(n + 2);
-      consume(pair[0]);
-      fetch(pair[0], ahead[0], n + 2);
-      ahead[1] = places(n + 3);
-      if (n + 1 < pairs) consume(pair[1]);
+    if constexpr (kOdd) {
+      for (int n = 0; n < pairs; ++n) {
+        fetch(pair[0], places(n), n);
+        consume(pair[0]);
+      }
+    } else {
+      for (int n = 0; n < pairs; n += 2) {
+        fetch(pair[1], ahead[1], n + 1);
+        ahead[0] = places(n + 2);
+        consume(pair[0]);
+        fetch(pair[0], ahead[0], n + 2);
+        ahead[1] = places(n + 3);
+        if (n + 1 < pairs) consume(pair[1]);
+      }
     }
 
+    auto column_sum = [](float x) {
+      x = wave_sum16(x);
+      if constexpr (kFold >= 2) x += row_from8(x);
+      if constexpr (kFold == 4) x += row_from4(x);
+      return x;
+    };
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) l_run[i] = column_sum(l_run[i]), z[i] = column_sum(z[i]);
+    if constexpr (!kOdd) {
+      if (scaled) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          float most = 0.f;
+#pragma unroll
+          for (int k = 0; k < kO; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) most = fmaxf(most, O[i][k][r]);
+          odd |= __builtin_amdgcn_ballot_w64(wave_max16(most) < kLeastSum && l_run[i] > 0.f);
+        }
+      }
+      if (qa_lane() == 0) odd_lds[w] = odd != 0;
+      __syncthreads();
+      int any = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) any |= odd_lds[i];
+      if (__builtin_amdgcn_readfirstlane(any)) return true;
+    }
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      float sum = wave_sum16(l_run[i]), rest = wave_sum16(z[i]);
-      if constexpr (kFold >= 2) sum += row_from8(sum), rest += row_from8(rest);
-      if constexpr (kFold == 4) sum += row_from4(sum), rest += row_from4(rest);
       if (i) __syncthreads();  // the last tile's states are read
-      qa_finish<D, kBits, kColumns>(p, smem, O[i], m_run[i], sum, rest, kTiles * ct + i, h, b, slot);
+      qa_finish<D, kBits, kColumns, kOdd>(p, smem, O[i], m_run[i], l_run[i], z[i], off_run[i], kTiles * ct + i, h, b,
+                                          slot);
     }
+    return false;
   };
 
   for (;;) {
@@ -688,7 +821,7 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
         p.ws_plan[b] = int2{slot, whole ? 1 : qa_part_of(start + tiles - 1, parts, total) + 1 - part};
       slot = whole ? -1 : slot;
     }
-    segment(max(len, 0), t0, t1, slot);
+    if (segment(std::false_type{}, max(len, 0), t0, t1, slot)) segment(std::true_type{}, max(len, 0), t0, t1, slot);
     start += tiles;
     if (++b >= p.batch || p.splits || (start >= to && part != parts - 1)) return;
     len = lens[b];

@@ -91,7 +91,7 @@ constexpr int kPartWaves = kPartMergeThreads / 64;
 template <int D, int kShare>
 __global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge p) {
   constexpr int kV = D / 64, kColumns = kPartWaves / kShare, kAtOnce = 8;
-  __shared__ float part[kPartWaves][D + 2];
+  __shared__ double part[kPartWaves][D + 2];
   const uint32_t bh = p.over_pieces.div(blockIdx.x), piece = blockIdx.x - bh * p.over_pieces.d;
   const uint32_t b = p.over_heads_k.div(bh), h = bh - b * p.over_heads_k.d;
   int first = b * p.splits, next = first + 1, step = 1, splits = p.splits;
@@ -108,9 +108,13 @@ __global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge 
   const bool live = column < p.columns;
   const int64_t rows = (int64_t)p.over_heads_k.d * p.columns, at = (int64_t)h * p.columns + column;
   auto slot = [&](int i) { return (i == 0 ? first : next + (i - 1) * step) * rows + at; };
-  float m_run = -FLT_MAX, sum = 0.f, acc[kV] = {};
+  // Sums in 64 bits: a sum of weights times a result that fits fp32 need not, and powers of two
+  // apart by any number of a split's are exact.
+  auto scaled = [](double x, float log2) { return ldexp(x, (int)fmaxf(log2, -4000.f)); };
+  float m_run = -FLT_MAX;
+  double sum = 0., acc[kV] = {};
   for (int c0 = share; live && c0 < splits; c0 += 64 * kShare) {
-    // 64 splits of this wave's: a lane's own maximum and sum, then their outputs
+    // 64 splits of this wave's: a lane's own reference and sum, then their results
     const int n = min((splits - c0 + kShare - 1) / kShare, 64);
     const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
     const float2 own = l < n ? ml[slot(c0 + l * kShare)] : float2{-FLT_MAX, 0.f};
@@ -128,20 +132,21 @@ __global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge 
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
     m = fmaxf(m, m_run);
-    // (weights in two steps: they can be as far apart as 2^-160, of sums as large)
-    const float alpha = __builtin_amdgcn_exp2f(0.5f * (m_run - m));
-    const float f = __builtin_amdgcn_exp2f(0.5f * (own.x - m));
-    m_run = m;
-    sum = sum * alpha * alpha + own.y * f * f;  // of this lane's splits (0 past the last)
+    const double f = scaled(own.y, own.x - m);
+    sum = scaled(sum, m_run - m) + f;  // of this lane's splits (0 past the last)
 #pragma unroll
-    for (int i = 0; i < kV; ++i) acc[i] = acc[i] * alpha * alpha;
+    for (int i = 0; i < kV; ++i) acc[i] = scaled(acc[i], m_run - m);
+    m_run = m;
+    const uint64_t bits = __builtin_bit_cast(uint64_t, f);
     for (int s0 = 0; s0 < n; s0 += kAtOnce) {
       if (s0) load(s0);
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j) {
-        const float g = s0 + j < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + j)) : 0.f;
+        const uint32_t lower = __builtin_amdgcn_readlane((uint32_t)bits, min(s0 + j, 63));
+        const uint32_t upper = __builtin_amdgcn_readlane((uint32_t)(bits >> 32), min(s0 + j, 63));
+        const double g = __builtin_bit_cast(double, (uint64_t)upper << 32 | lower);
 #pragma unroll
-        for (int i = 0; i < kV; ++i) acc[i] += s0 + j < n ? x[j][i] * g * g : 0.f;
+        for (int i = 0; i < kV; ++i) acc[i] = s0 + j < n ? fma((double)x[j][i], g, acc[i]) : acc[i];
       }
     }
   }
@@ -155,28 +160,28 @@ __global__ __launch_bounds__(kPartWaves * 64) void merge_parts_kernel(PartMerge 
     if (share != 0) return;
     float m = -FLT_MAX;
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) m = fmaxf(m, part[w + i][D]);
-    sum = 0.f;
+    for (int i = 0; i < kShare; ++i) m = fmaxf(m, (float)part[w + i][D]);
+    sum = 0.;
 #pragma unroll
-    for (int i = 0; i < kV; ++i) acc[i] = 0.f;
+    for (int i = 0; i < kV; ++i) acc[i] = 0.;
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {
-      const float f = __builtin_amdgcn_exp2f(0.5f * (part[w + i][D] - m));
-      sum += part[w + i][D + 1] * f * f;
+      const float less = (float)part[w + i][D] - m;
+      sum += scaled(part[w + i][D + 1], less);
 #pragma unroll
-      for (int j = 0; j < kV; ++j) acc[j] += part[w + i][kV * l + j] * f * f;
+      for (int j = 0; j < kV; ++j) acc[j] += scaled(part[w + i][kV * l + j], less);
     }
     m_run = m;
   }
   if (!live) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const double inv = sum == 0. ? 0. : 1. / sum;
   const int fresh = (int)p.over_group.div((uint32_t)column), group = (int)p.over_group.d;
   const int heads = group * (int)p.over_heads_k.d, head = h * group + column - fresh * group;
   uint16_t* out = p.out + (((int64_t)b * p.new_tokens + fresh) * heads + head) * D;
   if constexpr (kV == 2)
-    *reinterpret_cast<uint32_t*>(out + 2 * l) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    *reinterpret_cast<uint32_t*>(out + 2 * l) = pack_bf16x2((float)(acc[0] * inv), (float)(acc[1] * inv));
   else
-    out[l] = (uint16_t)pack_bf16x2(acc[0] * inv, 0.f);
+    out[l] = (uint16_t)pack_bf16x2((float)(acc[0] * inv), 0.f);
   if (p.lse && l == 0)
     p.lse[((int64_t)b * heads + head) * p.new_tokens + fresh] = natural_log_sum(m_run, sum);
 }

@@ -24,19 +24,20 @@ hipError_t merge_splits(hipStream_t stream, const SplitMerge& p, int head_dim);
 
 // ln(sum 2^m), -inf for no sum.  (The sum's exponent goes to m, in 64 bits, so that neither
 // the size of the sum nor that of m costs digits.)
-__device__ __forceinline__ float natural_log_sum(float m, float sum) {
-  const double log2 = ((double)m + __builtin_amdgcn_frexp_expf(sum)) + __log2f(__builtin_amdgcn_frexp_mantf(sum));
-  return sum == 0.f ? -INFINITY : (float)(log2 * 0.69314718055994530942);
+__device__ __forceinline__ float natural_log_sum(float m, double sum) {
+  const double log2 = ((double)m + __builtin_amdgcn_frexp_exp(sum)) + __log2f((float)__builtin_amdgcn_frexp_mant(sum));
+  return sum == 0. ? -INFINITY : (float)(log2 * 0.69314718055994530942);
 }
 
 // Slots of [heads_k][columns] rows, a column being new token * group + head of the
-// group; out is [sequence][new token][head][D], lse [sequence][head][new token].  A
+// group, a row the result over the slot's tokens and the sum of their weights, relative to
+// a power of two; out is [sequence][new token][head][D], lse [sequence][head][new token].  A
 // sequence's slots are b * splits and up, or with a plan, (first, number) a sequence,
 // the first and then first / 2 * 2 + 2, + 4, ...; a sequence of one is written already.
 struct PartMerge {
-  const float* ws_o;
-  const float* ws_ml;
-  const int2* plan;  // or null
+  const float* ws_o;   // [slot][row][D]
+  const float* ws_ml;  // [slot][row][2]: the power's log2 (-FLT_MAX for no weight), the sum
+  const int2* plan;    // or null
   uint16_t* out;
   float* lse;
   int splits, columns, new_tokens;
