@@ -11,7 +11,7 @@
 // A column is a (new token, query head) of one KV head's group; a workgroup of
 // kQaWaves waves takes up to 16 columns (of many: 32) and a part of the tokens, a wave 32
 // tokens (two tiles of 16) at a time, all in registers, with the next pair's loads on the way:
-//   S^T = C_k q^T with v_mfma_f32_16x16x32_f16: lane l holds D / 4 codes of token
+//   S^T = C_k q^T with v_mfma_f32_16x16x32_bf16: lane l holds D / 4 codes of token
 //   l%16 (channels D/4 * (l/16) and up, one piece of its row), 8 of them the A operand of a
 //   step; q^T (lane l: column l%16, the same channels) is the B operand.
 //   Online softmax in the log2 domain, fp32.
@@ -20,16 +20,15 @@
 //   index 8*(l/16) + j stands for token 4*(l/16) + j%4 of tile j/4; lane l reads the
 //   l%16-th part of those eight rows, D / 16 channels of 8 tokens, which are D / 16 A
 //   operands.
-// A key's code is an fp16 subnormal's bits, which the matrix cores take as they are: an
-// "and" for two codes and a shift for two.  What meets them is fp16 as well: q, times a
-// power of two a column.  A value's code is a bf16's bits in the same way (below 128 a
-// subnormal's, and above they go on in the same steps): an "and" for two codes and a shift
-// for four, or a byte permute for two.  They meet weights times s_v as three bf16 each, all
-// of their 24 bits, of a range that a bf16 has as well: a weight is relative to the largest
-// score alone, and the size of a value needs no reference of its own as long as it is an
-// ordinary one (kLeastScale, kMostValue).  A part of a sequence in which it is not is done
-// a second time, with a power of two for each value and a reference for weights times these
-// beside the one for weights.
+// A code is a bf16's bits, which the matrix cores take as they are: below 128 a subnormal's,
+// and above they go on in the same steps.  That takes an "and" for two codes and a
+// shift for four (8 bits of values: a byte permute for two).  What meets them is bf16 as well:
+// q itself, times a power of two a column, and the weights times s_v as three bf16 each, all
+// of their 24 bits.  A weight is relative to the largest score alone: the size of a value
+// needs no reference of its own as long as it is an ordinary one (kLeastScale,
+// kMostValue).  A part of a sequence in which it is not is done a second time, with a
+// power of two for each value and a reference for weights times these beside the one
+// for weights.
 // With 8 columns or fewer the tile's other columns repeat them, and a lane does the softmax
 // of only a half of its tokens (4 or fewer: a quarter) and gets the other weights from
 // the lanes that did them.
@@ -80,17 +79,19 @@ struct QuantAttnParams {
 };
 
 constexpr int kQaWaves = 4;
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-// A column's largest weight so far is 2^64, or up to 2^68 before the reference moves.  A value
-// row is ordinary if its scale is 0 or 2^-30 .. 2^16 and its low 2^16 at most: sums of
-// 2^31 weights times such values stay below 2^124, and weight * scale times a code in
-// units of 2^kValueUnit is 2^-99 or more for the largest weight, 27 bits above the least
-// normal number.
-constexpr float kWeightTop = 64.f, kWeightLag = 4.f;
+// A column's largest weight so far is 1, or up to 2^4 before the reference moves (small, so that
+// the argument of a weight's exponential has few digits before its point).  A value row is
+// ordinary if its scale is 0 or 2^-30 .. 2^16 and its low 2^16 at most.  Such a scale goes
+// in times 2^kScaleUp, so that weight * scale times a code in units of 2^kCodeUnit is 2^-64
+// or more for the largest weight, 62 bits above the least normal number, and sums of 2^31
+// of the largest stay below 2^35.
+constexpr float kWeightLag = 4.f;
+constexpr int kScaleUp = 100;
+constexpr float kScaleFactor = 0x1p100f;  // 2^kScaleUp
 constexpr uint32_t kLeastScale = (127 - 30) << 23, kMostValue = (127 + 16) << 23;
 // Where none of a column's sums of those products reaches this, its large weights all met
 // rows of scale 0, and what the others gave may be short of digits.
-constexpr float kLeastSum = 0x1p-100f;
+constexpr float kLeastSum = 0x1p-80f;
 
 template <int D, int kBits>
 struct QaShape {
@@ -110,58 +111,48 @@ __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* w) {
   for (int i = 0; i < N; ++i) w[i] = x[i];
 }
 
-// Codes as fp16 subnormals, whose bits are a multiple of 2^-24.  In 4 bits nibbles 0 and
-// 2 of a dword's halves come to bits 2..5 and nibbles 1 and 3 to bits 6..9, 4 and 64 times
-// the code; two shifts for four of them.  (The matrix cores line sums up by the
-// exponent that an operand could have, and a small subnormal's leading zeros are digits
-// lost: at bits 0..3 and 4..7, with one shift, scores are 2^-22 off, at these 2^-24.)
-template <int kBits>
-constexpr float kCodeUnit = kBits == 4 ? 0x1p-22f : 0x1p-24f;
+// Codes as a bf16's bits: code c stands for c 2^kCodeUnit, in nibbles 1 and 3 for 16 times as
+// much.  (The matrix cores line sums up by the exponent that an operand could have, and a
+// small subnormal's leading zeros are digits lost: 4-bit scores are 2^-24.7 of their
+// products' sizes off at most and 2^-28.5 on average here.  As fp16 subnormals at bits 0..3 and
+// 4..7 they were 2^-21.2 and 2^-23.8 off, at bits 2..5 and 6..9, with another shift, 2^-24.1 and
+// 2^-27.1.)
+constexpr int kCodeUnit = -133;
 
 template <int i>
-__device__ __forceinline__ uint32_t nibbles_f16(uint32_t w) {
-  const uint32_t x = i >= 2 ? w >> 6 : w << 2;
-  return x & (i % 2 ? 0x03C003C0u : 0x003C003Cu);
+__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w) {
+  return (i >= 2 ? w >> 8 : w) & (i % 2 ? 0x00F000F0u : 0x000F000Fu);
 }
 
 // Step c's operand from a lane's piece of a key row.  Nibbles 1 and 3 are 16 times as
 // large, and q is 1/16 there.
 template <int kBits>
-__device__ __forceinline__ f16x8 key_operand(const uint32_t* w, int c) {
+__device__ __forceinline__ bf16x8 key_operand(const uint32_t* w, int c) {
   u32x4 x;
   if constexpr (kBits == 4) {
-    x = u32x4{nibbles_f16<0>(w[c]), nibbles_f16<1>(w[c]), nibbles_f16<2>(w[c]), nibbles_f16<3>(w[c])};
+    x = u32x4{nibbles_bf16<0>(w[c]), nibbles_bf16<1>(w[c]), nibbles_bf16<2>(w[c]), nibbles_bf16<3>(w[c])};
   } else {
     const uint32_t u = w[2 * c], v = w[2 * c + 1];
     x = u32x4{u & 0x00FF00FFu, u >> 8 & 0x00FF00FFu, v & 0x00FF00FFu, v >> 8 & 0x00FF00FFu};
   }
-  return __builtin_bit_cast(f16x8, x);
+  return __builtin_bit_cast(bf16x8, x);
 }
 
-// The same channels of q, 8 bf16 times `factor` (a power of two), in the order and
-// with the factors of a key operand.
+// The same channels of q, 8 bf16 times 2^up (and by, 1 or -1), in the order and with the factors
+// of a key operand.
 template <int kBits>
-__device__ __forceinline__ f16x8 query_operand(u32x4 in, float factor) {
+__device__ __forceinline__ bf16x8 query_operand(u32x4 in, float by, int up) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(in[i] << 16) * factor;
-    x[2 * i + 1] = __uint_as_float(in[i] & 0xFFFF0000u) * factor;
+    x[2 * i] = ldexpf(__uint_as_float(in[i] << 16) * by, up);
+    x[2 * i + 1] = ldexpf(__uint_as_float(in[i] & 0xFFFF0000u) * by, up);
   }
-  f16x8 y;
+  bf16x8 y;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    y[i] = (_Float16)(kBits == 4 ? x[i] * (i & 2 ? 0.0625f : 1.f) : x[(i & 4) + (i & 1) * 2 + (i >> 1 & 1)]);
+    y[i] = (__bf16)(kBits == 4 ? x[i] * (i & 2 ? 0.0625f : 1.f) : x[(i & 4) + (i & 1) * 2 + (i >> 1 & 1)]);
   return y;
-}
-
-// Value codes as a bf16's bits: code c stands for c 2^-133, in nibbles 1 and 3 for 16 times as
-// much.
-constexpr int kValueUnit = -133;
-
-template <int i>
-__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w) {
-  return (i >= 2 ? w >> 8 : w) & (i % 2 ? 0x00F000F0u : 0x000F000Fu);
 }
 
 // A lane's parts of eight value rows, and the operand of output tile n from them, its
@@ -281,7 +272,7 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
   for (int i = 0; i < kO; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      cb[(4 * i + r) * 64] = ldexpf(O[i][r], (ValuePart<D, kBits>::sixteenfold(i) ? -4 : 0) - kValueUnit) + z;
+      cb[(4 * i + r) * 64] = ldexpf(O[i][r], (ValuePart<D, kBits>::sixteenfold(i) ? -4 : 0) - kCodeUnit - kScaleUp) + z;
   cb[4 * kO * 64] = m_own;
   cb[(4 * kO + 1) * 64] = l_own;
   if constexpr (kOdd) cb[(4 * kO + 2) * 64] = off_own;
@@ -392,7 +383,7 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
   constexpr int kColumns = 16 / kFold, kTokens = 8 / kFold;  // of a tile of columns; a lane's tokens of a pair
   typedef QaPair<D, kBits, kTokens> Pair;
   __shared__ float smem[W * Shape::kState];
-  __shared__ __attribute__((aligned(16))) f16x8 q_lds[kTiles][kC][64];  // (one tile's stays in registers)
+  __shared__ __attribute__((aligned(16))) bf16x8 q_lds[kTiles][kC][64];  // (one tile's stays in registers)
   __shared__ float2 column_lds[kTiles][16];
   __shared__ int odd_lds[W];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
@@ -514,14 +505,15 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
     }
 
     // This lane's column of a tile: new token `fresh` of head h * group + hh; it sees `limit`
-    // tokens.  q goes in as fp16, times a power of two that takes the largest of a
-    // column's to 2^14..2^15: of the others nothing above 2^-39 of that is lost.  Scores
-    // are kept without `unit`, which is left to do.
+    // tokens.  q goes in times a power of two that takes the largest of a column's to 2^117 or
+    // more, so that products with codes of units of 2^kCodeUnit are normal numbers, those of q
+    // 2^-100 of the largest among them, and s_k (q.c) is below 2^128 whatever s_k.  Scores are
+    // kept without `unit`, which is left to do.
     const int first = len - p.new_tokens + 1;
-    f16x8 Q[kTiles == 1 ? kC : 1];
-    float qs[kTiles], unit[kTiles];
+    bf16x8 Q[kTiles == 1 ? kC : 1];
+    float qs[kTiles], qs_rest[kTiles], unit[kTiles];
     int limit[kTiles];
-    auto query = [&](int i, f16x8* to, float& sum_q, float& unit_q) {
+    auto query = [&](int i, bf16x8* to, float& sum_q, float& unit_q) {
       const int column = min(kColumns * (kTiles * ct + i) + g % kColumns, p.columns - 1);
       const int fresh = (int)p.over_group.div((uint32_t)column), hh = column - fresh * p.group;
       const int64_t head = h * p.group + hh;
@@ -539,19 +531,18 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
         }
       }
       most = wave_max16(most);
-      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100);
-      const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+      const int e = (int)(__float_as_uint(most) >> 23) - 127;
 #pragma unroll
-      for (int c = 0; c < kC; ++c) to[c] = query_operand<kBits>(x[c], p.flip * up);
-      sum_q = wave_sum16(sum) * (p.flip * up * kCodeUnit<kBits>);
-      unit_q = p.scale_log2 * (__uint_as_float((uint32_t)(127 - 14 + e) << 23) / kCodeUnit<kBits>);
+      for (int c = 0; c < kC; ++c) to[c] = query_operand<kBits>(x[c], p.flip, 117 - e);
+      sum_q = ldexpf(wave_sum16(sum) * p.flip, 117 - e + kCodeUnit);
+      unit_q = ldexpf(p.scale_log2, e - 117 - kCodeUnit);
     };
     if constexpr (kTiles == 1) {
       query(0, Q, qs[0], unit[0]);
     } else {
       // wave i makes tile i's, for all of them
       if (w < kTiles) {
-        f16x8 mine_q[kC];
+        bf16x8 mine_q[kC];
         float2 x;
         query(w, mine_q, x.x, x.y);
 #pragma unroll
@@ -569,6 +560,11 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
         qs[i] = x.x;
         unit[i] = x.y;
       }
+      // (a low times 16 bits of sum q is exact, so what the two terms of a score cancel takes
+      // no digits of their products')
+      const float sum_q = qs[i];
+      qs[i] = __uint_as_float(__float_as_uint(sum_q) & 0xFFFFFF00u);
+      qs_rest[i] = sum_q - qs[i];
     }
 
     // l_run: sum of weights, weight * 2^-m_run; z: of weights * low_v.  kOdd: O and z are of
@@ -588,16 +584,16 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
       f32x4 S[kTiles][2] = {};
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
-        const f16x8 K0 = key_operand<kBits>(x.k[0], c), K1 = key_operand<kBits>(x.k[1], c);
+        const bf16x8 K0 = key_operand<kBits>(x.k[0], c), K1 = key_operand<kBits>(x.k[1], c);
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
-          f16x8 q;
+          bf16x8 q;
           if constexpr (kTiles == 1)
             q = Q[c];
           else
             q = q_lds[i][c][l];
-          S[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K0, q, S[i][0], 0, 0, 0);
-          S[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K1, q, S[i][1], 0, 0, 0);
+          S[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K0, q, S[i][0], 0, 0, 0);
+          S[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K1, q, S[i][1], 0, 0, 0);
         }
       }
       float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kOdd ? kTokens : 1];
@@ -608,12 +604,14 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
         kl[j] = __uint_as_float(kp & 0xFFFF0000u);
         vs[j] = __uint_as_float(vp << 16);
         vl[j] = __uint_as_float(vp & 0xFFFF0000u);
-        if constexpr (kOdd) {
+        if constexpr (!kOdd) {
+          vs[j] *= kScaleFactor;
+        } else {
           // The exponent field f of the scale or, if more, of low 2^-kBits; times 2^(128 - f) the
           // scale is below 4 and low below 2^(kBits + 2).
           const int size = max(max((int)(vp << 16 & 0x7FFF0000u), (int)(vp & 0x7FFF0000u) - (kBits << 23)), 1 << 23);
           const float by = __uint_as_float((255u << 23) - (size & 0x7F800000u));
-          vs[j] *= by;
+          vs[j] = vs[j] * by * kScaleFactor;
           vl[j] *= by;
           vs_log[j] = (float)(size >> 23);
         }
@@ -667,7 +665,7 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
             c = fold ? S[i][1][j] : S[i][0][j];
           else
             c = fold & 2 ? (fold & 1 ? S[i][1][2 + j] : S[i][1][j]) : (fold & 1 ? S[i][0][2 + j] : S[i][0][j]);
-          s[j] = fmaf(ks[j], c, kl[j] * qs[i]) * unit[i];
+          s[j] = fmaf(kl[j], qs_rest[i], fmaf(ks[j], c, kl[j] * qs[i])) * unit[i];
           vs_i[j] = vs[j];
           vl_i[j] = vl[j];
         }
@@ -691,14 +689,14 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
         float mx = s[0];
 #pragma unroll
         for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, s[j]);
-        bool late = mx > m_run[i] + (kWeightTop + kWeightLag);
+        bool late = mx > m_run[i] + kWeightLag;
         if constexpr (kOdd) {
 #pragma unroll
           for (int j = 0; j < kTokens; ++j)
-            late = late || s[j] - m_run[i] + (vs_log[j] - off_run[i]) > kWeightTop + kWeightLag;
+            late = late || s[j] - m_run[i] + (vs_log[j] - off_run[i]) > kWeightLag;
         }
         if (__builtin_amdgcn_ballot_w64(late)) {
-          const float m_new = fmaxf(m_run[i], ceilf(column_max(mx)) - kWeightTop);
+          const float m_new = fmaxf(m_run[i], ceilf(column_max(mx)));
           const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
           float beta = alpha;
           l_run[i] *= alpha;
@@ -707,7 +705,7 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
 #pragma unroll
             for (int j = 1; j < kTokens; ++j) most = fmaxf(most, s[j] - m_new + vs_log[j]);
             const float old = off_run[i] + (m_run[i] - m_new);
-            off_run[i] = fmaxf(old, ceilf(column_max(most)) - kWeightTop);
+            off_run[i] = fmaxf(old, ceilf(column_max(most)));
             beta = __builtin_amdgcn_exp2f(old - off_run[i]);
           }
           m_run[i] = m_new;
