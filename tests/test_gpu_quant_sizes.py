@@ -178,3 +178,40 @@ def test_weights_keep_their_digits(torch_cuda, group, new, dim, bits):
     out, lse = run(T, q, data, table, [3], page, bits, num_splits=1, softmax_scale=math.log(2))
     assert lse[0, :, -1].isfinite().all()
     assert (out[:, -1].abs() <= 2.0 ** -26).all(), float(out[:, -1].abs().max()) * 2 ** 26
+
+
+@pytest.mark.parametrize("kind", ["2^-50", "2^-48", "2^-47", "2^-46", "2^-44", "2^24", "2^26", "2^27", "2^28", "2^40", "flat106",
+                                  "flat110", "flat112", "flat113", "flat114"])
+@pytest.mark.parametrize("group,new,dim,bits", SHAPES)
+def test_value_rows_at_the_borders_of_a_second_pass(torch_cuda, group, new, dim, bits, kind):
+    # sums just within what one pass holds, and just past it; in some sequences, heads and parts only
+    T = torch_cuda
+    lens, page, width = [1100, 333, 64, 1], 16, 70
+    q, data, table, g = make(T, 37 + new, 4, new, 2 * group, 2, dim, page, width, bits)
+    ordinary = sides(data, page).copy()
+    values_of(T, kind, sides(data, page), bits, g)
+    keep = np.zeros(ordinary.shape[:3], dtype=bool)
+    keep[table[1].numpy()] = True
+    keep[:, 1] = True
+    keep[table[0, 20:50].numpy()] = True
+    sides(data, page)[keep] = ordinary[keep]
+    check(T, q, data, table, lens, page, bits)
+
+
+@pytest.mark.parametrize("group,new,dim,bits", SHAPES)
+def test_pools_without_a_value(torch_cuda, group, new, dim, bits):
+    # a pool of zeros, and one of rows without a scale
+    T = torch_cuda
+    lens, page, width = [1100, 333, 64, 0], 16, 70
+    q, data, table, g = make(T, 41, 4, new, 2 * group, 2, dim, page, width, bits)
+    side = sides(data, page)
+    side[..., 2] = 0
+    check(T, q, data, table, lens, page, bits)
+    data[:] = 0
+    for n in (1, 0, 5):
+        out, lse = run(T, q, data, table, lens, page, bits, num_splits=n)
+        assert (out == 0).all()
+        for i in range(new):
+            for b, length in enumerate(lens):
+                want = math.log(length - new + 1 + i) if length - new + 1 + i > 0 else -math.inf
+                assert (lse[b, :, i] == want).all() or (lse[b, :, i] - want).abs().max() <= 2.0 ** -22 * max(want, 1)

@@ -25,10 +25,9 @@
 // shift for four (8 bits of values: a byte permute for two).  What meets them is bf16 as well:
 // q itself, times a power of two a column, and the weights times s_v as three bf16 each, all
 // of their 24 bits.  A weight is relative to the largest score alone: the size of a value
-// needs no reference of its own as long as it is an ordinary one (kLeastScale,
-// kMostValue).  A part of a sequence in which it is not is done a second time, with a
-// power of two for each value and a reference for weights times these beside the one
-// for weights.
+// needs no reference of its own as long as the sums stay between kLeastSum and kMostSum.  A
+// part of a sequence where they do not is done a second time, with a power of two for each
+// value and a reference for weights times these beside the one for weights.
 // With 8 columns or fewer the tile's other columns repeat them, and a lane does the softmax
 // of only a half of its tokens (4 or fewer: a quarter) and gets the other weights from
 // the lanes that did them.
@@ -80,18 +79,18 @@ struct QuantAttnParams {
 
 constexpr int kQaWaves = 4;
 // A column's largest weight so far is 1, or up to 2^4 before the reference moves (small, so that
-// the argument of a weight's exponential has few digits before its point).  A value row is
-// ordinary if its scale is 0 or 2^-30 .. 2^16 and its low 2^16 at most.  Such a scale goes
-// in times 2^kScaleUp, so that weight * scale times a code in units of 2^kCodeUnit is 2^-64
-// or more for the largest weight, 62 bits above the least normal number, and sums of 2^31
-// of the largest stay below 2^35.
+// the argument of a weight's exponential has few digits before its point).  Scales of values go
+// in times 2^kScaleUp, so that weight * scale times a code in units of 2^kCodeUnit is
+// 2^-33 of what it stands for: 2^-63 for the largest weight and a scale of 2^-30, 63
+// bits above the least normal number, while scales up to 2^22 leave sums of 2^31 room.
 constexpr float kWeightLag = 4.f;
 constexpr int kScaleUp = 100;
 constexpr float kScaleFactor = 0x1p100f;  // 2^kScaleUp
-constexpr uint32_t kLeastScale = (127 - 30) << 23, kMostValue = (127 + 16) << 23;
-// Where none of a column's sums of those products reaches this, its large weights all met
-// rows of scale 0, and what the others gave may be short of digits.
-constexpr float kLeastSum = 0x1p-80f;
+constexpr float kSumFactor = 0x1p33f;  // 2^-(kCodeUnit + kScaleUp)
+// Whether that was enough is seen from a column's largest sum of such products: below the one
+// (small scales, or none with the large weights) digits may be lost, above the other (or
+// with a sum of lows above kSumFactor times that) a sum may have left fp32.
+constexpr float kLeastSum = 0x1p-80f, kMostSum = 0x1p80f;
 
 template <int D, int kBits>
 struct QaShape {
@@ -258,11 +257,11 @@ __device__ __forceinline__ int qa_lane() {
 
 // The waves' states of a tile of columns merged and written, two output tiles a wave: the
 // result, or what goes into a slot (slot >= 0; O divided by the sum as well, so that
-// slots are alike whatever their weights were relative to).  kOdd: O and z are to be
+// slots are alike whatever their weights were relative to).  kOdd: O is to be
 // multiplied by 2^(off_own - 128).
 template <int D, int kBits, int kColumns, bool kOdd>
 __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem, const f32x4* O, float m_own,
-                                          float l_own, float z, float off_own, int ct, int h, int b, int slot) {
+                                          float l_own, float off_own, int ct, int h, int b, int slot) {
   typedef QaShape<D, kBits> Shape;
   constexpr int kO = Shape::kO, W = kQaWaves;
   static_assert(W >= kO / 2, "");
@@ -272,7 +271,7 @@ __device__ __forceinline__ void qa_finish(const QuantAttnParams& p, float* smem,
   for (int i = 0; i < kO; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      cb[(4 * i + r) * 64] = ldexpf(O[i][r], (ValuePart<D, kBits>::sixteenfold(i) ? -4 : 0) - kCodeUnit - kScaleUp) + z;
+      cb[(4 * i + r) * 64] = O[i][r];
   cb[4 * kO * 64] = m_own;
   cb[(4 * kO + 1) * 64] = l_own;
   if constexpr (kOdd) cb[(4 * kO + 2) * 64] = off_own;
@@ -371,22 +370,414 @@ constexpr int qa_waves(int dim, int bits, int fold, int tiles) {
   return tiles > 1 || (dim == 128 && bits == 8 && fold < 4) ? 2 : 3;
 }
 
-// kTiles tiles of columns in one workgroup: codes are loaded and widened once for all.  With
-// more than one, q is read from LDS for each pair.
-template <int D, int kBits, int kFold, int kTiles>
-__global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) void quant_attn_kernel(
-    QuantAttnParams p) {
+// What a workgroup's waves share.
+template <int D, int kBits, int kTiles>
+struct QaShared {
+  float states[kQaWaves * QaShape<D, kBits>::kState];
+  __attribute__((aligned(16))) bf16x8 q[kTiles][QaShape<D, kBits>::kC][64];  // (one tile's stays in registers)
+  float2 column[kTiles][16];
+  int odd[kQaWaves];
+};
+
+// Tiles t0 .. t1 of sequence b, into its slot or as its result.  kOdd: value rows may be of any
+// size; without, whether sums say that some are too small or too large is returned (for the
+// whole workgroup), and then nothing is written.
+template <int D, int kBits, int kFold, int kTiles, bool kOdd>
+__device__ __forceinline__ bool qa_segment(const QuantAttnParams& p, QaShared<D, kBits, kTiles>& shared, int ct, int h,
+                                           int b, int len, int t0, int t1, int slot) {
   static_assert(kTiles == 1 || (kFold == 1 && kTiles <= kQaWaves), "");
   typedef QaShape<D, kBits> Shape;
   typedef QuantRow<D, kBits> Row;
   constexpr int kC = Shape::kC, kO = Shape::kO, W = kQaWaves;
   constexpr int kColumns = 16 / kFold, kTokens = 8 / kFold;  // of a tile of columns; a lane's tokens of a pair
   typedef QaPair<D, kBits, kTokens> Pair;
-  __shared__ float smem[W * Shape::kState];
-  __shared__ __attribute__((aligned(16))) bf16x8 q_lds[kTiles][kC][64];  // (one tile's stays in registers)
-  __shared__ float2 column_lds[kTiles][16];
-  __shared__ int odd_lds[W];
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l = qa_lane();
+  const int g = l & 15, lg = l >> 4;
+  const int fold = g / kColumns;
+  // the lane's tokens of a pair: kTokens from `token` of tile `mine` (all of both: 4 each)
+  const int mine = fold * 2 / kFold, token = 4 * lg + (kFold == 4 ? 2 * (fold & 1) : 0);
+  // Where the two tiles of the wave's n-th pair are: the table's entry and the tile in the
+  // page.  Scalar loads, which the many vector loads on the way do not have to be waited
+  // out for, and looked at only when the pair is fetched.
+  struct Place {
+    int block[2], sub[2];
+  };
+  const volatile auto* row = as_constant(p.table + b * p.table_stride);  // (volatile: or the loads move to their use)
+  auto places = [&](int n) {
+    Place x;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int tile = t0 + 2 * (w + W * n) + t;
+      const int lp = (int)p.tiles.div((uint32_t)min(tile, t1 - 1));
+      x.sub[t] = tile - lp * (int)p.tiles.d;
+      x.block[t] = row[lp];
+    }
+    return x;
+  };
+  const uint32_t k_at = g * Row::kBytes + 4 * Shape::kKey * lg, v_at = 4 * lg * Row::kBytes + Row::kBytes / 16 * g;
+  // The wave's n-th pair, on its way.  A tile without a page reads page 0.
+  auto fetch = [&](Pair& x, const Place& at, int n) {
+    x.tile = t0 + 2 * (w + W * n);
+    const uint8_t* kr[2];
+    const uint8_t* vr[2];
+    const uint8_t* sr[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x.none[t] = (uint32_t)at.block[t] >= (uint32_t)p.num_blocks || x.tile + t >= t1;
+      const int bl = x.none[t] ? 0 : at.block[t], su = x.none[t] ? 0 : at.sub[t];
+      // (scalar addresses, and a lane's own part in 32 bits)
+      const uint8_t* record = p.cache + ((int64_t)bl * p.heads_k + h) * p.record;
+      kr[t] = record + 8 * p.page + 16 * su * Row::kBytes;
+      vr[t] = kr[t] + p.page * Row::kBytes;
+      load_words<Shape::kKey>(kr[t] + k_at, x.k[t]);
+      sr[t] = record + 128 * su;
+    }
+    if constexpr (kFold == 1) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) load_words<8>(sr[t] + 32u * lg, x.side + 8 * t);
+    } else {
+      load_words<2 * kTokens>((mine ? sr[1] : sr[0]) + 8u * token, x.side);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.v.load(j, vr[j / 4] + v_at + j % 4 * Row::kBytes);
+  };
+  const int pairs = t1 - t0 - 2 * w > 0 ? (t1 - t0 - 2 * w + 2 * W - 1) / (2 * W) : 0;  // of this wave
+  Pair pair[kOdd ? 1 : 2];
+  Place ahead[2];
+  if (!kOdd && pairs > 0) {
+    ahead[0] = places(0);
+    ahead[1] = places(1);
+    fetch(pair[0], ahead[0], 0);
+  }
+
+  // This lane's column of a tile: new token `fresh` of head h * group + hh; it sees `limit`
+  // tokens.  q goes in times a power of two that takes the largest of a column's to 2^117 or
+  // more, so that products with codes of units of 2^kCodeUnit are normal numbers, those of q
+  // 2^-100 of the largest among them, and s_k (q.c) is below 2^128 whatever s_k.  Scores are
+  // kept without `unit`, which is left to do.
+  const int first = len - p.new_tokens + 1;
+  bf16x8 Q[kTiles == 1 ? kC : 1];
+  float qs[kTiles], qs_rest[kTiles], unit[kTiles];
+  int limit[kTiles];
+  auto query = [&](int i, bf16x8* to, float& sum_q, float& unit_q) {
+    const int column = min(kColumns * (kTiles * ct + i) + g % kColumns, p.columns - 1);
+    const int fresh = (int)p.over_group.div((uint32_t)column), hh = column - fresh * p.group;
+    const int64_t head = h * p.group + hh;
+    const uint16_t* row = p.q + b * p.q_batch + fresh * p.q_token + head * p.q_head + D / 4 * lg;
+    u32x4 x[kC];
+    float sum = 0.f, most = 0.f;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      x[c] = *reinterpret_cast<const u32x4*>(row + 8 * c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float u = __uint_as_float(x[c][j] << 16), v = __uint_as_float(x[c][j] & 0xFFFF0000u);
+        sum += u + v;
+        most = fmaxf(most, fmaxf(fabsf(u), fabsf(v)));
+      }
+    }
+    most = wave_max16(most);
+    const int e = (int)(__float_as_uint(most) >> 23) - 127;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) to[c] = query_operand<kBits>(x[c], p.flip, 117 - e);
+    sum_q = ldexpf(wave_sum16(sum) * p.flip, 117 - e + kCodeUnit);
+    unit_q = ldexpf(p.scale_log2, e - 117 - kCodeUnit);
+  };
+  if constexpr (kTiles == 1) {
+    query(0, Q, qs[0], unit[0]);
+  } else {
+    // wave i makes tile i's, for all of them
+    if (w < kTiles) {
+      bf16x8 mine_q[kC];
+      float2 x;
+      query(w, mine_q, x.x, x.y);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) shared.q[w][c][l] = mine_q[c];
+      if (lg == 0) shared.column[w][g] = x;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    const int column = min(kColumns * (kTiles * ct + i) + g % kColumns, p.columns - 1);
+    limit[i] = first + (int)p.over_group.div((uint32_t)column);
+    if constexpr (kTiles > 1) {
+      const float2 x = shared.column[i][g];
+      qs[i] = x.x;
+      unit[i] = x.y;
+    }
+    // (a low times 16 bits of sum q is exact, so what the two terms of a score cancel takes
+    // no digits of their products')
+    const float sum_q = qs[i];
+    qs[i] = __uint_as_float(__float_as_uint(sum_q) & 0xFFFFFF00u);
+    qs_rest[i] = sum_q - qs[i];
+  }
+
+  // l_run: sum of weights, weight * 2^-m_run; z: of weights * low_v.  kOdd: O and z are of
+  // weights * 2^-off_run, and of values times a power of two each.
+  f32x4 O[kTiles][kO];
+  float m_run[kTiles], l_run[kTiles], z[kTiles], off_run[kTiles];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+    for (int k = 0; k < kO; ++k) O[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m_run[i] = -FLT_MAX;
+    l_run[i] = z[i] = 0.f;
+    off_run[i] = -1000.f;
+  }
+  auto consume = [&](const Pair& x) {
+    f32x4 S[kTiles][2] = {};
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const bf16x8 K0 = key_operand<kBits>(x.k[0], c), K1 = key_operand<kBits>(x.k[1], c);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        bf16x8 q;
+        if constexpr (kTiles == 1)
+          q = Q[c];
+        else
+          q = shared.q[i][c][l];
+        S[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K0, q, S[i][0], 0, 0, 0);
+        S[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K1, q, S[i][1], 0, 0, 0);
+      }
+    }
+    float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kOdd ? kTokens : 1];
+#pragma unroll
+    for (int j = 0; j < kTokens; ++j) {
+      const uint32_t kp = x.side[2 * j], vp = x.side[2 * j + 1];
+      ks[j] = __uint_as_float(kp << 16);
+      kl[j] = __uint_as_float(kp & 0xFFFF0000u);
+      vs[j] = __uint_as_float(vp << 16);
+      vl[j] = __uint_as_float(vp & 0xFFFF0000u);
+      if constexpr (!kOdd) {
+        vs[j] *= kScaleFactor;
+      } else {
+        // The exponent field f of the scale or, if more, of low 2^-kBits; times 2^(128 - f) the
+        // scale is below 4 and low below 2^(kBits + 2).
+        const int size = max(max((int)(vp << 16 & 0x7FFF0000u), (int)(vp & 0x7FFF0000u) - (kBits << 23)), 1 << 23);
+        const float by = __uint_as_float((255u << 23) - (size & 0x7F800000u));
+        vs[j] = vs[j] * by * kScaleFactor;
+        vl[j] *= by;
+        vs_log[j] = (float)(size >> 23);
+      }
+    }
+    // Behind a column's limit and where there is no page nothing counts, whatever it holds.
+    const bool cut = x.none[0] || x.none[1] || first - 16 * x.tile < 32;  // (uniform)
+    constexpr int kWords = kTokens / 2;  // packed pairs of a lane's weights
+    bf16x8 weights[kTiles][3];
+    auto products = [&](int i0, int i1) {
+      unrolled<0, kO>([&](auto n) {
+        constexpr int o = decltype(n)::value;
+        const bf16x8 A = x.v.template operand<o>();
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+          for (int i = i0; i < i1; ++i)
+            O[i][o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, weights[i][k], O[i][o], 0, 0, 0);
+      });
+    };
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      float s[kTokens], vs_i[kTokens], vl_i[kTokens];
+#pragma unroll
+      for (int j = 0; j < kTokens; ++j) {
+        float c;
+        if constexpr (kFold == 1)
+          c = S[i][j / 4][j % 4];
+        else if constexpr (kFold == 2)
+          c = fold ? S[i][1][j] : S[i][0][j];
+        else
+          c = fold & 2 ? (fold & 1 ? S[i][1][2 + j] : S[i][1][j]) : (fold & 1 ? S[i][0][2 + j] : S[i][0][j]);
+        s[j] = fmaf(kl[j], qs_rest[i], fmaf(ks[j], c, kl[j] * qs[i])) * unit[i];
+        vs_i[j] = vs[j];
+        vl_i[j] = vl[j];
+      }
+      if (cut) {
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+          const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
+          const bool seen = at < limit[i] - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
+          s[j] = seen ? s[j] : -INFINITY;
+          vs_i[j] = seen ? vs[j] : 0.f;
+          vl_i[j] = seen ? vl[j] : 0.f;
+        }
+      }
+      // References are whole numbers, so that moving one changes exponents only, and are moved
+      // where a weight (kOdd: or one times a value's power of two) would be larger than it may.
+      auto column_max = [](float x) {
+        if constexpr (kFold >= 2) x = fmaxf(x, row_from8(x));
+        if constexpr (kFold == 4) x = fmaxf(x, row_from4(x));
+        return wave_max16(x);
+      };
+      float mx = s[0];
+#pragma unroll
+      for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, s[j]);
+      bool late = mx > m_run[i] + kWeightLag;
+      if constexpr (kOdd) {
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j)
+          late = late || s[j] - m_run[i] + (vs_log[j] - off_run[i]) > kWeightLag;
+      }
+      if (__builtin_amdgcn_ballot_w64(late)) {
+        const float m_new = fmaxf(m_run[i], ceilf(column_max(mx)));
+        const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
+        float beta = alpha;
+        l_run[i] *= alpha;
+        if constexpr (kOdd) {
+          float most = s[0] - m_new + vs_log[0];
+#pragma unroll
+          for (int j = 1; j < kTokens; ++j) most = fmaxf(most, s[j] - m_new + vs_log[j]);
+          const float old = off_run[i] + (m_run[i] - m_new);
+          off_run[i] = fmaxf(old, ceilf(column_max(most)));
+          beta = __builtin_amdgcn_exp2f(old - off_run[i]);
+        }
+        m_run[i] = m_new;
+        z[i] *= beta;
+#pragma unroll
+        for (int k = 0; k < kO; ++k) O[i][k] *= beta;
+      }
+      // Weights times scales as sums of three bf16, which is exact: the upper 8 of 24 bits, the
+      // upper 8 of the rest, and the rest of that.
+      uint32_t own[3][kWords];
+#pragma unroll
+      for (int j = 0; j < kTokens; j += 2) {
+        uint32_t y[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float d = s[j + e] - m_run[i];
+          float weight = __builtin_amdgcn_exp2f(d);
+          l_run[i] += weight;
+          if constexpr (kOdd) weight = __builtin_amdgcn_exp2f(d + (vs_log[j + e] - off_run[i]));
+          z[i] = fmaf(weight, vl_i[j + e], z[i]);
+          y[e] = __float_as_uint(weight * vs_i[j + e]);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          own[k][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            y[e] = __float_as_uint(__uint_as_float(y[e]) - __uint_as_float(y[e] & 0xFFFF0000u));
+        }
+      }
+      // the other folds' tokens of the column
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        u32x4 y;
+        if constexpr (kFold == 1)
+          y = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
+        else if constexpr (kFold == 2)
+          y = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
+        else
+          y = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
+        weights[i][k] = __builtin_bit_cast(bf16x8, y);
+      }
+      if constexpr (kOdd) products(i, i + 1);
+    }
+    if constexpr (!kOdd) products(0, kTiles);
+  };
+
+  // A pair's loads go out while the one before is worked on, and its places are read one
+  // pair earlier still.  (Past the last pair page 0 is read, so that the number of loads
+  // on the way is known.)
+  if constexpr (kOdd) {
+    for (int n = 0; n < pairs; ++n) {
+      fetch(pair[0], places(n), n);
+      consume(pair[0]);
+    }
+  } else {
+    for (int n = 0; n < pairs; n += 2) {
+      fetch(pair[1], ahead[1], n + 1);
+      ahead[0] = places(n + 2);
+      consume(pair[0]);
+      fetch(pair[0], ahead[0], n + 2);
+      ahead[1] = places(n + 3);
+      if (n + 1 < pairs) consume(pair[1]);
+    }
+  }
+
+  auto column_sum = [](float x) {
+    x = wave_sum16(x);
+    if constexpr (kFold >= 2) x += row_from8(x);
+    if constexpr (kFold == 4) x += row_from4(x);
+    return x;
+  };
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) l_run[i] = column_sum(l_run[i]), z[i] = column_sum(z[i]);
+  bool small = false, large = false;
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    // (fmaxf passes over what is no number: where a sum of a column is that, another of it is
+    // infinite, or all are and the largest is 0)
+    float most = 0.f;
+#pragma unroll
+    for (int k = 0; k < kO; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        most = fmaxf(most, O[i][k][r]);
+        O[i][k][r] = fmaf(O[i][k][r], ValuePart<D, kBits>::sixteenfold(k) ? kSumFactor / 16 : kSumFactor, z[i]);
+      }
+    most = wave_max16(most);
+    small = small || (most < kLeastSum && l_run[i] > 0.f);
+    large = large || !(most <= kMostSum && fabsf(z[i]) <= kMostSum * kSumFactor);
+  }
+  if constexpr (!kOdd) {
+    uint64_t odd = __builtin_amdgcn_ballot_w64(large);
+    if (!odd && __builtin_amdgcn_ballot_w64(small)) {
+      // not where no row has a scale (a cache of zeros)
+      for (int n = 0; n < pairs && !odd; ++n) {
+        const Place at = places(n);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (t0 + 2 * (w + W * n) + t >= t1 || (uint32_t)at.block[t] >= (uint32_t)p.num_blocks) continue;
+          const uint8_t* record = p.cache + ((int64_t)at.block[t] * p.heads_k + h) * p.record;
+          odd |= __builtin_amdgcn_ballot_w64(
+              *reinterpret_cast<const uint16_t*>(record + 128 * at.sub[t] + 8 * (qa_lane() & 15) + 4) != 0);
+        }
+      }
+    }
+    if (qa_lane() == 0) shared.odd[w] = odd != 0;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) any |= shared.odd[i];
+    if (__builtin_amdgcn_readfirstlane(any)) return true;
+  }
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    if (i) __syncthreads();  // the last tile's states are read
+    qa_finish<D, kBits, kColumns, kOdd>(p, shared.states, O[i], m_run[i], l_run[i], off_run[i], kTiles * ct + i, h, b, slot);
+  }
+  return false;
+}
+
+// Whether the second time is a function of its own.  Where both together need more registers than
+// there are it is the main loop that loses them; where not, a call's rules cost more.
+constexpr bool qa_calls(int dim, int bits, int fold, int tiles) {
+  return dim == 128 && (tiles > 1 || (bits == 4 && fold <= 2));
+}
+// (Addresses as numbers: of the kernel's arguments and in the workgroup's memory, so
+// that both are read as what they are.)
+template <int D, int kBits, int kFold, int kTiles>
+__device__ __attribute__((noinline)) void qa_segment_odd(uint64_t params, uint32_t shared, int ct, int h, int b,
+                                                         int len, int t0, int t1, int slot) {
+  typedef const QuantAttnParams __attribute__((address_space(4))) * Params;
+  typedef QaShared<D, kBits, kTiles> __attribute__((address_space(3))) * Shared;
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const uint64_t at = (uint64_t)(uint32_t)uniform((int)(params >> 32)) << 32 | (uint32_t)uniform((int)params);
+  qa_segment<D, kBits, kFold, kTiles, true>(*(const QuantAttnParams*)(Params)at,
+                                            *(QaShared<D, kBits, kTiles>*)(Shared)(uintptr_t)uniform(shared), uniform(ct),
+                                            uniform(h), uniform(b), uniform(len), uniform(t0), uniform(t1),
+                                            uniform(slot));
+}
+
+// kTiles tiles of columns in one workgroup: codes are loaded and widened once for all.  With
+// more than one, q is read from LDS for each pair.
+template <int D, int kBits, int kFold, int kTiles>
+__global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) void quant_attn_kernel(
+    QuantAttnParams p) {
+  __shared__ QaShared<D, kBits, kTiles> shared;
+  const int l = lane_id();
   // Column tiles of the same tokens go to one XCD (workgroups are dealt out to the
   // eight in turn), one soon after another.
   const int item = (int)p.over_column_tiles.div(blockIdx.x >> 3);
@@ -440,374 +831,6 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
     }
   }
 
-  // Tiles t0 .. t1 of sequence b, into its slot or as its result.  odd_tag: value rows may
-  // be of any size; without, whether one was not ordinary is returned (for the whole workgroup),
-  // and then nothing is written.
-  auto segment = [&](auto odd_tag, int len, int t0, int t1, int slot) {
-    constexpr bool kOdd = decltype(odd_tag)::value;
-    const int l = qa_lane();
-    const int g = l & 15, lg = l >> 4;
-    const int fold = g / kColumns;
-    // the lane's tokens of a pair: kTokens from `token` of tile `mine` (all of both: 4 each)
-    const int mine = fold * 2 / kFold, token = 4 * lg + (kFold == 4 ? 2 * (fold & 1) : 0);
-    // Where the two tiles of the wave's n-th pair are: the table's entry and the tile in the
-    // page.  Scalar loads, which the many vector loads on the way do not have to be waited
-    // out for, and looked at only when the pair is fetched.
-    struct Place {
-      int block[2], sub[2];
-    };
-    const volatile auto* row = as_constant(p.table + b * p.table_stride);  // (volatile: or the loads move to their use)
-    auto places = [&](int n) {
-      Place x;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int tile = t0 + 2 * (w + W * n) + t;
-        const int lp = (int)p.tiles.div((uint32_t)min(tile, t1 - 1));
-        x.sub[t] = tile - lp * (int)p.tiles.d;
-        x.block[t] = row[lp];
-      }
-      return x;
-    };
-    const uint32_t k_at = g * Row::kBytes + 4 * Shape::kKey * lg, v_at = 4 * lg * Row::kBytes + Row::kBytes / 16 * g;
-    // The wave's n-th pair, on its way.  A tile without a page reads page 0.
-    auto fetch = [&](Pair& x, const Place& at, int n) {
-      x.tile = t0 + 2 * (w + W * n);
-      const uint8_t* kr[2];
-      const uint8_t* vr[2];
-      const uint8_t* sr[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        x.none[t] = (uint32_t)at.block[t] >= (uint32_t)p.num_blocks || x.tile + t >= t1;
-        const int bl = x.none[t] ? 0 : at.block[t], su = x.none[t] ? 0 : at.sub[t];
-        // (scalar addresses, and a lane's own part in 32 bits)
-        const uint8_t* record = p.cache + ((int64_t)bl * p.heads_k + h) * p.record;
-        kr[t] = record + 8 * p.page + 16 * su * Row::kBytes;
-        vr[t] = kr[t] + p.page * Row::kBytes;
-        load_words<Shape::kKey>(kr[t] + k_at, x.k[t]);
-        sr[t] = record + 128 * su;
-      }
-      if constexpr (kFold == 1) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) load_words<8>(sr[t] + 32u * lg, x.side + 8 * t);
-      } else {
-        load_words<2 * kTokens>((mine ? sr[1] : sr[0]) + 8u * token, x.side);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x.v.load(j, vr[j / 4] + v_at + j % 4 * Row::kBytes);
-    };
-    const int pairs = t1 - t0 - 2 * w > 0 ? (t1 - t0 - 2 * w + 2 * W - 1) / (2 * W) : 0;  // of this wave
-    Pair pair[kOdd ? 1 : 2];
-    Place ahead[2];
-    if (!kOdd && pairs > 0) {
-      ahead[0] = places(0);
-      ahead[1] = places(1);
-      fetch(pair[0], ahead[0], 0);
-    }
-
-    // This lane's column of a tile: new token `fresh` of head h * group + hh; it sees `limit`
-    // tokens.  q goes in times a power of two that takes the largest of a column's to 2^117 or
-    // more, so that products with codes of units of 2^kCodeUnit are normal numbers, those of q
-    // 2^-100 of the largest among them, and s_k (q.c) is below 2^128 whatever s_k.  Scores are
-    // kept without `unit`, which is left to do.
-    const int first = len - p.new_tokens + 1;
-    bf16x8 Q[kTiles == 1 ? kC : 1];
-    float qs[kTiles], qs_rest[kTiles], unit[kTiles];
-    int limit[kTiles];
-    auto query = [&](int i, bf16x8* to, float& sum_q, float& unit_q) {
-      const int column = min(kColumns * (kTiles * ct + i) + g % kColumns, p.columns - 1);
-      const int fresh = (int)p.over_group.div((uint32_t)column), hh = column - fresh * p.group;
-      const int64_t head = h * p.group + hh;
-      const uint16_t* row = p.q + b * p.q_batch + fresh * p.q_token + head * p.q_head + D / 4 * lg;
-      u32x4 x[kC];
-      float sum = 0.f, most = 0.f;
-#pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        x[c] = *reinterpret_cast<const u32x4*>(row + 8 * c);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float u = __uint_as_float(x[c][j] << 16), v = __uint_as_float(x[c][j] & 0xFFFF0000u);
-          sum += u + v;
-          most = fmaxf(most, fmaxf(fabsf(u), fabsf(v)));
-        }
-      }
-      most = wave_max16(most);
-      const int e = (int)(__float_as_uint(most) >> 23) - 127;
-#pragma unroll
-      for (int c = 0; c < kC; ++c) to[c] = query_operand<kBits>(x[c], p.flip, 117 - e);
-      sum_q = ldexpf(wave_sum16(sum) * p.flip, 117 - e + kCodeUnit);
-      unit_q = ldexpf(p.scale_log2, e - 117 - kCodeUnit);
-    };
-    if constexpr (kTiles == 1) {
-      query(0, Q, qs[0], unit[0]);
-    } else {
-      // wave i makes tile i's, for all of them
-      if (w < kTiles) {
-        bf16x8 mine_q[kC];
-        float2 x;
-        query(w, mine_q, x.x, x.y);
-#pragma unroll
-        for (int c = 0; c < kC; ++c) q_lds[w][c][l] = mine_q[c];
-        if (lg == 0) column_lds[w][g] = x;
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-      const int column = min(kColumns * (kTiles * ct + i) + g % kColumns, p.columns - 1);
-      limit[i] = first + (int)p.over_group.div((uint32_t)column);
-      if constexpr (kTiles > 1) {
-        const float2 x = column_lds[i][g];
-        qs[i] = x.x;
-        unit[i] = x.y;
-      }
-      // (a low times 16 bits of sum q is exact, so what the two terms of a score cancel takes
-      // no digits of their products')
-      const float sum_q = qs[i];
-      qs[i] = __uint_as_float(__float_as_uint(sum_q) & 0xFFFFFF00u);
-      qs_rest[i] = sum_q - qs[i];
-    }
-
-    // l_run: sum of weights, weight * 2^-m_run; z: of weights * low_v.  kOdd: O and z are of
-    // weights * 2^-off_run, and of values times a power of two each.
-    f32x4 O[kTiles][kO];
-    float m_run[kTiles], l_run[kTiles], z[kTiles], off_run[kTiles];
-    uint64_t odd = 0, scaled = 0;  // lanes that met a value row that is not ordinary, one with a scale
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-#pragma unroll
-      for (int k = 0; k < kO; ++k) O[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-      m_run[i] = -FLT_MAX;
-      l_run[i] = z[i] = 0.f;
-      off_run[i] = -1000.f;
-    }
-    auto consume = [&](const Pair& x) {
-      f32x4 S[kTiles][2] = {};
-#pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        const bf16x8 K0 = key_operand<kBits>(x.k[0], c), K1 = key_operand<kBits>(x.k[1], c);
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          bf16x8 q;
-          if constexpr (kTiles == 1)
-            q = Q[c];
-          else
-            q = q_lds[i][c][l];
-          S[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K0, q, S[i][0], 0, 0, 0);
-          S[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K1, q, S[i][1], 0, 0, 0);
-        }
-      }
-      float ks[kTokens], kl[kTokens], vs[kTokens], vl[kTokens], vs_log[kOdd ? kTokens : 1];
-#pragma unroll
-      for (int j = 0; j < kTokens; ++j) {
-        const uint32_t kp = x.side[2 * j], vp = x.side[2 * j + 1];
-        ks[j] = __uint_as_float(kp << 16);
-        kl[j] = __uint_as_float(kp & 0xFFFF0000u);
-        vs[j] = __uint_as_float(vp << 16);
-        vl[j] = __uint_as_float(vp & 0xFFFF0000u);
-        if constexpr (!kOdd) {
-          vs[j] *= kScaleFactor;
-        } else {
-          // The exponent field f of the scale or, if more, of low 2^-kBits; times 2^(128 - f) the
-          // scale is below 4 and low below 2^(kBits + 2).
-          const int size = max(max((int)(vp << 16 & 0x7FFF0000u), (int)(vp & 0x7FFF0000u) - (kBits << 23)), 1 << 23);
-          const float by = __uint_as_float((255u << 23) - (size & 0x7F800000u));
-          vs[j] = vs[j] * by * kScaleFactor;
-          vl[j] *= by;
-          vs_log[j] = (float)(size >> 23);
-        }
-      }
-      // Behind a column's limit and where there is no page nothing counts, whatever it holds.
-      const bool cut = x.none[0] || x.none[1] || first - 16 * x.tile < 32;  // (uniform)
-      if constexpr (!kOdd) {
-        // each lane looks at one of its tokens, the row's lanes at all
-        uint32_t vp[kTokens];
-#pragma unroll
-        for (int j = 0; j < kTokens; ++j) vp[j] = x.side[2 * j + 1];
-#pragma unroll
-        for (int n = kTokens / 2; n > 0; n /= 2)
-#pragma unroll
-          for (int j = 0; j < n; ++j) {
-            const uint32_t upper = vp[j + n], lower = vp[j];
-            vp[j] = g & n ? upper : lower;
-          }
-        const uint32_t scale = vp[0] << 16;
-        uint64_t met = __builtin_amdgcn_ballot_w64(scale - 1 < kLeastScale - 1 ||
-                                                   max(scale, vp[0] & 0x7FFF0000u) > kMostValue);
-        if (cut) {
-          const int j = g % kTokens, t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
-          met &= __builtin_amdgcn_ballot_w64(at < len - 16 * x.tile && !(t ? x.none[1] : x.none[0]));
-        }
-        odd |= met;
-        scaled |= __builtin_amdgcn_ballot_w64(scale != 0);
-      }
-      constexpr int kWords = kTokens / 2;  // packed pairs of a lane's weights
-      bf16x8 weights[kTiles][3];
-      auto products = [&](int i0, int i1) {
-        unrolled<0, kO>([&](auto n) {
-          constexpr int o = decltype(n)::value;
-          const bf16x8 A = x.v.template operand<o>();
-#pragma unroll
-          for (int k = 0; k < 3; ++k)
-#pragma unroll
-            for (int i = i0; i < i1; ++i)
-              O[i][o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, weights[i][k], O[i][o], 0, 0, 0);
-        });
-      };
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        float s[kTokens], vs_i[kTokens], vl_i[kTokens];
-#pragma unroll
-        for (int j = 0; j < kTokens; ++j) {
-          float c;
-          if constexpr (kFold == 1)
-            c = S[i][j / 4][j % 4];
-          else if constexpr (kFold == 2)
-            c = fold ? S[i][1][j] : S[i][0][j];
-          else
-            c = fold & 2 ? (fold & 1 ? S[i][1][2 + j] : S[i][1][j]) : (fold & 1 ? S[i][0][2 + j] : S[i][0][j]);
-          s[j] = fmaf(kl[j], qs_rest[i], fmaf(ks[j], c, kl[j] * qs[i])) * unit[i];
-          vs_i[j] = vs[j];
-          vl_i[j] = vl[j];
-        }
-        if (cut) {
-#pragma unroll
-          for (int j = 0; j < kTokens; ++j) {
-            const int t = kFold == 1 ? j / 4 : mine, at = 16 * t + token + (kFold == 1 ? j % 4 : j);
-            const bool seen = at < limit[i] - 16 * x.tile && !(t ? x.none[1] : x.none[0]);
-            s[j] = seen ? s[j] : -INFINITY;
-            vs_i[j] = seen ? vs[j] : 0.f;
-            vl_i[j] = seen ? vl[j] : 0.f;
-          }
-        }
-        // References are whole numbers, so that moving one changes exponents only, and are moved
-        // where a weight (kOdd: or one times a value's power of two) would be larger than it may.
-        auto column_max = [](float x) {
-          if constexpr (kFold >= 2) x = fmaxf(x, row_from8(x));
-          if constexpr (kFold == 4) x = fmaxf(x, row_from4(x));
-          return wave_max16(x);
-        };
-        float mx = s[0];
-#pragma unroll
-        for (int j = 1; j < kTokens; ++j) mx = fmaxf(mx, s[j]);
-        bool late = mx > m_run[i] + kWeightLag;
-        if constexpr (kOdd) {
-#pragma unroll
-          for (int j = 0; j < kTokens; ++j)
-            late = late || s[j] - m_run[i] + (vs_log[j] - off_run[i]) > kWeightLag;
-        }
-        if (__builtin_amdgcn_ballot_w64(late)) {
-          const float m_new = fmaxf(m_run[i], ceilf(column_max(mx)));
-          const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
-          float beta = alpha;
-          l_run[i] *= alpha;
-          if constexpr (kOdd) {
-            float most = s[0] - m_new + vs_log[0];
-#pragma unroll
-            for (int j = 1; j < kTokens; ++j) most = fmaxf(most, s[j] - m_new + vs_log[j]);
-            const float old = off_run[i] + (m_run[i] - m_new);
-            off_run[i] = fmaxf(old, ceilf(column_max(most)));
-            beta = __builtin_amdgcn_exp2f(old - off_run[i]);
-          }
-          m_run[i] = m_new;
-          z[i] *= beta;
-#pragma unroll
-          for (int k = 0; k < kO; ++k) O[i][k] *= beta;
-        }
-        // Weights times scales as sums of three bf16, which is exact: the upper 8 of 24 bits, the
-        // upper 8 of the rest, and the rest of that.
-        uint32_t own[3][kWords];
-#pragma unroll
-        for (int j = 0; j < kTokens; j += 2) {
-          uint32_t y[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float d = s[j + e] - m_run[i];
-            float weight = __builtin_amdgcn_exp2f(d);
-            l_run[i] += weight;
-            if constexpr (kOdd) weight = __builtin_amdgcn_exp2f(d + (vs_log[j + e] - off_run[i]));
-            z[i] = fmaf(weight, vl_i[j + e], z[i]);
-            y[e] = __float_as_uint(weight * vs_i[j + e]);
-          }
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            own[k][j / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302);
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              y[e] = __float_as_uint(__uint_as_float(y[e]) - __uint_as_float(y[e] & 0xFFFF0000u));
-          }
-        }
-        // the other folds' tokens of the column
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          u32x4 y;
-          if constexpr (kFold == 1)
-            y = u32x4{own[k][0], own[k][1], own[k][kWords - 2], own[k][kWords - 1]};
-          else if constexpr (kFold == 2)
-            y = u32x4{own[k][0], own[k][kWords - 1], row_from<8>(own[k][0]), row_from<8>(own[k][kWords - 1])};
-          else
-            y = u32x4{own[k][0], row_from<4>(own[k][0]), row_from<8>(own[k][0]), row_from<12>(own[k][0])};
-          weights[i][k] = __builtin_bit_cast(bf16x8, y);
-        }
-        if constexpr (kOdd) products(i, i + 1);
-      }
-      if constexpr (!kOdd) products(0, kTiles);
-    };
-
-    // A pair's loads go out while the one before is worked on, and its places are read one
-    // pair earlier still.  (Past the last pair page 0 is read, so that the number of loads
-    // on the way is known.)
-    if constexpr (kOdd) {
-      for (int n = 0; n < pairs; ++n) {
-        fetch(pair[0], places(n), n);
-        consume(pair[0]);
-      }
-    } else {
-      for (int n = 0; n < pairs; n += 2) {
-        fetch(pair[1], ahead[1], n + 1);
-        ahead[0] = places(n + 2);
-        consume(pair[0]);
-        fetch(pair[0], ahead[0], n + 2);
-        ahead[1] = places(n + 3);
-        if (n + 1 < pairs) consume(pair[1]);
-      }
-    }
-
-    auto column_sum = [](float x) {
-      x = wave_sum16(x);
-      if constexpr (kFold >= 2) x += row_from8(x);
-      if constexpr (kFold == 4) x += row_from4(x);
-      return x;
-    };
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) l_run[i] = column_sum(l_run[i]), z[i] = column_sum(z[i]);
-    if constexpr (!kOdd) {
-      if (scaled) {
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          float most = 0.f;
-#pragma unroll
-          for (int k = 0; k < kO; ++k)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) most = fmaxf(most, O[i][k][r]);
-          odd |= __builtin_amdgcn_ballot_w64(wave_max16(most) < kLeastSum && l_run[i] > 0.f);
-        }
-      }
-      if (qa_lane() == 0) odd_lds[w] = odd != 0;
-      __syncthreads();
-      int any = 0;
-#pragma unroll
-      for (int i = 0; i < W; ++i) any |= odd_lds[i];
-      if (__builtin_amdgcn_readfirstlane(any)) return true;
-    }
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-      if (i) __syncthreads();  // the last tile's states are read
-      qa_finish<D, kBits, kColumns, kOdd>(p, smem, O[i], m_run[i], l_run[i], z[i], off_run[i], kTiles * ct + i, h, b,
-                                          slot);
-    }
-    return false;
-  };
-
   for (;;) {
     const int tiles = qa_tiles_of(p, len);
     const int t0 = max(from - start, 0), t1 = min(to - start, tiles);
@@ -819,7 +842,15 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
         p.ws_plan[b] = int2{slot, whole ? 1 : qa_part_of(start + tiles - 1, parts, total) + 1 - part};
       slot = whole ? -1 : slot;
     }
-    if (segment(std::false_type{}, max(len, 0), t0, t1, slot)) segment(std::true_type{}, max(len, 0), t0, t1, slot);
+    const int most = max(len, 0);
+    const bool again = qa_segment<D, kBits, kFold, kTiles, false>(p, shared, ct, h, b, most, t0, t1, slot);
+    if constexpr (qa_calls(D, kBits, kFold, kTiles)) {
+      if (again)
+        qa_segment_odd<D, kBits, kFold, kTiles>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(),
+                                                (uint32_t)(uintptr_t)&shared, ct, h, b, most, t0, t1, slot);
+    } else {
+      if (again) qa_segment<D, kBits, kFold, kTiles, true>(p, shared, ct, h, b, most, t0, t1, slot);
+    }
     start += tiles;
     if (++b >= p.batch || p.splits || (start >= to && part != parts - 1)) return;
     len = lens[b];
