@@ -4,11 +4,11 @@
 // Pair i of a token at position t turns by t w_i:
 //   y_a = f (x_a cos - x_b sin),  y_b = f (x_b cos + x_a sin)
 // with (a, b) = (2i, 2i + 1), or (i, i + n) of 2n rotated channels; the others
-// pass.  The angle is made in 64 bits (t w_i of a far position has no digits left in
-// 32) and taken into an eighth of a turn there; sine and cosine are their Taylor
-// polynomials in 64 bits, rounded once to fp32 (off by 2^-33 before), so no table
-// of positions is read.  They are made once a token and shared by its heads through
-// LDS.
+// pass.  The angle is made in two numbers of 64 bits (t w_i of a far position has no digits
+// left in 32, and of the farthest 2^-21 in 64) and taken into an eighth of a turn there;
+// sine and cosine are their Taylor polynomials in 64 bits, rounded once to fp32 (off by
+// 2^-37 before, at any position), so no table of positions is read.  They are made once a
+// token and shared by its heads through LDS.
 //
 // A workgroup takes one token, or up to four while they have no more than 64 angles, one
 // wave's work; a thread 16 bytes of both members of its pairs (of one, where they are
@@ -50,8 +50,14 @@ struct RotaryParams {
 
 // cos and sin of t w, times the factor.
 __device__ __forceinline__ float2 rotary_turn(int t, double w, double factor) {
-  const double turns = (double)t * w * 0.15915494309189533577;  // of a whole turn
-  const double frac = turns - rint(turns);
+#pragma clang fp contract(off)  // (a product taken twice has to be the same number)
+  // t w / 2 pi, of a whole turn, with what its product and 1 / 2 pi's rounding leave out: far
+  // positions have turned 2^30 times and more, and the whole turns are taken off exactly.
+  constexpr double kTurn = 0.15915494309189535, kTurnRest = -9.839338337591243e-18;
+  const double angle = t * w, angle_rest = fma((double)t, w, -angle);
+  const double turns = angle * kTurn;
+  const double turns_rest = fma(angle, kTurn, -turns) + fma(angle, kTurnRest, angle_rest * kTurn);
+  const double frac = (turns - rint(turns)) + turns_rest;
   const double quarter = rint(4.0 * frac);
   const double x = (4.0 * frac - quarter) * 1.57079632679489661923, y = x * x;
   double s = fma(y, -1.0 / 39916800, 1.0 / 362880);
