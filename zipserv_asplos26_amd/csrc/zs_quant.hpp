@@ -21,8 +21,6 @@ namespace zs {
 template <int D, int kBits>
 struct QuantRow {
   static constexpr int kBytes = D * kBits / 8;  // of a row of codes
-  static constexpr int kToken = 8 + 2 * kBytes;  // of a token
-  static constexpr int kMost = (1 << kBits) - 1;  // the last code
 };
 
 constexpr int quant_token_bytes(int head_dim, int bits) { return 8 + head_dim * bits / 4; }
