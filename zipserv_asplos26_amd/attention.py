@@ -409,10 +409,16 @@ def flash_attn_with_kvcache_quantized(q, cache, block_table, cache_seqlens, soft
     cache_seqlens - new + 1 + i, its own the last of them (cache_seqlens: int32 [B]
     or an int, the new tokens counted).  block_table: (B, max_blocks) int32.
     Scores, softmax and sums are fp32 over the cache's values low + code * scale,
-    which are not rounded first.  Returns out shaped like q (and softmax_lse [B,
-    H], or [B, H, new] for a q of four dimensions, when asked); a row that sees no
-    token gives zeros and lse -inf.  num_splits cuts each sequence's tokens alike, 0 by
-    the size of the call."""
+    which are not rounded first, and may be of any size that an append makes (|q| at most
+    2^100).  Returns out shaped like q (and softmax_lse [B, H], or [B, H, new] for a q
+    of four dimensions, when asked); a row that sees no token gives zeros and lse -inf.
+
+    num_splits cuts each sequence's tokens alike, 0 by the lengths, so that workgroups
+    have as much to do each; a large batch, of 6 (sequence, KV head, 16 of its rows) a CU
+    and more (192 sequences with 8 KV heads), is not cut then, and if one of its
+    sequences is much longer than the others a few num_splits (8) are faster.  A part
+    of a sequence whose values are too small, too large or too unlike for one pass in
+    fp32 takes about twice as long."""
     torch = _torch()
     shape = q.shape if isinstance(q, torch.Tensor) else ()
     paged._check(q, "q", torch.bfloat16, (None,) * (4 if len(shape) == 4 else 3), contiguous=False)

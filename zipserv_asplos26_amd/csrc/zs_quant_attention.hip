@@ -32,11 +32,11 @@
 // of only a half of its tokens (4 or fewer: a quarter) and gets the other weights from
 // the lanes that did them.
 //
-// What bounds it: 64 sequences' 8000 tokens (64 / 8 heads of 128 in 4 bits, 557 MB) take 106
-// us, 5.3 TB/s, where a kernel that only reads them takes 98; with 16 columns and more
-// the vector instructions do (three tiles of columns over 113 MB: 64 us, reading
-// alone 37); one sequence's 32000 tokens 13 us and 4 for the merge, start, loads and
-// merge being a chain of latencies.
+// What bounds it: 64 sequences' 8000 tokens (64 / 8 heads of 128 in 4 bits, 557 MB) take 107
+// us, 5.2 TB/s, with the vector unit at work in half of the cycles; with 16 columns and
+// more the vector instructions do (three tiles of columns over 113 MB: 67 us); one
+// sequence's 32000 tokens 13.5 us and 4 for the merge, start, loads and merge being a chain
+// of latencies.  A part that is done a second time takes 1.5 to 2.3 times as long.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -80,13 +80,12 @@ struct QuantAttnParams {
 constexpr int kQaWaves = 4;
 // A column's largest weight so far is 1, or up to 2^4 before the reference moves (small, so that
 // the argument of a weight's exponential has few digits before its point).  Scales of values go
-// in times 2^kScaleUp, so that weight * scale times a code in units of 2^kCodeUnit is
-// 2^-33 of what it stands for: 2^-63 for the largest weight and a scale of 2^-30, 63
+// in times kScaleFactor, so that weight * scale times a code in units of 2^kCodeUnit is
+// 1 / kSumFactor of what it stands for: 2^-63 for the largest weight and a scale of 2^-30, 63
 // bits above the least normal number, while scales up to 2^22 leave sums of 2^31 room.
 constexpr float kWeightLag = 4.f;
-constexpr int kScaleUp = 100;
-constexpr float kScaleFactor = 0x1p100f;  // 2^kScaleUp
-constexpr float kSumFactor = 0x1p33f;  // 2^-(kCodeUnit + kScaleUp)
+constexpr float kScaleFactor = 0x1p100f;
+constexpr float kSumFactor = 0x1p33f;  // 2^-kCodeUnit / kScaleFactor
 // Whether that was enough is seen from a column's largest sum of such products: below the one
 // (small scales, or none with the large weights) digits may be lost, above the other (or
 // with a sum of lows above kSumFactor times that) a sum may have left fp32.
@@ -232,7 +231,7 @@ __device__ __forceinline__ void unrolled(F&& f) {
 // starts at tile floor(i T / P) of the T.  What it has of a sequence that it does not
 // have whole goes into slot 2 i, or 2 i + 1 where the sequence starts inside the part (a
 // part has one at most that ends, and one that starts, outside it).
-constexpr int kLeastChunk = 16;  // tiles of a part (one sequence of 2000 tokens: 13.7 us with 32, 11.8 with 16)
+constexpr int kLeastChunk = 16;  // tiles of a part (one sequence of 2000 tokens: 14.3 us with 32, 12.5 with 16)
 
 __device__ __forceinline__ int qa_tiles_of(const QuantAttnParams& p, int len) {
   return (int)min(((int64_t)max(len, 0) + 15) / 16, (int64_t)p.width * p.tiles.d);
@@ -746,13 +745,16 @@ __device__ __forceinline__ bool qa_segment(const QuantAttnParams& p, QaShared<D,
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
     if (i) __syncthreads();  // the last tile's states are read
-    qa_finish<D, kBits, kColumns, kOdd>(p, shared.states, O[i], m_run[i], l_run[i], off_run[i], kTiles * ct + i, h, b, slot);
+    qa_finish<D, kBits, kColumns, kOdd>(p, shared.states, O[i], m_run[i], l_run[i], off_run[i], kTiles * ct + i, h, b,
+                                        slot);
   }
   return false;
 }
 
 // Whether the second time is a function of its own.  Where both together need more registers than
-// there are it is the main loop that loses them; where not, a call's rules cost more.
+// there are it is the main loop that loses them (64 sequences of 8000 tokens: 116 us, 110 with
+// a call; five new tokens of 16 sequences 73 and 70); where not, a call's rules cost more (heads
+// of 64 in 8 bits, 20 ragged sequences: 30 us, 36 with a call).
 constexpr bool qa_calls(int dim, int bits, int fold, int tiles) {
   return dim == 128 && (tiles > 1 || (bits == 4 && fold <= 2));
 }
@@ -765,10 +767,10 @@ __device__ __attribute__((noinline)) void qa_segment_odd(uint64_t params, uint32
   typedef QaShared<D, kBits, kTiles> __attribute__((address_space(3))) * Shared;
   auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   const uint64_t at = (uint64_t)(uint32_t)uniform((int)(params >> 32)) << 32 | (uint32_t)uniform((int)params);
-  qa_segment<D, kBits, kFold, kTiles, true>(*(const QuantAttnParams*)(Params)at,
-                                            *(QaShared<D, kBits, kTiles>*)(Shared)(uintptr_t)uniform(shared), uniform(ct),
-                                            uniform(h), uniform(b), uniform(len), uniform(t0), uniform(t1),
-                                            uniform(slot));
+  const Shared states = (Shared)(uintptr_t)uniform(shared);
+  qa_segment<D, kBits, kFold, kTiles, true>(*(const QuantAttnParams*)(Params)at, *(QaShared<D, kBits, kTiles>*)states,
+                                            uniform(ct), uniform(h), uniform(b), uniform(len), uniform(t0),
+                                            uniform(t1), uniform(slot));
 }
 
 // kTiles tiles of columns in one workgroup: codes are loaded and widened once for all.  With
@@ -860,17 +862,22 @@ __global__ __launch_bounds__(kQaWaves * 64, qa_waves(D, kBits, kFold, kTiles)) v
 
 // How a call is cut.  Where num_splits leaves it open: sequences whole where the table
 // holds no more than kWholeTiles (the merge costs 4 us: 1000 tokens of one sequence take
-// 11 us whole, 11.7 in parts), or where there are six (sequence, KV head, column
-// tile) units a CU, which even out by themselves; else into parts, as many as registers
-// allow at once, two to four workgroups a CU (one less or one more costs 2 to 30%: 20
-// ragged sequences of 8000 tokens with 64 heads of 128 in 8 bits take 38 us in two a CU, 43 in
-// three), but 64 a sequence at most (32000 tokens: 17.0 us in 96, 16.3 in 64).
+// 11.8 us whole, 12.2 in parts, 1500 15.1 and 12.5), or where there are six (sequence, KV
+// head, column tile) units a CU; else into parts, as many as registers allow at once, two
+// to four workgroups a CU (one less or one more costs up to 30%: 20 ragged sequences of
+// 8000 tokens with 64 heads of 128 in 8 bits take 38 us in two a CU, 45 in three), but 64
+// a sequence at most (32000 tokens: 19.1 us in 96, 17.1 in 64).
+// The six units even out where lengths are spread evenly (256 sequences of 2000 tokens with
+// 8 KV heads: 109 us whole, 127 in parts; of 16 to 4000 tokens 108 and 184), but the host
+// does not see the lengths, and one sequence much longer than the others is then one
+// workgroup's work a KV head: 255 sequences of 500 tokens and one of 64000 take 388 us,
+// with num_splits = 8 157; 190 and one, which are cut by their lengths, 59.
 constexpr int kWholeTiles = 64;
 // Tiles of columns go two to a workgroup where none or few are left over, and in 8 bits
 // of 128 channels always.  Sixteen sequences of 8000 tokens, heads of 128, one tile
-// against two a workgroup: two tiles 55 and 49 us (8 bits 75 and 58), three 71 and 77 (8
-// bits 98 and 83; heads of 64 57 and 62), four 93 and 79 (8 bits 118 and 89); four
-// sequences of 4000 tokens with 32 tiles 97 and 73.
+// against two a workgroup: two tiles 59 and 55 us (8 bits 75 and 63), three 74 and 84 (8
+// bits 116 and 93; heads of 64 59 and 67), four 94 and 85 (8 bits 118 and 96), seven 163
+// and 143; four sequences of 4000 tokens with 32 tiles 104 and 83.
 constexpr int kOddTiles = 7;
 struct QaCut {
   int64_t columns, column_tiles;  // the latter: of `tiles` times 16 columns

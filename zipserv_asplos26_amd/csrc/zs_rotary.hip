@@ -13,8 +13,8 @@
 // A workgroup takes one token, or up to four while they have no more than 64 angles, one
 // wave's work; a thread 16 bytes of both members of its pairs (of one, where they are
 // neighbours) at a time, written past the caches.  HBM bounds it: 8192 tokens of 40 heads of
-// 128 in bf16 take 26.2 us, 168 MB at 6.4 TB/s, some of it from the last-level cache (28.5
-// in workgroups of 256 threads and four tokens); one token 3.4 us, launch and latency.
+// 128 in bf16 take 26.0 us, 168 MB at 6.5 TB/s, some of it from the last-level cache (28.5
+// in workgroups of 256 threads and four tokens); one token 3.2 us, launch and latency.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
