@@ -628,7 +628,8 @@ int zs_paged_read_quant(void* stream, const uint8_t* cache, int num_blocks, int 
  * num_splits = 0 cuts a batch by its lengths, n > 0 every sequence into n parts (of
  * 128 tokens or more); the workspace (16-byte aligned) is what the query says for
  * the same arguments.  batch * num_heads * new_tokens is below 2^31.  Scores, weights
- * and sums have the digits of fp32 for rows of any size that an append makes; where values
+ * and sums have the digits of fp32 for rows of any size that an append makes (a channel's
+ * sum to 2^-60 of the largest channel's at least); where values
  * are so small, so large or so unlike that sums would leave fp32, or no number, that part
  * of the sequence takes about twice as long.  |q| is at most 2^100, no scale is negative or
  * infinite, no low infinite (an append makes none).  With num_splits = 0 a batch of 6

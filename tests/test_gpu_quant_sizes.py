@@ -215,3 +215,43 @@ def test_pools_without_a_value(torch_cuda, group, new, dim, bits):
             for b, length in enumerate(lens):
                 want = math.log(length - new + 1 + i) if length - new + 1 + i > 0 else -math.inf
                 assert (lse[b, :, i] == want).all() or (lse[b, :, i] - want).abs().max() <= 2.0 ** -22 * max(want, 1)
+
+
+@pytest.mark.parametrize("group,new,dim,bits", SHAPES)
+def test_captured_passes_over_changing_rows(torch_cuda, group, new, dim, bits):
+    # one captured call, replayed as rows of a part become unusual and ordinary again, with two streams' calls between
+    T = torch_cuda
+    lens, page, width = [1100, 333, 64, 0], 16, 70
+    q, data, table, g = make(T, 43, 4, new, 2 * group, 2, dim, page, width, bits)
+    pools = [data.copy() for _ in range(4)]
+    values_of(T, "2^60", sides(pools[1], page), bits, g)
+    for block in table[0, 40:45].tolist():
+        sides(pools[3], page)[block, :, ::2, 2:] = 0, 0x7180  # flat rows of 2^100
+    wants = [attend(q, x, table, lens, page, bits) for x in pools]
+    cache = paged.QuantizedKVCache(T.from_numpy(data).cuda(), page, dim, bits)
+    qd, tab, n = q.cuda(), table.cuda(), T.tensor(lens, dtype=T.int32, device="cuda")
+
+    def call():
+        return attention.flash_attn_with_kvcache_quantized(qd, cache, tab, n, return_softmax_lse=True)
+
+    call()
+    T.cuda.synchronize()
+    graph = T.cuda.CUDAGraph()
+    with T.cuda.graph(graph):
+        out, lse = call()
+    streams = [T.cuda.Stream() for _ in range(2)]
+    for turn in (0, 1, 2, 3, 1, 0):
+        cache.data.copy_(T.from_numpy(pools[turn]))
+        graph.replay()
+        T.cuda.synchronize()
+        others = []
+        for s in streams:
+            with T.cuda.stream(s):
+                others.append(call())
+        T.cuda.synchronize()
+        want, want_lse, tol, lse_tol = wants[turn]
+        seen = want_lse > -math.inf
+        assert ((out.cpu().double() - want).abs() <= tol).all(), turn
+        assert ((lse.cpu().double() - want_lse).abs() <= lse_tol)[seen].all(), turn
+        for o, l in others:
+            assert T.equal(o, out) and T.equal(l, lse), turn
